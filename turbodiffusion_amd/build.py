@@ -20,8 +20,9 @@ LIB = os.path.join(HERE, "libturbodiffusion_amd.so")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 # -fno-slp-vectorize: hipcc otherwise packs adjacent fp32 adds/FMAs into v_pk_*_f32, which measured ~4x
 # slower than the plain forms beside MFMAs on gfx950 (the GEMM dequant segments: 600 -> ~300 cycles)
+# -packed-fp32-ops: no v_pk_{add,mul,fma}_f32 from float pairs either (wrong results seen from some of their forms on gfx950)
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=off", "-fno-slp-vectorize",
-         "-Wno-unused-result"]
+         "-Wno-unused-result", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 
 def sources():
