@@ -1,0 +1,84 @@
+"""Host side of the packed operators: the work tables replayed row by row, and refusals that need no GPU."""
+import ctypes
+import random
+
+import pytest
+import torch
+
+from turbodiffusion_amd import _lib as L
+from turbodiffusion_amd import ops, packed
+
+
+def attention_table(lq, lk, heads, kv_heads, causal):
+    a, b, c = packed._i64_array(lq), packed._i64_array(lk), (ctypes.c_int64 * 6)()
+    L.call("td_attn_packed_plan", a, b, len(lq), heads, kv_heads, causal, None, 0, c)
+    n = sum(c[:3])
+    t = torch.full((n + 1, 8), -7, dtype=torch.int32)
+    L.call("td_attn_packed_plan", a, b, len(lq), heads, kv_heads, causal, ctypes.c_void_p(t.data_ptr()), n, c)
+    assert (t[n] == -7).all()
+    return t[:n].tolist(), list(c)
+
+
+@pytest.mark.parametrize("seed", range(8))
+def test_attention_plan_covers_every_visible_key_once(seed):
+    rng = random.Random(seed)
+    for _ in range(25):
+        ns, kv = rng.randint(0, 6), rng.choice([1, 2, 3])
+        G = rng.choice([1, 2, 5, 40])
+        lq = [rng.choice([0, 1, 2, 31, 33, 127, 129, 300]) for _ in range(ns)]
+        lk = [rng.choice([0, 1, 63, 64, 65, 128, 700, 5000]) for _ in range(ns)]
+        causal = rng.randint(0, 1)
+        t, (tiles, few, joins, ws_rows, tq, tk) = attention_table(lq, lk, kv * G, kv, causal)
+        assert (tq, tk) == (sum(lq), sum(lk))
+        starts = {}
+        for s in range(ns):
+            if lq[s]:
+                starts[sum(lq[:s])] = s
+        seen = {}
+        for i, (qb, kb, ql, kl, row0, a, b, slot) in enumerate(t[:tiles + few]):
+            s = starts[qb]
+            assert (kb, ql, kl) == (sum(lk[:s]), lq[s], lk[s]) and 0 <= a <= b <= kl
+            for row in range(row0, min(row0 + (128 if i < tiles else 32), ql * G)):
+                seen.setdefault((s, row), []).append((a, b, slot))
+        for s in range(ns):
+            for row in range(lq[s] * G):
+                end = min(lk[s], max(0, row // G + lk[s] - lq[s] + 1)) if causal else lk[s]
+                parts, at = sorted(seen.pop((s, row))), 0
+                for a, b, slot in parts:
+                    assert a == at and (slot >= 0) == (len(parts) > 1)
+                    at = b
+                assert end <= at <= lk[s]
+        assert not seen
+        slots = [j[4] + i * j[6] for j in t[tiles + few:] for i in range(j[5])]
+        rows = [x + r for j in t[tiles + few:] for x in range(j[4], j[4] + j[5] * j[6], j[6]) for r in range(j[6])]
+        assert sorted(slots) == sorted(x[7] for x in t[:tiles + few] if x[7] >= 0)
+        assert len(set(rows)) == len(rows) and (not rows or max(rows) < ws_rows)
+
+
+def test_attention_plan_refusals():
+    with pytest.raises(ValueError):
+        ops.AttentionPlan([3, 4], [3], heads=2)
+    with pytest.raises(ValueError):
+        ops.AttentionPlan([3], heads=5, kv_heads=2)
+    with pytest.raises(ValueError):
+        ops.AttentionPlan([3], heads=2, head_dim=96)
+    with pytest.raises(ValueError):
+        ops.AttentionPlan([2.5], heads=2)
+    with pytest.raises(ValueError):
+        ops.AttentionPlan(torch.tensor([2.0]), heads=2)
+    with pytest.raises(L.TurboDiffusionAMDError):
+        ops.AttentionPlan([-1], heads=2)
+    with pytest.raises(L.TurboDiffusionAMDError):
+        ops.AttentionPlan([1 << 31], heads=2)
+    with pytest.raises(L.TurboDiffusionAMDError):
+        ops.AttentionPlan([1 << 30, 1 << 30], heads=2)
+    with pytest.raises(ValueError):
+        ops.AttentionPlan([3], heads=2, device="cpu")
+
+
+def test_attention_refuses_cpu_tensors():
+    class Plan:
+        heads, kv_heads, head_dim = 2, 2, 64
+    q = torch.zeros(3, 2, 64, dtype=torch.bfloat16)
+    with pytest.raises(L.TurboDiffusionAMDError):
+        ops.packed_attention(q, q, q, Plan())

@@ -1,0 +1,519 @@
+// Attention over packed sequences: the tokens of many requests stand behind one another without padding,
+//
+//     o[i, h] = sum_j p_ij v[j, h / G],   p_i = softmax_j( scale q[i, h] . k[j, h / G] + bias[h, clamp(j - pos_i, -R, R)] ),
+//     pos_i = i + k_len - q_len  (the queries are the LAST q_len positions of their sequence),  j <= pos_i when causal,
+//
+// with G = heads / kv_heads query heads per key / value head, D = 64 or 128, bf16 or f16.  A row with nothing to attend to is 0.
+//
+// One pass over the keys with a running maximum and sum per row (fp32, exp2 domain).  Rows: the G query heads that share a key
+// head are rows of ONE tile (row r of a sequence = query r / G, head kvh * G + r % G), so a key tile is read once for all of
+// them and a single new token still fills G rows.  Both products are issued transposed, S^T = K Q^T and O^T = V^T P^T: a lane
+// owns one row, its maximum / sum / rescale are lane-local but for one exchange with lane ^ 32.  The K rows enter the first MFMA
+// in the order (bits 2 and 3 of the row swapped) in which its result registers are the second one's B operand: P never leaves
+// the registers.  V^T fragments come from the row-major V tile by the transposing LDS read.
+//
+// Two kernels, by rows of a sequence:
+//   tile  128 rows per workgroup, 32 per wave, key tiles of 64 shared by the four waves (LDS-DMA, two stages);
+//   few   <= 32 rows (new tokens, short prompts): the four waves take different keys, each with its own two LDS stages and no
+//         barrier in the loop, and join at the end through LDS.
+// Where there are too few workgroups for the chip the key range is split over several and joined by a third kernel.
+// P is rounded to the operands' 16-bit type for the second product (half a step, relative, of every weight: the errors of
+// independent weights average out below the output's own rounding); sums and statistics stay fp32.
+#include "td_common.h"
+#include <algorithm>
+#include <math.h>
+#include <vector>
+
+typedef __attribute__((address_space(3))) void* ap_lptr_t;
+typedef short ap_v4s __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) ap_v4s* ap_trptr_t;
+
+#define AP_ROWS 128        // rows of a tile item
+#define AP_FEW 32          // rows of a few item
+#define AP_TAU 8.0f        // the reference maximum moves only when exceeded by 2^8: P <= 256 fits f16 / bf16 and the fp32 sum
+
+struct ApItem {            // one workgroup's work per key head: rows [row0, ..) of a sequence over keys [key0, key1)
+  int32_t q_begin, k_begin, q_len, k_len, row0, key0, key1, slot;   // slot: row in the partial buffer, -1 = writes o
+};
+struct ApJoin { int32_t q_begin, q_len, row0, rows, slot, splits, tile_rows, pad; };
+
+struct ApParams {
+  const uint16_t *q, *k, *v; uint16_t* o;
+  int64_t q_ts, q_hs, k_ts, k_hs, v_ts, v_hs, o_ts, o_hs;   // token / head strides, elements
+  const float* bias; int R;                                  // [H, 2R + 1] or null
+  const ApItem* items;
+  float* po; float* pml; int64_t ws_rows;                    // partials [Hkv][ws_rows][D], [Hkv][ws_rows][2] (max, sum)
+  int Hkv, G, causal;
+  float c;                                                   // scale * log2(e)
+};
+
+template <int DT> struct ap_mma;
+template <> struct ap_mma<TD_F16> {
+  __device__ static __forceinline__ v16f run(v4i a, v4i b, v16f c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0, 0);
+  }
+};
+template <> struct ap_mma<TD_BF16> {
+  __device__ static __forceinline__ v16f run(v4i a, v4i b, v16f c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), c, 0, 0, 0);
+  }
+};
+
+__device__ __forceinline__ float ap_other_half(float x, bool mx) {   // x of this lane (+ | max) x of lane ^ 32
+  const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  const float a = __uint_as_float(s[0]), b = __uint_as_float(s[1]);
+  return mx ? fmaxf(a, b) : a + b;
+}
+
+// Tiles in LDS: row-major, rows of 2 D bytes, the 16-byte chunks of a row permuted by an XOR so that the reads touch every
+// bank once (K: ds_read_b128 by 16 lanes of 16 different rows; V: 4 rows x 64 bytes twice per transposing read)
+template <int D> __device__ __forceinline__ uint32_t ap_kx(uint32_t row) { return D == 128 ? (row & 15u) : ((row >> 1) & 7u); }
+template <int D> __device__ __forceinline__ uint32_t ap_vx(uint32_t row) { return D == 128 ? 4u * (row & 3u) : 4u * ((row >> 1) & 1u); }
+
+// 64 lanes x 16 bytes from base + off (a lane each) to LDS, lane after lane; `bytes` bounds the offsets
+__device__ __forceinline__ void ap_dma(const void* base, uint32_t bytes, char* lds, uint32_t off) {
+  const auto r = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, (int)bytes, 0x00020000);
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (ap_lptr_t)lds, 16, off, 0, 0, 0);
+}
+
+template <int DT, int D, bool FEW, bool BIAS>
+__global__ __launch_bounds__(256, FEW ? 1 : 2) void attn_packed_kernel(const ApParams p) {
+  constexpr int NB = FEW && D == 128 ? 1 : 2;       // 32-key blocks per tile
+  constexpr int BK = 32 * NB;
+  constexpr int ROWB = 2 * D;
+  constexpr int TILE = BK * ROWB;                   // bytes of a K or V tile
+  constexpr int STAGE = 2 * TILE;
+  constexpr int PIECES = TILE / 1024 / (FEW ? 1 : 4);   // 1 KB LDS-DMA pieces per wave, K and V each
+  constexpr int RPP = 1024 / ROWB;                  // rows per piece
+  constexpr int KK = D / 16, DB = D / 32;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int kvh = blockIdx.x % p.Hkv;
+  const ApItem it = p.items[blockIdx.x / p.Hkv];
+  float* const lbias = reinterpret_cast<float*>(smem + (FEW ? 8 : 2) * STAGE);
+
+  // ---- this lane's row ----
+  const int nrows = it.q_len * p.G;
+  const int wrow0 = it.row0 + (FEW ? 0 : 32 * wave);
+  const int row = wrow0 + (lane & 31);
+  const bool valid = row < nrows;
+  const int rc = min(row, nrows - 1);
+  const int qi = rc / p.G, g = rc - qi * p.G;
+  const int shift = it.k_len - it.q_len;
+  const int pos = qi + shift;
+  const int kmax = p.causal ? min(it.key1, pos + 1) : it.key1;         // keys [key0, kmax) of this row
+  // the tile's last row sees most keys, the wave's first row fewest
+  const int last = min(it.row0 + (FEW ? AP_FEW : AP_ROWS), nrows) - 1;
+  const int key_end = p.causal ? min(it.key1, last / p.G + shift + 1) : it.key1;
+  const int wfirst = min(wrow0, nrows - 1) / p.G + shift, wlast = min(wrow0 + 31, nrows - 1) / p.G + shift;   // positions
+  const int wmin = p.causal ? min(it.key1, wfirst + 1) : it.key1;
+  const int wmax = wrow0 >= nrows ? 0 : (p.causal ? min(it.key1, wlast + 1) : it.key1);
+
+  // ---- Q^T fragments: B operand, lane = row, 8 consecutive d per register quad ----
+  v4i qf[KK];
+  {
+    const uint16_t* qp = p.q + (int64_t)(it.q_begin + qi) * p.q_ts + (int64_t)(kvh * p.G + g) * p.q_hs + 8 * half;
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk) qf[kk] = *reinterpret_cast<const v4i*>(qp + 16 * kk);
+  }
+  if constexpr (BIAS) {   // exp2 domain; the type's lowest values as a finite low (a row of nothing else stays a uniform row)
+    const int n = p.G * (2 * p.R + 1);
+    const float* b = p.bias + (int64_t)kvh * n;
+    for (int i = tid; i < n; i += 256) {
+      const float x = b[i];
+      lbias[i] = fabsf(x) > 1e37f && fabsf(x) < INFINITY ? copysignf(1e37f, x) : x * 1.4426950408889634f;
+    }
+    __syncthreads();
+  }
+  const float* const lb = lbias + (BIAS ? g * (2 * p.R + 1) + p.R : 0);
+  const float b_far_past = BIAS ? lb[-p.R] : 0.f, b_far_next = BIAS ? lb[p.R] : 0.f;
+
+  // ---- LDS-DMA: piece t of this wave; rows past the range re-read the last one (finite, masked) ----
+  const int drow = lane / (ROWB / 16), dchunk = lane & (ROWB / 16 - 1);
+  uint32_t koff[PIECES], voff[PIECES];
+  auto piece_row = [&](int t) { return RPP * (FEW ? t : wave + 4 * t) + drow; };
+#pragma unroll
+  for (int t = 0; t < PIECES; ++t) {
+    const uint32_t r = piece_row(t);
+    koff[t] = r * (uint32_t)(2 * p.k_ts) + ((dchunk ^ ap_kx<D>(r)) << 4);
+    voff[t] = r * (uint32_t)(2 * p.v_ts) + ((dchunk ^ ap_vx<D>(r)) << 4);
+  }
+  const uint16_t* const kbase = p.k + (int64_t)it.k_begin * p.k_ts + (int64_t)kvh * p.k_hs;
+  const uint16_t* const vbase = p.v + (int64_t)it.k_begin * p.v_ts + (int64_t)kvh * p.v_hs;
+  char* const mystage = smem + (FEW ? wave * 2 * STAGE : 0);
+  auto fetch = [&](int kt, int buf) {
+    const int nv = min(it.key1 - kt, BK);
+    const uint16_t* kp = kbase + (int64_t)kt * p.k_ts;
+    const uint16_t* vp = vbase + (int64_t)kt * p.v_ts;
+    const uint32_t kbytes = (uint32_t)((nv - 1) * 2 * p.k_ts + ROWB), vbytes = (uint32_t)((nv - 1) * 2 * p.v_ts + ROWB);
+    char* st = mystage + buf * STAGE + (FEW ? 0 : wave * 1024);
+    constexpr int STEP = FEW ? 1024 : 4096;
+    if (nv == BK) {
+#pragma unroll
+      for (int t = 0; t < PIECES; ++t)
+        ap_dma(kp, kbytes, st + t * STEP, koff[t]);
+#pragma unroll
+      for (int t = 0; t < PIECES; ++t)
+        ap_dma(vp, vbytes, st + TILE + t * STEP, voff[t]);
+    } else {
+#pragma unroll
+      for (int t = 0; t < PIECES; ++t) {
+        const uint32_t r = piece_row(t), rcl = min((int)r, nv - 1);
+        const uint32_t ko = rcl * (uint32_t)(2 * p.k_ts) + ((dchunk ^ ap_kx<D>(r)) << 4);
+        const uint32_t vo = rcl * (uint32_t)(2 * p.v_ts) + ((dchunk ^ ap_vx<D>(r)) << 4);
+        ap_dma(kp, kbytes, st + t * STEP, ko);
+        ap_dma(vp, vbytes, st + TILE + t * STEP, vo);
+      }
+    }
+  };
+
+  // ---- fragment addresses ----
+  const uint32_t kr = (lane & 19) | ((lane & 4) << 1) | ((lane & 8) >> 1);      // bits 2 and 3 of the row swapped
+  const uint32_t krow = kr * ROWB, kxor = (half ^ ap_kx<D>(kr)) << 4;
+  const uint32_t i16 = lane & 15;
+  const uint32_t vkey = 8 * half + (i16 >> 2);
+  const uint32_t vrow = vkey * ROWB + ((((lane >> 4) & 1) * 2 + ((i16 & 3) >> 1)) << 4) + (i16 & 1) * 8;
+  const uint32_t vxor = ap_vx<D>(vkey) << 4;                                    // a multiple of 64: moves whole 32-d blocks
+
+  v16f acc[DB];
+#pragma unroll
+  for (int d = 0; d < DB; ++d)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) acc[d][r] = 0.f;
+  float m = -INFINITY, mref = 0.f, l = 0.f;
+
+  const int step = FEW ? 4 * BK : BK;
+  int kt = it.key0 + (FEW ? wave * BK : 0);
+  const int kend = key_end;
+  if (kt < kend) fetch(kt, 0);
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  if constexpr (!FEW) __syncthreads();
+  for (int buf = 0; kt < kend; kt += step, buf ^= 1) {
+    if (kt + step < kend) fetch(kt + step, buf ^ 1);
+    if (FEW || kt < wmax) {
+      const char* sk = mystage + buf * STAGE;
+      const char* sv = sk + TILE;
+      v16f s[NB];
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[b][r] = 0.f;
+#pragma unroll
+        for (int kk = 0; kk < KK; ++kk) {
+          const v4i kf = *reinterpret_cast<const v4i*>(sk + b * 32 * ROWB + krow + (kxor ^ (kk << 5)));
+          s[b] = ap_mma<DT>::run(kf, qf[kk], s[b]);
+        }
+      }
+      // register r of block b is key kt + 32 b + 16 (r >> 3) + 8 half + (r & 7)
+      if constexpr (BIAS) {
+        float far = 0.f; bool isfar = false;
+        if (kt - wlast >= p.R) { far = b_far_next; isfar = true; }
+        else if (kt + BK - 1 - wfirst <= -p.R) { far = b_far_past; isfar = true; }
+        const int d0 = kt + 8 * half - pos;
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            float bb = far;
+            if (!isfar) bb = lb[max(-p.R, min(p.R, d0 + 32 * b + 16 * (r >> 3) + (r & 7)))];
+            s[b][r] = fmaf(s[b][r], p.c, bb);
+          }
+      }
+      if (kt + BK > wmin) {
+        const int lim = kmax - kt - 8 * half;
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[b][r] = 32 * b + 16 * (r >> 3) + (r & 7) < lim ? s[b][r] : -INFINITY;
+      }
+      float mx = s[0][0];
+#pragma unroll
+      for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[b][r]);
+      mx = ap_other_half(mx, true);
+      if constexpr (!BIAS) mx *= p.c;
+      if (__any(mx > m + AP_TAU)) {
+        const float mn = fmaxf(m, mx);
+        mref = mn == -INFINITY ? 0.f : mn;
+        const float alpha = __builtin_amdgcn_exp2f(m - mref);
+        m = mn;
+        l *= alpha;
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) acc[d][r] *= alpha;
+      }
+      uint32_t pk[NB][8];
+#pragma unroll
+      for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int r = 0; r < 16; r += 2) {
+          const float e0 = __builtin_amdgcn_exp2f(BIAS ? s[b][r] - mref : fmaf(s[b][r], p.c, -mref));
+          const float e1 = __builtin_amdgcn_exp2f(BIAS ? s[b][r + 1] - mref : fmaf(s[b][r + 1], p.c, -mref));
+          l += e0 + e1;
+          pk[b][r >> 1] = pack2<DT>(e0, e1);
+        }
+#pragma unroll
+      for (int t = 0; t < 2 * NB; ++t) {
+        const uint32_t* w = &pk[t >> 1][4 * (t & 1)];
+        const v4i pf = {(int)w[0], (int)w[1], (int)w[2], (int)w[3]};
+#pragma unroll
+        for (int d = 0; d < DB; ++d) {
+          const char* a = sv + t * 16 * ROWB + vrow + ((d << 6) ^ vxor);
+          const ap_v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ap_trptr_t)a);
+          const ap_v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ap_trptr_t)(a + 4 * ROWB));
+          const v8s vf = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+          acc[d] = ap_mma<DT>::run(__builtin_bit_cast(v4i, vf), pf, acc[d]);
+        }
+      }
+    }
+    // this tile's reads have returned and the next tile has landed (FEW: the stages are this wave's own)
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    if constexpr (!FEW) __syncthreads();
+  }
+  l = ap_other_half(l, false);
+
+  // ---- results.  acc[d][r] is d = 32 d + 8 (r >> 2) + 4 half + (r & 3) of this lane's row ----
+  if constexpr (FEW) {   // join the four waves through LDS
+    constexpr int LD = D + 4;
+    float* jo = reinterpret_cast<float*>(smem);                 // [4][32][LD]
+    float* jm = jo + 4 * 32 * LD;                               // [4][32][2]
+    __syncthreads();
+    float* mo = jo + (wave * 32 + (lane & 31)) * LD;
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; r += 4)
+        *reinterpret_cast<float4*>(mo + 32 * d + 2 * r + 4 * half) = make_float4(acc[d][r], acc[d][r + 1], acc[d][r + 2], acc[d][r + 3]);
+    if (half == 0) { jm[(wave * 32 + lane) * 2] = m; jm[(wave * 32 + lane) * 2 + 1] = l; }
+    __syncthreads();
+    constexpr int W = D / 8;                                    // d per thread
+    const int jr = tid >> 3, d0 = (tid & 7) * W;
+    const int r2 = it.row0 + jr;
+    if (r2 < nrows) {
+      float mm = -INFINITY, ll = 0.f, oo[W];
+#pragma unroll
+      for (int w = 0; w < 4; ++w) mm = fmaxf(mm, jm[(w * 32 + jr) * 2]);
+      const float mr = mm == -INFINITY ? 0.f : mm;
+#pragma unroll
+      for (int e = 0; e < W; ++e) oo[e] = 0.f;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const float a = __builtin_amdgcn_exp2f(jm[(w * 32 + jr) * 2] - mr);
+        ll += a * jm[(w * 32 + jr) * 2 + 1];
+#pragma unroll
+        for (int e = 0; e < W; e += 4) {
+          const float4 x = *reinterpret_cast<const float4*>(jo + (w * 32 + jr) * LD + d0 + e);
+          oo[e] += a * x.x; oo[e + 1] += a * x.y; oo[e + 2] += a * x.z; oo[e + 3] += a * x.w;
+        }
+      }
+      if (it.slot >= 0) {
+        const int64_t pr = (int64_t)kvh * p.ws_rows + it.slot + jr;
+#pragma unroll
+        for (int e = 0; e < W; e += 4)
+          *reinterpret_cast<float4*>(p.po + pr * D + d0 + e) = make_float4(oo[e], oo[e + 1], oo[e + 2], oo[e + 3]);
+        if (d0 == 0) { p.pml[pr * 2] = mm; p.pml[pr * 2 + 1] = ll; }
+      } else {
+        const float inv = ll == 0.f ? 0.f : 1.0f / ll;
+        const int q2 = r2 / p.G, g2 = r2 - q2 * p.G;
+        uint16_t* op = p.o + (int64_t)(it.q_begin + q2) * p.o_ts + (int64_t)(kvh * p.G + g2) * p.o_hs + d0;
+#pragma unroll
+        for (int e = 0; e < W; ++e) oo[e] *= inv;
+#pragma unroll
+        for (int e = 0; e < W; e += 8) *reinterpret_cast<uint4*>(op + e) = pack8<DT>(oo + e);
+      }
+    }
+  } else {
+    if (!valid) return;
+    if (it.slot >= 0) {
+      const int64_t pr = (int64_t)kvh * p.ws_rows + it.slot + 32 * wave + (lane & 31);
+#pragma unroll
+      for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; r += 4)
+          *reinterpret_cast<float4*>(p.po + pr * D + 32 * d + 2 * r + 4 * half) = make_float4(acc[d][r], acc[d][r + 1], acc[d][r + 2], acc[d][r + 3]);
+      if (half == 0) { p.pml[pr * 2] = m; p.pml[pr * 2 + 1] = l; }
+    } else {
+      const float inv = l == 0.f ? 0.f : 1.0f / l;
+      uint16_t* op = p.o + (int64_t)(it.q_begin + qi) * p.o_ts + (int64_t)(kvh * p.G + g) * p.o_hs + 8 * half;
+#pragma unroll
+      for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int r = 8 * j;
+          const uint32_t a0 = pack2<DT>(acc[d][r] * inv, acc[d][r + 1] * inv), a1 = pack2<DT>(acc[d][r + 2] * inv, acc[d][r + 3] * inv);
+          const uint32_t b0 = pack2<DT>(acc[d][r + 4] * inv, acc[d][r + 5] * inv), b1 = pack2<DT>(acc[d][r + 6] * inv, acc[d][r + 7] * inv);
+          const auto s0 = __builtin_amdgcn_permlane32_swap(a0, b0, false, false);
+          const auto s1 = __builtin_amdgcn_permlane32_swap(a1, b1, false, false);
+          *reinterpret_cast<uint4*>(op + 32 * d + 16 * j) = make_uint4(s0[0], s1[0], s0[1], s1[1]);
+        }
+    }
+  }
+}
+
+// one wave per row: the splits of a row, weighted by exp2(max - common max)
+template <int DT, int D>
+__global__ __launch_bounds__(256) void attn_packed_join_kernel(const ApParams p, const ApJoin* joins) {
+  constexpr int E = D / 64;
+  const ApJoin j = joins[blockIdx.x];
+  const int kvh = blockIdx.y, lane = threadIdx.x & 63;
+  const int r = blockIdx.z * 4 + (threadIdx.x >> 6);
+  if (r >= j.rows) return;
+  const int64_t base = (int64_t)kvh * p.ws_rows + j.slot + r;
+  float mm = -INFINITY, ll = 0.f, o[E];
+  for (int s = 0; s < j.splits; ++s) mm = fmaxf(mm, p.pml[(base + (int64_t)s * j.tile_rows) * 2]);
+  const float mr = mm == -INFINITY ? 0.f : mm;
+#pragma unroll
+  for (int e = 0; e < E; ++e) o[e] = 0.f;
+  for (int s = 0; s < j.splits; ++s) {
+    const int64_t pr = base + (int64_t)s * j.tile_rows;
+    const float a = __builtin_amdgcn_exp2f(p.pml[pr * 2] - mr);
+    ll += a * p.pml[pr * 2 + 1];
+#pragma unroll
+    for (int e = 0; e < E; ++e) o[e] += a * p.po[pr * D + lane * E + e];
+  }
+  const float inv = ll == 0.f ? 0.f : 1.0f / ll;
+  const int row = j.row0 + r, qi = row / p.G, g = row - qi * p.G;
+  uint16_t* op = p.o + (int64_t)(j.q_begin + qi) * p.o_ts + (int64_t)(kvh * p.G + g) * p.o_hs + lane * E;
+  if constexpr (E == 2) *reinterpret_cast<uint32_t*>(op) = pack2<DT>(o[0] * inv, o[1] * inv);
+  else *op = (uint16_t)pack2<DT>(o[0] * inv, 0.f);
+}
+
+// ---- the plan: which workgroup does what (host) --------------------------------------------------------------------
+// Table of 8-word records: tile items, few items, joins (in this order).  counts = {tile items, few items, joins, partial rows,
+// query tokens, key tokens}.
+extern "C" int td_attn_packed_plan(const int64_t* lens_q, const int64_t* lens_k, int64_t nseq, int heads, int kv_heads, int causal,
+                                   int32_t* table, int64_t capacity, int64_t* counts) {
+  TD_REQUIRE(lens_q && lens_k && counts && nseq >= 0, TD_ERR_INVALID, "td_attn_packed_plan: null pointer or %lld sequences", (long long)nseq);
+  TD_REQUIRE(kv_heads > 0 && heads > 0 && heads % kv_heads == 0, TD_ERR_INVALID, "td_attn_packed_plan: %d heads over %d key heads", heads, kv_heads);
+  const int64_t G = heads / kv_heads, MAXT = 1ll << 30;
+  int64_t tq = 0, tk = 0;
+  for (int64_t s = 0; s < nseq; ++s) {
+    TD_REQUIRE(lens_q[s] >= 0 && lens_k[s] >= 0 && lens_q[s] <= MAXT && lens_k[s] <= MAXT, TD_ERR_INVALID,
+               "td_attn_packed_plan: sequence %lld has lengths %lld, %lld", (long long)s, (long long)lens_q[s], (long long)lens_k[s]);
+    tq += lens_q[s]; tk += lens_k[s];
+    TD_REQUIRE(tq <= MAXT && tk <= MAXT && tq * G <= MAXT, TD_ERR_UNSUPPORTED, "td_attn_packed_plan: more than 2^30 rows");
+  }
+  try {
+    struct Work { ApItem it; int64_t keys; };
+    std::vector<Work> work[2];
+    std::vector<ApJoin> joins;
+    int64_t keys_total[2] = {0, 0};
+    // pass 0 counts the keys each kernel reads, pass 1 emits items of at most `chunk` keys
+    int64_t chunk[2] = {0, 0}, ws_rows = 0;
+    for (int pass = 0; pass < 2; ++pass) {
+      int64_t q0 = 0, k0 = 0;
+      for (int64_t s = 0; s < nseq; ++s) {
+        const int64_t ql = lens_q[s], kl = lens_k[s], rows = ql * G;
+        const int few = rows <= AP_FEW;
+        const int64_t tr = few ? AP_FEW : AP_ROWS;
+        for (int64_t r0 = 0; r0 < rows; r0 += tr) {
+          const int64_t last = std::min(r0 + tr, rows) - 1;
+          const int64_t end = causal ? std::max<int64_t>(0, std::min(kl, last / G + kl - ql + 1)) : kl;
+          if (pass == 0) { keys_total[few] += end; continue; }
+          const int64_t parts = std::max<int64_t>(1, td_cdiv(end, chunk[few]));
+          const int64_t quantum = few ? 128 : 64;
+          const int64_t per = td_cdiv(td_cdiv(std::max<int64_t>(end, 1), parts), quantum) * quantum;
+          const int64_t n = std::max<int64_t>(1, td_cdiv(end, per));
+          if (n > 1) joins.push_back({(int32_t)q0, (int32_t)ql, (int32_t)r0, (int32_t)(last - r0 + 1), (int32_t)ws_rows, (int32_t)n, (int32_t)tr, 0});
+          for (int64_t i = 0; i < n; ++i) {
+            const int64_t a = i * per, b = std::min(end, a + per);
+            work[few].push_back({{(int32_t)q0, (int32_t)k0, (int32_t)ql, (int32_t)kl, (int32_t)r0, (int32_t)a, (int32_t)b,
+                                  n > 1 ? (int32_t)(ws_rows + i * tr) : -1}, b - a});
+          }
+          if (n > 1) ws_rows += n * tr;
+          TD_REQUIRE(ws_rows <= MAXT, TD_ERR_UNSUPPORTED, "td_attn_packed_plan: more than 2^30 partial rows");
+        }
+        q0 += ql; k0 += kl;
+      }
+      if (pass == 0) {
+        // 256 CUs.  A key range is split when the whole work is less than two full rounds of workgroups of the longest
+        // range; a part is at least 512 keys (few: 256), below which writing and joining partials costs more than it saves.
+        chunk[0] = std::max<int64_t>(512, td_cdiv(keys_total[0] * kv_heads, 1024));
+        chunk[1] = std::max<int64_t>(256, td_cdiv(keys_total[1] * kv_heads, 512));
+      }
+    }
+    for (auto& w : work)   // longest first: the short ones fill the tail
+      std::stable_sort(w.begin(), w.end(), [](const Work& a, const Work& b) { return a.keys > b.keys; });
+    counts[0] = (int64_t)work[0].size(); counts[1] = (int64_t)work[1].size(); counts[2] = (int64_t)joins.size();
+    counts[3] = ws_rows; counts[4] = tq; counts[5] = tk;
+    const int64_t n = counts[0] + counts[1] + counts[2];
+    if (table) {
+      TD_REQUIRE(capacity >= n, TD_ERR_INVALID, "td_attn_packed_plan: table of %lld records, %lld needed", (long long)capacity, (long long)n);
+      ApItem* t = reinterpret_cast<ApItem*>(table);
+      for (auto& w : work) for (auto& x : w) *t++ = x.it;
+      for (auto& j : joins) *reinterpret_cast<ApJoin*>(t++) = j;
+    }
+  } catch (const std::bad_alloc&) {
+    td_set_error("td_attn_packed_plan: out of host memory");
+    return TD_ERR_INVALID;
+  }
+  return TD_OK;
+}
+
+template <int DT, int D, bool FEW, bool BIAS>
+static void ap_launch(const ApParams& p, int64_t n, int bias_bytes, hipStream_t st) {
+  static std::atomic<uint64_t> mask{0};
+  constexpr int NB = FEW && D == 128 ? 1 : 2;
+  const int tiles = (FEW ? 8 : 2) * 2 * 32 * NB * 2 * D;
+  td_ensure_dyn_lds((const void*)attn_packed_kernel<DT, D, FEW, BIAS>, tiles + 32768, mask);
+  attn_packed_kernel<DT, D, FEW, BIAS><<<(unsigned)(n * p.Hkv), 256, tiles + bias_bytes, st>>>(p);
+}
+
+extern "C" int td_attn_packed(const void* q, int64_t q_ts, int64_t q_hs, const void* k, int64_t k_ts, int64_t k_hs, const void* v,
+                              int64_t v_ts, int64_t v_hs, void* o, int64_t o_ts, int64_t o_hs, int dtype, int heads, int kv_heads,
+                              int head_dim, float scale, int causal, const float* bias, int bias_range, const int32_t* table,
+                              const int64_t* counts, float* ws, td_stream_t stream) {
+  TD_REQUIRE(q && o && counts && table, TD_ERR_INVALID, "td_attn_packed: null pointer");
+  TD_REQUIRE(dtype == TD_BF16 || dtype == TD_F16, TD_ERR_UNSUPPORTED, "td_attn_packed: dtype %d", dtype);
+  TD_REQUIRE(head_dim == 64 || head_dim == 128, TD_ERR_UNSUPPORTED, "td_attn_packed: head_dim = %d (64 or 128)", head_dim);
+  TD_REQUIRE(kv_heads > 0 && heads > 0 && heads % kv_heads == 0, TD_ERR_INVALID, "td_attn_packed: %d heads over %d key heads", heads, kv_heads);
+  const int64_t st_[8] = {q_ts, q_hs, k_ts, k_hs, v_ts, v_hs, o_ts, o_hs};
+  for (int64_t s : st_) TD_REQUIRE(s >= 0 && s % 8 == 0, TD_ERR_UNSUPPORTED, "td_attn_packed: stride %lld (a multiple of 8 elements)", (long long)s);
+  TD_REQUIRE(k_ts < (1 << 24) && v_ts < (1 << 24), TD_ERR_UNSUPPORTED, "td_attn_packed: key / value token stride of 2^24 elements or more");
+  TD_REQUIRE((((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)o | (uintptr_t)ws) & 15) == 0, TD_ERR_UNSUPPORTED,
+             "td_attn_packed: pointers must be 16-byte aligned");
+  TD_REQUIRE(scale > 0.f && scale <= 3.0e38f, TD_ERR_INVALID, "td_attn_packed: scale must be positive and finite");
+  const int64_t nt = counts[0], nf = counts[1], nj = counts[2], wr = counts[3];
+  TD_REQUIRE(nt >= 0 && nf >= 0 && nj >= 0 && wr >= 0 && (nj == 0 || ws), TD_ERR_INVALID, "td_attn_packed: counts / workspace");
+  TD_REQUIRE(counts[5] == 0 || (k && v), TD_ERR_INVALID, "td_attn_packed: null keys or values");
+  TD_REQUIRE(nt * kv_heads < (1ll << 31) && nf * kv_heads < (1ll << 31) && nj < (1ll << 31) && kv_heads <= 65535, TD_ERR_UNSUPPORTED,
+             "td_attn_packed: more than 2^31 workgroups");
+  const int G = heads / kv_heads;
+  int bias_bytes = 0;
+  if (bias) {
+    TD_REQUIRE(bias_range >= 0 && bias_range < 8192 && (int64_t)G * (2 * bias_range + 1) * 4 <= 32768, TD_ERR_UNSUPPORTED,
+               "td_attn_packed: bias of range %d for %d heads per key head exceeds 32 KB", bias_range, G);
+    bias_bytes = G * (2 * bias_range + 1) * 4;
+  }
+  ApParams p;
+  p.q = (const uint16_t*)q; p.k = (const uint16_t*)k; p.v = (const uint16_t*)v; p.o = (uint16_t*)o;
+  p.q_ts = q_ts; p.q_hs = q_hs; p.k_ts = k_ts; p.k_hs = k_hs; p.v_ts = v_ts; p.v_hs = v_hs; p.o_ts = o_ts; p.o_hs = o_hs;
+  p.bias = bias; p.R = bias_range; p.items = reinterpret_cast<const ApItem*>(table);
+  p.po = ws; p.pml = ws ? ws + (int64_t)kv_heads * wr * head_dim : nullptr; p.ws_rows = wr;
+  p.Hkv = kv_heads; p.G = G; p.causal = causal ? 1 : 0;
+  p.c = scale * 1.4426950408889634f;
+  hipStream_t st = (hipStream_t)stream;
+  for (int few = 0; few < 2; ++few) {
+    const int64_t n = few ? nf : nt;
+    p.items = reinterpret_cast<const ApItem*>(table) + (few ? nt : 0);
+    if (n == 0) continue;
+#define AP_GO2(DT_, D_, F_) { if (bias) ap_launch<DT_, D_, F_, true>(p, n, bias_bytes, st); else ap_launch<DT_, D_, F_, false>(p, n, 0, st); }
+#define AP_GO1(DT_, D_) { if (few) AP_GO2(DT_, D_, true) else AP_GO2(DT_, D_, false) }
+    if (dtype == TD_BF16) { if (head_dim == 64) AP_GO1(TD_BF16, 64) else AP_GO1(TD_BF16, 128) }
+    else { if (head_dim == 64) AP_GO1(TD_F16, 64) else AP_GO1(TD_F16, 128) }
+#undef AP_GO1
+#undef AP_GO2
+    TD_CHECK_LAUNCH();
+  }
+  if (nj > 0) {
+    const ApJoin* joins = reinterpret_cast<const ApJoin*>(table) + nt + nf;
+    const dim3 grid((unsigned)nj, (unsigned)kv_heads, (nt > 0 ? AP_ROWS : AP_FEW) / 4);
+    if (dtype == TD_BF16) { if (head_dim == 64) attn_packed_join_kernel<TD_BF16, 64><<<grid, 256, 0, st>>>(p, joins); else attn_packed_join_kernel<TD_BF16, 128><<<grid, 256, 0, st>>>(p, joins); }
+    else { if (head_dim == 64) attn_packed_join_kernel<TD_F16, 64><<<grid, 256, 0, st>>>(p, joins); else attn_packed_join_kernel<TD_F16, 128><<<grid, 256, 0, st>>>(p, joins); }
+    TD_CHECK_LAUNCH();
+  }
+  return TD_OK;
+}

@@ -11,8 +11,10 @@ import torch
 import torch.nn as nn
 
 from . import kernels as K
+from .packed import AttentionPlan, packed_attention
 
-__all__ = ["int8_quant", "int8_linear", "rmsnorm", "layernorm", "Int8Linear", "FastRMSNorm", "FastLayerNorm"]
+__all__ = ["int8_quant", "int8_linear", "rmsnorm", "layernorm", "Int8Linear", "FastRMSNorm", "FastLayerNorm",
+           "AttentionPlan", "packed_attention"]
 
 
 def int8_quant(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
