@@ -82,3 +82,69 @@ def test_attention_refuses_cpu_tensors():
     q = torch.zeros(3, 2, 64, dtype=torch.bfloat16)
     with pytest.raises(L.TurboDiffusionAMDError):
         ops.packed_attention(q, q, q, Plan())
+
+
+@pytest.mark.parametrize("seed", range(4))
+def test_adapter_plan_takes_every_row_once(seed):
+    rng = random.Random(seed)
+    for _ in range(40):
+        ns = rng.randint(0, 9)
+        lens = [rng.choice([0, 1, 2, 63, 64, 65, 300]) for _ in range(ns)]
+        ids = [rng.randint(-1, 3) for _ in range(ns)]
+        a, b, c = packed._i64_array(lens), packed._i64_array(ids), (ctypes.c_int64 * 5)()
+        L.call("td_lora_plan", a, b, ns, None, 0, c)
+        n = 4 * (c[0] + c[1]) + c[2]
+        t = torch.full((n + 1,), -7, dtype=torch.int32)
+        L.call("td_lora_plan", a, b, ns, ctypes.c_void_p(t.data_ptr()), n, c)
+        assert t[n] == -7
+        t = t.tolist()
+        owner = [i for m, i in zip(lens, ids) for _ in range(m)]
+        assert list(c)[2:] == [len(owner), sum(i >= 0 for i in owner), max(ids, default=-1) + 1]
+        perm, seen = t[4 * (c[0] + c[1]):n], []
+        for j in range(c[0] + c[1]):
+            p0, rows, adapter, _ = t[4 * j:4 * j + 4]
+            assert 1 <= rows <= 64 and (adapter >= 0) == (j < c[0])
+            if adapter >= 0:
+                assert p0 + rows <= c[3]           # rows of the fp32 workspace
+            assert all(owner[r] == adapter for r in perm[p0:p0 + rows])
+            seen += perm[p0:p0 + rows]
+        assert sorted(seen) == list(range(len(owner)))
+
+
+def test_adapter_refusals():
+    a, b = torch.zeros(4, 16, dtype=torch.bfloat16), torch.zeros(24, 4, dtype=torch.bfloat16)
+    with pytest.raises(ValueError):
+        ops.AdapterPlan([3], [0, 1])
+    with pytest.raises(L.TurboDiffusionAMDError):
+        ops.AdapterPlan([3], [-2])
+    with pytest.raises(L.TurboDiffusionAMDError):
+        ops.AdapterPlan([-3], [0])
+    with pytest.raises(ValueError):
+        ops.AdapterBank([])
+    with pytest.raises(ValueError):
+        ops.AdapterBank([(a, b)], scales=[1.0, 2.0])
+    with pytest.raises(ValueError):
+        ops.AdapterBank([(a, b)], scales=[float("nan")])
+    with pytest.raises(TypeError):
+        ops.AdapterBank([(a.float(), b.float())])
+    with pytest.raises(TypeError):
+        ops.AdapterBank([(a, b), (a.half(), b.half())])
+    with pytest.raises(ValueError):
+        ops.AdapterBank([(a, b[:, :3])])
+    with pytest.raises(ValueError):
+        ops.AdapterBank([(a[:, :12], b)])
+    with pytest.raises(ValueError):
+        ops.AdapterBank([(a, b)], device="cpu")
+
+
+def test_adapter_workspace_of_every_plan():
+    """no rows with an adapter need no workspace; otherwise at least one fp32 part of every such row"""
+    for tiles, rows in ((0, 0), (1, 1), (3, 150), (511, 511 * 64), (600, 600 * 64)):
+        c = (ctypes.c_int64 * 5)(tiles, 0, rows, rows, 1)
+        for k in (8, 64, 4096, 10240):
+            for rank in (8, 16, 24, 256):
+                out = ctypes.c_int64(-1)
+                L.call("td_lora_workspace", c, k, rank, ctypes.byref(out))
+                assert out.value == 0 if rows == 0 else out.value >= rows * rank
+    with pytest.raises(L.TurboDiffusionAMDError):
+        L.call("td_lora_workspace", c, 64, 257, ctypes.byref(out))

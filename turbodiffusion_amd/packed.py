@@ -158,3 +158,131 @@ def packed_attention(q, k, v, plan, scale=None, bias=None, out=None):
         call("td_attn_packed", ptr(q), *qs, ptr(k), *ks, ptr(v), *vs, ptr(out), *os_, dt_code(q.dtype), H, Hkv, D, scale,
              1 if plan.causal else 0, ptr(bias), R, ptr(plan.table), plan._counts, ptr(ws), plan.use())
     return out
+
+
+class AdapterBank:
+    """Low-rank pairs for ONE projection, laid out once: ``pairs[i]`` = (A [rank, k], B [n, rank]), all bf16 or all f16, ranks of
+    1 to 256 that may differ; ``scales[i]`` (default 1) multiplies the update (the usual alpha / rank)."""
+
+    MAX_RANK = 256
+
+    def __init__(self, pairs, scales=None, device="cuda"):
+        pairs = list(pairs)
+        if not pairs:
+            raise ValueError("AdapterBank: no adapters")
+        scales = [1.0] * len(pairs) if scales is None else [float(s) for s in scales]
+        if len(scales) != len(pairs):
+            raise ValueError(f"AdapterBank: {len(pairs)} adapters, {len(scales)} scales")
+        if not all(math.isfinite(s) for s in scales):
+            raise ValueError(f"AdapterBank: scales must be finite, got {scales}")
+        self.dtype = pairs[0][0].dtype
+        if self.dtype not in (torch.bfloat16, torch.float16):
+            raise TypeError(f"AdapterBank: bf16 or f16 adapters, got {self.dtype}")
+        self.k, self.n = pairs[0][0].shape[-1], pairs[0][1].shape[0]
+        if self.k % 8 or self.n % 8 or not self.k or not self.n:
+            raise ValueError(f"AdapterBank: k = {self.k}, n = {self.n} must be positive multiples of 8")
+        for i, (a, b) in enumerate(pairs):
+            if a.dim() != 2 or b.dim() != 2 or a.shape[1] != self.k or b.shape != (self.n, a.shape[0]):
+                raise ValueError(f"AdapterBank: adapter {i} is {tuple(a.shape)} / {tuple(b.shape)}, wanted [rank, {self.k}] / [{self.n}, rank]")
+            if a.dtype != self.dtype or b.dtype != self.dtype:
+                raise TypeError(f"AdapterBank: adapter {i} is {a.dtype} / {b.dtype}, the first {self.dtype}")
+            if not 1 <= a.shape[0] <= self.MAX_RANK:
+                raise ValueError(f"AdapterBank: adapter {i} has rank {a.shape[0]} (1 to {self.MAX_RANK})")
+        self.device = torch.device(device)
+        if self.device.type != "cuda":
+            raise ValueError(f"AdapterBank: the operators run on a GPU, got device {device!r}")
+        if self.device.index is None:
+            self.device = torch.device("cuda", torch.cuda.current_device())
+        self.ranks = [a.shape[0] for a, _ in pairs]
+        r8 = [-(-r // 8) * 8 for r in self.ranks]
+        self.max_rank = max(r8)
+        with _guard(self.device):
+            self.data = torch.zeros(sum(r * (self.k + self.n) for r in r8), dtype=self.dtype, device=self.device)
+            meta = torch.zeros(len(pairs), 3, dtype=torch.int64)
+            off = 0
+            for i, ((a, b), r, r_) in enumerate(zip(pairs, self.ranks, r8)):
+                oa, ob = off, off + r_ * self.k
+                off = ob + self.n * r_
+                self.data[oa:ob].view(r_, self.k)[:r] = a.detach()
+                self.data[ob:off].view(self.n, r_)[:, :r] = b.detach()
+                meta[i, 0], meta[i, 1] = oa, ob
+                words = meta[i, 2:].view(torch.int32)
+                words[0] = r_
+                words.view(torch.float32)[1] = scales[i]
+            self.meta = meta.to(self.device)
+        torch.cuda.current_stream(self.device).synchronize()      # laid out once, complete for every stream
+
+    def __len__(self):
+        return len(self.ranks)
+
+
+class AdapterPlan(_Plan):
+    """The work of ``lora_add`` for packed requests of ``lens`` rows, request i with adapter ``ids[i]`` (-1: none)."""
+
+    def __init__(self, lens, ids, device="cuda"):
+        self.lens, self.ids = _lengths(lens, "AdapterPlan lens"), _lengths(ids, "AdapterPlan ids")
+        if len(self.lens) != len(self.ids):
+            raise ValueError(f"AdapterPlan: {len(self.lens)} lengths, {len(self.ids)} adapter ids")
+        args = (_i64_array(self.lens), _i64_array(self.ids), len(self.lens))
+        self._counts = (ctypes.c_int64 * 5)()
+        L.call("td_lora_plan", *args, None, 0, self._counts)
+        n = 4 * (self._counts[0] + self._counts[1]) + self._counts[2]
+        host = torch.zeros(max(1, n), dtype=torch.int32)
+        L.call("td_lora_plan", *args, ptr(host), n, self._counts)
+        self.rows = self._counts[2]
+        self._ws = {}
+        self._upload(host, device)
+
+    def workspace(self, k, max_rank):
+        """f32 elements a call needs"""
+        n = self._ws.get((k, max_rank))
+        if n is None:
+            out = ctypes.c_int64()
+            L.call("td_lora_workspace", self._counts, k, max_rank, ctypes.byref(out))
+            n = self._ws[(k, max_rank)] = out.value
+        return n
+
+
+def _rows(t, rows, cols, what):
+    if t.dim() != 2 or tuple(t.shape) != (rows, cols):
+        raise ValueError(f"lora_add: {what} is {tuple(t.shape)}, wanted ({rows}, {cols})")
+    if t.stride(1) != 1:
+        raise ValueError(f"lora_add: the last dimension of {what} must be contiguous")
+    return t.stride(0) if rows > 1 else 0
+
+
+def lora_add(y, x, bank, plan, out=None):
+    """y [rows, n] + the adapters' updates of x [rows, k] (row stride: any multiple of 8 elements) -> [rows, n]: row r of a request
+    with adapter i becomes y[r] + scale_i * (x[r] A_i^T) B_i^T, one without stays y[r].  ``y`` is the output of the projection that
+    all requests share (``int8_linear``, ``Int8Linear``, a 16-bit GEMM).  ``out``: written instead of a new tensor; ``out=y`` adds
+    in place; any other overlap is refused.  x A^T is summed in fp32 and, scaled, rounded once to the adapters' type; the update
+    is added in fp32 and rounded with the result.  Any stream, capturable; bank and plan must outlive a captured graph."""
+    require_gpu(y, x, out)
+    _no_grad_inputs(y, x)
+    dev = plan.device
+    if any(t is not None and t.device != dev for t in (y, x, out, bank.data)):
+        raise ValueError(f"lora_add: bank, plan and every tensor must be on one device ({dev})")
+    if x.dtype != bank.dtype or y.dtype != bank.dtype:
+        raise TypeError(f"lora_add: x is {x.dtype}, y {y.dtype}, the adapters {bank.dtype}")
+    if plan._counts[4] > len(bank):
+        raise ValueError(f"lora_add: the plan names adapter {plan._counts[4] - 1}, the bank holds {len(bank)}")
+    ldx, ldy = _rows(x, plan.rows, bank.k, "x"), _rows(y, plan.rows, bank.n, "y")
+    if out is None:
+        out = torch.empty((plan.rows, bank.n), dtype=y.dtype, device=dev)
+        ldo = bank.n
+    else:
+        if out.dtype != y.dtype:
+            raise TypeError(f"lora_add: out is {out.dtype}, y {y.dtype}")
+        ldo = _rows(out, plan.rows, bank.n, "out")
+        if plan.rows > 1 and ldo < bank.n:
+            raise ValueError("lora_add: out overlaps itself")
+        if _overlap(out, x) or (_overlap(out, y) and (out.data_ptr() != y.data_ptr() or ldo != ldy)):
+            raise ValueError("lora_add: out overlaps an input (out=y alone may)")
+    if plan.rows == 0:
+        return out
+    with _guard(dev):
+        n = plan.workspace(bank.k, bank.max_rank)
+        ws = torch.empty(n, dtype=torch.float32, device=dev) if n else None
+        call("td_lora_add", ptr(x), ldx, ptr(y), ldy, ptr(out), ldo, dt_code(y.dtype), bank.k, bank.n, ptr(bank.data), ptr(bank.meta),
+             len(bank), bank.max_rank, ptr(plan.table), plan._counts, ptr(ws), plan.use())
+    return out
