@@ -524,11 +524,15 @@ int td_attn_packed(const void* q, int64_t q_ts, int64_t q_hs, const void* k, int
 /* ---- low-rank adapters of many requests (csrc/lora.hip) ----
  * out[r] = y[r] + scale_i B_i (A_i x[r]) for rows r of a request with adapter i; out[r] = y[r] for one without (id -1; not touched
  * when out == y).  x [rows, k], y / out [rows, n]: 16-bit, row strides in elements (multiples of 8; k, n too), 16-byte aligned.
- * bank: every A_i [rank8, k] and B_i [n, rank8] back to back, rank8 = the rank rounded up to 8, padded with zeros; adapters:
- * num_adapters records {int64 offset of A_i, int64 offset of B_i (elements), int32 rank8, f32 scale}; both on the device, trusted.
+ * bank: every adapter in fragment order (td_lora_pack): 32 ceil(k / 32) rank8 elements for A_i [rank, k], 32 ceil(n / 32) rank8 for
+ * B_i [n, rank], rank8 = the rank rounded up to 8; adapters: num_adapters records {int64 offset of A_i, int64 offset of B_i
+ * (elements), int32 rank8, f32 scale}; both on the device, trusted; the bank ends with 16384 spare elements of any content, which
+ * are read and not used.  max_rank: the largest rank8 (at most 256).
  * td_lora_plan (host only): lengths and adapter ids of the requests -> counts = {tiles with an adapter, tiles without, rows, rows
- * with an adapter, largest id + 1} and, with table != NULL, 4 (tiles with + without) + rows int32 words, which go to the device
- * unchanged.  td_lora_workspace: f32 elements of ws.  max_rank: the bank's largest rank8 (at most 256). */
+ * with an adapter, largest id + 1, rows per tile} and, with table != NULL, 4 (tiles with + without) + rows int32 words, which go to
+ * the device unchanged.  td_lora_workspace: f32 elements of ws. */
+int td_lora_pack(const void* a, int64_t lda, const void* b, int64_t ldb, int rank, int64_t k, int64_t n, void* bank_a, void* bank_b,
+                 td_stream_t stream);
 int td_lora_plan(const int64_t* lens, const int64_t* ids, int64_t nseq, int32_t* table, int64_t capacity, int64_t* counts);
 int td_lora_workspace(const int64_t* counts, int64_t k, int max_rank, int64_t* floats);
 int td_lora_add(const void* x, int64_t ldx, const void* y, int64_t ldy, void* out, int64_t ldo, int dtype, int64_t k, int64_t n,

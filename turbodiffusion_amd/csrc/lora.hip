@@ -3,32 +3,34 @@
 //     out[r] = y[r] + s_i B_i (A_i x[r]),    i = the adapter of row r's request;  rows without one: out[r] = y[r]
 //
 // x [rows, K], y / out [rows, N], A_i [rank_i, K], B_i [N, rank_i], 16-bit.  The rows are taken adapter by adapter (a permutation
-// made by the plan), in tiles of 64 of one adapter, so an adapter is read for all of its rows at once however its requests lie.
+// made by the plan), in tiles of one adapter, so an adapter is read for all of its rows at once however its requests lie.
 //
-//   shrink   S = A_i x:  fp32, MFMA 16x16x32 straight from global memory (x streams; A_i comes from L2).
-//            Many tiles: a wave owns 16 rows.  Few tiles: the four waves of a workgroup share 16 rows and split K, and K is split
-//            over workgroups too; expand adds the parts in order.
+//   shrink   S = A_i x by MFMA 16x16x32, fp32.  x streams from memory straight into fragments.
 //   expand   out = y + B_i (s_i S): S is scaled in fp32 and rounded once to the operands' type (half a step of the update only:
 //            it stays below the rounding of the output wherever the update is not many times larger than the output itself).
-//            A lane ends with 8 consecutive columns of one row: 16-byte reads of y and writes of out, 64 bytes of a row together.
-// Memory-bound: y and out dominate, then x; 2 rank flops per byte of them.
+// A wave works on 32 rows.  WIDE tiles (many rows): 128 rows, 32 per wave, the waves share the adapter through the CU's L1.  Narrow
+// tiles: 32 rows; shrink's waves split K, and K is split over workgroups too (expand adds the fp32 parts in order), expand's waves
+// split the columns.
+// The bank holds A and B in fragment order (td_lora_pack): every load of them is a contiguous kilobyte, ranks are padded to 8
+// only.  Memory-bound: y and out dominate, then x; 2 rank flops per byte of them.
 #include "td_common.h"
 #include <algorithm>
 #include <new>
 #include <vector>
 
-#define LR_TILE 64
+#define LR_WIDE 128
+#define LR_NARROW 32
 #define LR_MAX_RANK 256
 
 struct LoraTile { int32_t perm0, rows, adapter, pad; };
-struct LoraAdapter { int64_t a_off, b_off; int32_t rank8; float scale; };   // offsets in elements; rank rounded up to 8 (zero rows / columns)
+struct LoraAdapter { int64_t a_off, b_off; int32_t rank8; float scale; };   // offsets in elements; rank rounded up to 8 (zeros)
 
 struct LoraParams {
   const uint16_t *x, *y; uint16_t* out;
   int64_t ldx, ldy, ldo;
   const uint16_t* bank; const LoraAdapter* adapters;
   const LoraTile* tiles; const int32_t* perm;
-  float* s;                 // [splits][rows][RS]
+  void* s;                  // splits == 1: 16-bit, scaled [rows][RS]; else f32 parts [splits][rows][RS]
   int64_t rows, K, N;
   int splits, steps;        // K splits over workgroups, K steps of 32 per split
   int ntile;                // columns per workgroup of expand
@@ -46,71 +48,234 @@ template <> struct lr_mma<TD_BF16> {
   }
 };
 
-// RJ: 16-rank blocks of the largest adapter; KS: the waves split K
-template <int DT, int RJ, bool KS>
+// Fragment order of one adapter, r8 = its padded rank:
+//   A: [K / 32][rank][4 k-quads][8 k]: the fragment of ranks 16 j .. and K step s is the kilobyte at 32 r8 s + 512 j
+//   B: [N / 32][rank / 32][2 column sets b][rank quads (4, fewer in the last)][16 rows i][8 ranks], row i of set b = column
+//      8 (i >> 2) + 4 b + (i & 3): after both sets a lane holds 8 consecutive columns of one x row
+__global__ __launch_bounds__(256) void lora_pack_kernel(const uint16_t* a, int64_t lda, const uint16_t* b, int64_t ldb, int rank, int r8,
+                                                        int64_t K, int64_t N, uint16_t* da, uint16_t* db) {
+  const int64_t na = (K + 31) / 32 * 4 * r8, nb = (N + 31) / 32 * 4 * r8;       // 16-byte pieces
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < na + nb; i += (int64_t)gridDim.x * 256) {
+    uint16_t* d; const uint16_t* src = nullptr; int valid = 0;
+    if (i < na) {
+      const int64_t s = i / (4 * r8);
+      const int w = (int)(i - s * 4 * r8), r = w >> 2;
+      const int64_t k = 32 * s + 8 * (w & 3);
+      d = da + 8 * i;
+      if (r < rank && k < K) { src = a + r * lda + k; valid = 8; }
+    } else {
+      const int64_t j = i - na, pb = j / (4 * r8);
+      int w = (int)(j - pb * 4 * r8);
+      const int kk = w / 128;
+      w -= kk * 128;
+      const int nq = min(4, r8 / 8 - 4 * kk), bs = w / (16 * nq);
+      w -= bs * 16 * nq;
+      const int q = w >> 4, l = w & 15;
+      const int64_t n = 32 * pb + 8 * (l >> 2) + 4 * bs + (l & 3);
+      const int r0 = 32 * kk + 8 * q;
+      d = db + 8 * j;
+      if (n < N && r0 < rank) { src = b + n * ldb + r0; valid = min(8, rank - r0); }
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) d[e] = e < valid ? src[e] : (uint16_t)0;
+  }
+}
+
+// K steps [s0, s1) of 32 rows, ranks [0, 16 NJ) of one adapter.  No load sits behind a branch: the last fragment of a rank that is
+// no multiple of 16 brings ranks of whatever lies behind it in the bank (it ends with a spare kilobyte), which nothing reads.
+template <int DT, int NJ, int RJ>
+__device__ __forceinline__ void lr_shrink(v4f (&acc)[2][RJ], const uint16_t* x0, const uint16_t* x1, const uint16_t* ap, int64_t astep,
+                                          int s0, int s1, int64_t K, int lq) {
+  constexpr int U = NJ <= 2 ? 8 : NJ <= 4 ? 4 : 2;
+  const int full = min(s1, (int)(K / 32));
+  int s = s0;
+  for (; s + U <= full; s += U) {
+    v4i xf[U][2], af[U][NJ];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      xf[u][0] = *reinterpret_cast<const v4i*>(x0 + 32 * (int64_t)(s + u));
+      xf[u][1] = *reinterpret_cast<const v4i*>(x1 + 32 * (int64_t)(s + u));
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) af[u][j] = *reinterpret_cast<const v4i*>(ap + (s + u) * astep + 512 * j);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) {
+        acc[0][j] = lr_mma<DT>::run(af[u][j], xf[u][0], acc[0][j]);
+        acc[1][j] = lr_mma<DT>::run(af[u][j], xf[u][1], acc[1][j]);
+      }
+  }
+  const v4i zero = {0, 0, 0, 0};
+  for (; s < s1; ++s) {
+    const bool in = 32 * (int64_t)s + 8 * lq < K;
+    const v4i xf0 = in ? *reinterpret_cast<const v4i*>(x0 + 32 * (int64_t)s) : zero;
+    const v4i xf1 = in ? *reinterpret_cast<const v4i*>(x1 + 32 * (int64_t)s) : zero;
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) {
+      const v4i af = *reinterpret_cast<const v4i*>(ap + s * astep + 512 * j);
+      acc[0][j] = lr_mma<DT>::run(af, xf0, acc[0][j]);
+      acc[1][j] = lr_mma<DT>::run(af, xf1, acc[1][j]);
+    }
+  }
+}
+
+// RJ: 16-rank blocks of the largest adapter (1, 2, 4, 8, 16); an adapter takes the smallest of these that holds its rank
+template <int DT, int RJ, bool WIDE>
 __global__ __launch_bounds__(256) void lora_shrink_kernel(const LoraParams p) {
   constexpr int RS = 16 * RJ;
   const int lane = threadIdx.x & 63, l16 = lane & 15, lq = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const LoraTile t = p.tiles[KS ? blockIdx.x >> 2 : blockIdx.x];
-  const int group = KS ? (blockIdx.x & 3) : wave;
-  if (16 * group >= t.rows) return;                               // KS: the whole workgroup
+  const LoraTile t = p.tiles[blockIdx.x];
+  const int row0 = WIDE ? 32 * wave : 0;
+  if (row0 >= t.rows) return;
   const LoraAdapter ad = p.adapters[t.adapter];
-  const int prow = t.perm0 + min(16 * group + l16, t.rows - 1);   // rows past the tile repeat its last one
-  const uint16_t* xp = p.x + (int64_t)p.perm[prow] * p.ldx + 8 * lq;
-  const uint16_t* ap = p.bank + ad.a_off + (int64_t)l16 * p.K + 8 * lq;
+  const uint16_t* xp[2];
+#pragma unroll
+  for (int g = 0; g < 2; ++g)                                     // rows past the tile repeat its last one
+    xp[g] = p.x + (int64_t)p.perm[t.perm0 + min(row0 + 16 * g + l16, t.rows - 1)] * p.ldx + 8 * lq;
+  const uint16_t* ap = p.bank + ad.a_off + (l16 * 4 + lq) * 8;
+  const int64_t astep = 32 * ad.rank8;
   const int nsteps = (int)((p.K + 31) / 32);
   int s0 = blockIdx.y * p.steps, s1 = min(nsteps, s0 + p.steps);
-  if constexpr (KS) {
+  if constexpr (!WIDE) {
     const int per = (p.steps + 3) / 4;
     s0 += wave * per;
     s1 = min(s1, s0 + per);
   }
-  v4f acc[RJ];
+  v4f acc[2][RJ];
 #pragma unroll
-  for (int j = 0; j < RJ; ++j) acc[j] = (v4f){0.f, 0.f, 0.f, 0.f};
-  const v4i zero = {0, 0, 0, 0};
-#pragma unroll 4
-  for (int s = s0; s < s1; ++s) {
-    const int64_t k = 32 * (int64_t)s;
-    const bool in = k + 8 * lq < p.K;
-    const v4i xf = in ? *reinterpret_cast<const v4i*>(xp + k) : zero;
+  for (int g = 0; g < 2; ++g)
 #pragma unroll
-    for (int j = 0; j < RJ; ++j) {
-      if (16 * j < ad.rank8) {
-        const v4i af = in && 16 * j + l16 < ad.rank8 ? *reinterpret_cast<const v4i*>(ap + (int64_t)(16 * j) * p.K + k) : zero;
-        acc[j] = lr_mma<DT>::run(xf, af, acc[j]);
+    for (int j = 0; j < RJ; ++j) acc[g][j] = (v4f){0.f, 0.f, 0.f, 0.f};
+#define LR_SHRINK(NJ_) lr_shrink<DT, NJ_, RJ>(acc, xp[0], xp[1], ap, astep, s0, s1, p.K, lq)
+  if (ad.rank8 <= 16) LR_SHRINK(1);
+  else if constexpr (RJ > 1) {
+    if (ad.rank8 <= 32) LR_SHRINK(2);
+    else if constexpr (RJ > 2) {
+      if (ad.rank8 <= 64) LR_SHRINK(4);
+      else if constexpr (RJ > 4) {
+        if (ad.rank8 <= 128) LR_SHRINK(8);
+        else if constexpr (RJ > 8) LR_SHRINK(16);
       }
     }
   }
-  // acc[j][r] is row 4 lq + r, rank 16 j + l16
-  float* sp = p.s + ((int64_t)blockIdx.y * p.rows + t.perm0 + 16 * group) * RS;
-  const int nr = min(16, t.rows - 16 * group);
-  if constexpr (KS) {
-    __shared__ float red[3][16 * RS];
+#undef LR_SHRINK
+  // acc[g][j][r] is row 16 g + l16, rank 16 j + 4 lq + r
+  if constexpr (!WIDE) {
+    __shared__ float4 red[3][2][RJ][64];
     if (wave > 0) {
 #pragma unroll
-      for (int j = 0; j < RJ; ++j)
+      for (int g = 0; g < 2; ++g)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) red[wave - 1][(4 * lq + r) * RS + 16 * j + l16] = acc[j][r];
+        for (int j = 0; j < RJ; ++j) red[wave - 1][g][j][lane] = make_float4(acc[g][j][0], acc[g][j][1], acc[g][j][2], acc[g][j][3]);
     }
     __syncthreads();
     if (wave > 0) return;
 #pragma unroll
-    for (int j = 0; j < RJ; ++j)
+    for (int w = 0; w < 3; ++w)
 #pragma unroll
-      for (int r = 0; r < 4; ++r)
+      for (int g = 0; g < 2; ++g)
 #pragma unroll
-        for (int w = 0; w < 3; ++w) acc[j][r] += red[w][(4 * lq + r) * RS + 16 * j + l16];
+        for (int j = 0; j < RJ; ++j) {
+          const float4 o = red[w][g][j][lane];
+          acc[g][j][0] += o.x; acc[g][j][1] += o.y; acc[g][j][2] += o.z; acc[g][j][3] += o.w;
+        }
   }
 #pragma unroll
-  for (int j = 0; j < RJ; ++j)
+  for (int g = 0; g < 2; ++g) {
+    const int r = row0 + 16 * g + l16;
+    if (r < t.rows) {
+      const int64_t pr = t.perm0 + r;
+      if (p.splits == 1) {
+        uint16_t* sp = reinterpret_cast<uint16_t*>(p.s) + pr * RS + 4 * lq;
 #pragma unroll
-    for (int r = 0; r < 4; ++r)
-      if (4 * lq + r < nr) sp[(4 * lq + r) * RS + 16 * j + l16] = acc[j][r];
+        for (int j = 0; j < RJ; ++j)
+          if (16 * j < ad.rank8)
+            *reinterpret_cast<uint2*>(sp + 16 * j) = make_uint2(pack2<DT>(acc[g][j][0] * ad.scale, acc[g][j][1] * ad.scale),
+                                                                pack2<DT>(acc[g][j][2] * ad.scale, acc[g][j][3] * ad.scale));
+      } else {
+        float* sp = reinterpret_cast<float*>(p.s) + ((int64_t)blockIdx.y * p.rows + pr) * RS + 4 * lq;
+#pragma unroll
+        for (int j = 0; j < RJ; ++j)
+          if (16 * j < ad.rank8)
+            *reinterpret_cast<float4*>(sp + 16 * j) = make_float4(acc[g][j][0], acc[g][j][1], acc[g][j][2], acc[g][j][3]);
+      }
+    }
+  }
 }
 
-template <int DT, int RJ>
+struct LrRows {          // what a lane of expand holds: rows l16 and 16 + l16 of the wave's 32
+  const uint16_t* y[2];  // at column 8 lq
+  uint16_t* o[2];
+  bool in[2];
+};
+
+// columns n, n + step, .. < n1 of the wave's rows, ranks [0, 32 NK); 64 columns a round: both 64-byte halves of a row's line
+// are read and written together, and the next round's y is on its way while this one multiplies
+template <int DT, int NK, int KK>
+__device__ __forceinline__ void lr_expand(const v4i (&sf)[2][KK], const LrRows& w, const uint16_t* bp, int rank8, int64_t n, int64_t n1, int step,
+                                          int64_t N, int lq) {
+  uint4 yv[2][2], yc[2][2];
+  auto load_y = [&](int64_t c) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int64_t cc = min(c + 32 * h, N - 8 - 8 * lq);   // columns past the end: re-read, not stored
+#pragma unroll
+      for (int g = 0; g < 2; ++g) yv[g][h] = *reinterpret_cast<const uint4*>(w.y[g] + cc);
+    }
+  };
+  load_y(n);
+  for (; n < n1; n += step) {
+    v4i bf[2][2][NK];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint16_t* bh = bp + min(n / 32 + h, (N - 1) / 32) * 32 * rank8;
+#pragma unroll
+      for (int kk = 0; kk < NK; ++kk)
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+          const int quads = min(4, max(0, rank8 / 8 - 4 * kk));
+          bf[h][b][kk] = *reinterpret_cast<const v4i*>(bh + kk * 1024 + b * quads * 128);
+        }
+    }
+#pragma unroll
+    for (int g = 0; g < 2; ++g)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) yc[g][h] = yv[g][h];
+    if (n + step < n1) load_y(n + step);
+    v4f acc[2][2][2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        acc[0][h][b] = acc[1][h][b] = (v4f){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int kk = 0; kk < NK; ++kk) {
+          v4i f = bf[h][b][kk];
+          const int keep = lq < rank8 / 8 - 4 * kk ? -1 : 0;   // what lies behind the rank's last quad is not B's
+          f &= (v4i){keep, keep, keep, keep};
+          acc[0][h][b] = lr_mma<DT>::run(f, sf[0][kk], acc[0][h][b]);
+          acc[1][h][b] = lr_mma<DT>::run(f, sf[1][kk], acc[1][h][b]);
+        }
+      }
+#pragma unroll
+    for (int g = 0; g < 2; ++g)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        if (w.in[g] && n + 32 * h + 8 * lq < n1) {
+          float f[8];
+          unpack8<DT>(yc[g][h], f);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) f[e] += acc[g][h][e >> 2][e & 3];
+          *reinterpret_cast<uint4*>(w.o[g] + n + 32 * h) = pack8<DT>(f);
+        }
+  }
+}
+
+template <int DT, int RJ, bool WIDE>
 __global__ __launch_bounds__(256) void lora_expand_kernel(const LoraParams p) {
   constexpr int RS = 16 * RJ, KK = (RJ + 1) / 2;
   const int lane = threadIdx.x & 63, l16 = lane & 15, lq = lane >> 4;
@@ -125,79 +290,58 @@ __global__ __launch_bounds__(256) void lora_expand_kernel(const LoraParams p) {
     }
     return;
   }
+  const int row0 = WIDE ? 32 * wave : 0;
+  const int64_t n = n0 + (WIDE ? 0 : 64 * wave);
+  if (row0 >= t.rows || n >= n1) return;
   const LoraAdapter ad = p.adapters[t.adapter];
   const v4i zero = {0, 0, 0, 0};
   // S fragments: B operand, lane = row l16 of group g, 8 ranks from 32 kk + 8 lq
-  v4i sf[4][KK];
+  v4i sf[2][KK];
+  LrRows w;
 #pragma unroll
-  for (int g = 0; g < 4; ++g) {
-    if (16 * g < t.rows) {
-      const int pr = t.perm0 + min(16 * g + l16, t.rows - 1);
+  for (int g = 0; g < 2; ++g) {
+    const int r = row0 + 16 * g + l16;
+    w.in[g] = r < t.rows;
+    const int64_t pr = t.perm0 + min(r, t.rows - 1);
+    const int64_t row = p.perm[pr];
+    w.y[g] = p.y + row * p.ldy + 8 * lq;
+    w.o[g] = p.out + row * p.ldo + 8 * lq;
 #pragma unroll
-      for (int kk = 0; kk < KK; ++kk) {
-        const int r0 = 32 * kk + 8 * lq;
-        if (r0 < ad.rank8) {
-          float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-          for (int s = 0; s < p.splits; ++s) {
-            const float* sp = p.s + ((int64_t)s * p.rows + pr) * RS + r0;
-            const float4 a = *reinterpret_cast<const float4*>(sp), b = *reinterpret_cast<const float4*>(sp + 4);
-            f[0] += a.x; f[1] += a.y; f[2] += a.z; f[3] += a.w; f[4] += b.x; f[5] += b.y; f[6] += b.z; f[7] += b.w;
-          }
-#pragma unroll
-          for (int e = 0; e < 8; ++e) f[e] *= ad.scale;
-          sf[g][kk] = __builtin_bit_cast(v4i, pack8<DT>(f));
-        } else sf[g][kk] = zero;
-      }
-    }
-  }
-  int64_t yo[4], oo[4];
-#pragma unroll
-  for (int g = 0; g < 4; ++g) {
-    const int64_t row = p.perm[t.perm0 + min(16 * g + l16, t.rows - 1)];
-    yo[g] = row * p.ldy + 8 * lq;
-    oo[g] = row * p.ldo + 8 * lq;
-  }
-  const int nl = 8 * (l16 >> 2) + (l16 & 3);      // A operand row -> column: lane ends with 8 consecutive columns
-  for (int64_t n = n0 + 32 * wave; n < n1; n += 128) {
-    v4f acc[4][2];
-#pragma unroll
-    for (int g = 0; g < 4; ++g) acc[g][0] = acc[g][1] = (v4f){0.f, 0.f, 0.f, 0.f};
-    v4i bf[2][KK];
-#pragma unroll
-    for (int b = 0; b < 2; ++b) {
-      const int64_t nn = n + nl + 4 * b;
-#pragma unroll
-      for (int kk = 0; kk < KK; ++kk) {
-        const int r0 = 32 * kk + 8 * lq;
-        bf[b][kk] = nn < n1 && r0 < ad.rank8 ? *reinterpret_cast<const v4i*>(p.bank + ad.b_off + nn * ad.rank8 + r0) : zero;
-      }
-    }
-    const bool in = n + 8 * lq < n1;
-#pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      if (16 * g < t.rows) {
-#pragma unroll
-        for (int kk = 0; kk < KK; ++kk) {
-          if (32 * kk < ad.rank8) {
-            acc[g][0] = lr_mma<DT>::run(bf[0][kk], sf[g][kk], acc[g][0]);
-            acc[g][1] = lr_mma<DT>::run(bf[1][kk], sf[g][kk], acc[g][1]);
-          }
+    for (int kk = 0; kk < KK; ++kk) {
+      const int r0 = 32 * kk + 8 * lq;
+      if (r0 >= ad.rank8) sf[g][kk] = zero;
+      else if (p.splits == 1) sf[g][kk] = *reinterpret_cast<const v4i*>(reinterpret_cast<const uint16_t*>(p.s) + pr * RS + r0);
+      else {
+        float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        const float* sp = reinterpret_cast<const float*>(p.s) + pr * RS + r0;
+#pragma unroll 8
+        for (int s = 0; s < p.splits; ++s) {
+          const float4 a = *reinterpret_cast<const float4*>(sp + s * p.rows * RS), b = *reinterpret_cast<const float4*>(sp + s * p.rows * RS + 4);
+          f[0] += a.x; f[1] += a.y; f[2] += a.z; f[3] += a.w; f[4] += b.x; f[5] += b.y; f[6] += b.z; f[7] += b.w;
         }
-        if (in && 16 * g + l16 < t.rows) {
-          float f[8];
-          unpack8<DT>(*reinterpret_cast<const uint4*>(p.y + yo[g] + n), f);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) f[e] += acc[g][e >> 2][e & 3];
-          *reinterpret_cast<uint4*>(p.out + oo[g] + n) = pack8<DT>(f);
-        }
+        for (int e = 0; e < 8; ++e) f[e] *= ad.scale;
+        sf[g][kk] = __builtin_bit_cast(v4i, pack8<DT>(f));
       }
     }
   }
+  const int step = WIDE ? 64 : 256;
+  const uint16_t* bp = p.bank + ad.b_off + lane * 8;
+#define LR_EXPAND(NK_) lr_expand<DT, NK_, KK>(sf, w, bp, ad.rank8, n, n1, step, p.N, lq)
+  if (ad.rank8 <= 32) LR_EXPAND(1);
+  else if constexpr (KK > 1) {
+    if (ad.rank8 <= 64) LR_EXPAND(2);
+    else if constexpr (KK > 2) {
+      if (ad.rank8 <= 128) LR_EXPAND(4);
+      else if constexpr (KK > 4) LR_EXPAND(8);
+    }
+  }
+#undef LR_EXPAND
 }
 
-// ---- the plan (host): rows by adapter, tiles of up to 64 of one adapter, rows without one last --------------------------
-// counts = {tiles with an adapter, tiles without, rows, rows with an adapter, largest id + 1}; table = tiles (4 words each), then
-// the row permutation
+// ---- the plan (host): rows by adapter, tiles of one adapter, rows without one last -----------------------------------------
+// counts = {tiles with an adapter, tiles without, rows, rows with an adapter, largest id + 1, rows per tile}; table = tiles (4
+// words each), then the row permutation
 extern "C" int td_lora_plan(const int64_t* lens, const int64_t* ids, int64_t nseq, int32_t* table, int64_t capacity, int64_t* counts) {
   TD_REQUIRE(counts && nseq >= 0 && (nseq == 0 || (lens && ids)), TD_ERR_INVALID, "td_lora_plan: null pointer or %lld sequences", (long long)nseq);
   int64_t rows = 0, nid = 0;
@@ -211,18 +355,19 @@ extern "C" int td_lora_plan(const int64_t* lens, const int64_t* ids, int64_t nse
   try {
     std::vector<int64_t> count(nid + 1, 0), at(nid + 1, 0);      // slot nid: no adapter
     for (int64_t s = 0; s < nseq; ++s) count[ids[s] < 0 ? nid : ids[s]] += lens[s];
+    const int64_t tile = rows - count[nid] >= 8192 ? LR_WIDE : LR_NARROW;
     int64_t tiles[2] = {0, 0};
     for (int64_t i = 0, pos = 0; i <= nid; ++i) {
       at[i] = pos; pos += count[i];
-      tiles[i == nid] += td_cdiv(count[i], LR_TILE);
+      tiles[i == nid] += td_cdiv(count[i], tile);
     }
-    counts[0] = tiles[0]; counts[1] = tiles[1]; counts[2] = rows; counts[3] = rows - count[nid]; counts[4] = nid;
+    counts[0] = tiles[0]; counts[1] = tiles[1]; counts[2] = rows; counts[3] = rows - count[nid]; counts[4] = nid; counts[5] = tile;
     if (table) {
       TD_REQUIRE(capacity >= 4 * (tiles[0] + tiles[1]) + rows, TD_ERR_INVALID, "td_lora_plan: table of %lld words", (long long)capacity);
       LoraTile* t = reinterpret_cast<LoraTile*>(table);
       for (int64_t i = 0; i <= nid; ++i)
-        for (int64_t r = 0; r < count[i]; r += LR_TILE)
-          *t++ = {(int32_t)(at[i] + r), (int32_t)std::min<int64_t>(LR_TILE, count[i] - r), i == nid ? -1 : (int32_t)i, 0};
+        for (int64_t r = 0; r < count[i]; r += tile)
+          *t++ = {(int32_t)(at[i] + r), (int32_t)std::min<int64_t>(tile, count[i] - r), i == nid ? -1 : (int32_t)i, 0};
       int32_t* perm = reinterpret_cast<int32_t*>(t);
       for (int64_t s = 0, row = 0; s < nseq; ++s) {
         int64_t& pos = at[ids[s] < 0 ? nid : ids[s]];
@@ -236,19 +381,14 @@ extern "C" int td_lora_plan(const int64_t* lens, const int64_t* ids, int64_t nse
   return TD_OK;
 }
 
-struct LoraShape { int rj, splits, steps; bool ks; };
-// 256 CUs: with 512 tiles or more every wave owns 16 rows and walks the whole of K; below that the workgroups are 16 rows
-// each, their waves split K, and K is split further until there are about 512 workgroups (at least 512 of K each)
-static LoraShape lora_shape(int64_t tiles, int64_t rows, int64_t k, int max_rank) {
+struct LoraShape { int rj, splits, steps; bool wide; };
+// 256 CUs: K is split over workgroups until there are about 512 of them, at least 512 of K each
+static LoraShape lora_shape(const int64_t* counts, int64_t k, int max_rank) {
   LoraShape s;
   s.rj = max_rank <= 16 ? 1 : max_rank <= 32 ? 2 : max_rank <= 64 ? 4 : max_rank <= 128 ? 8 : 16;
-  const int nsteps = (int)td_cdiv(k, 32);
-  s.ks = tiles < 512;
-  int64_t want = 1;
-  if (s.ks) {
-    const int64_t groups = std::max<int64_t>(std::max<int64_t>(tiles, 1), td_cdiv(rows, 16));
-    want = std::max<int64_t>(1, std::min<int64_t>(td_cdiv(512, groups), nsteps / 16));
-  }
+  s.wide = counts[5] == LR_WIDE;
+  const int64_t nsteps = td_cdiv(k, 32), tiles = std::max<int64_t>(counts[0], 1);
+  const int64_t want = s.wide ? 1 : std::max<int64_t>(1, std::min<int64_t>(td_cdiv(512, tiles), nsteps / 16));
   s.steps = (int)td_cdiv(nsteps, want);
   s.splits = (int)td_cdiv(nsteps, s.steps);
   return s;
@@ -257,8 +397,22 @@ static LoraShape lora_shape(int64_t tiles, int64_t rows, int64_t k, int max_rank
 extern "C" int td_lora_workspace(const int64_t* counts, int64_t k, int max_rank, int64_t* floats) {
   TD_REQUIRE(counts && floats && k > 0 && max_rank > 0 && max_rank <= LR_MAX_RANK, TD_ERR_INVALID, "td_lora_workspace: k = %lld, rank %d",
              (long long)k, max_rank);
-  const LoraShape s = lora_shape(counts[0], counts[3], k, max_rank);
-  *floats = (int64_t)s.splits * counts[3] * 16 * s.rj;
+  const LoraShape s = lora_shape(counts, k, max_rank);
+  *floats = (int64_t)s.splits * counts[3] * 16 * s.rj / (s.splits == 1 ? 2 : 1);
+  return TD_OK;
+}
+
+extern "C" int td_lora_pack(const void* a, int64_t lda, const void* b, int64_t ldb, int rank, int64_t k, int64_t n, void* bank_a, void* bank_b,
+                            td_stream_t stream) {
+  TD_REQUIRE(a && b && bank_a && bank_b, TD_ERR_INVALID, "td_lora_pack: null pointer");
+  TD_REQUIRE(rank > 0 && rank <= LR_MAX_RANK && k > 0 && n > 0 && k % 8 == 0 && n % 8 == 0 && k < (1 << 30) && n < (1 << 30), TD_ERR_UNSUPPORTED,
+             "td_lora_pack: rank %d (at most %d), k = %lld, n = %lld (multiples of 8)", rank, LR_MAX_RANK, (long long)k, (long long)n);
+  TD_REQUIRE(((uintptr_t)bank_a & 15) == 0 && ((uintptr_t)bank_b & 15) == 0, TD_ERR_UNSUPPORTED, "td_lora_pack: the bank must be 16-byte aligned");
+  const int r8 = (rank + 7) / 8 * 8;
+  const int64_t pieces = (td_cdiv(k, 32) + td_cdiv(n, 32)) * 4 * r8;
+  lora_pack_kernel<<<(unsigned)std::min<int64_t>(td_cdiv(pieces, 256), 1024), 256, 0, (hipStream_t)stream>>>(
+      (const uint16_t*)a, lda, (const uint16_t*)b, ldb, rank, r8, k, n, (uint16_t*)bank_a, (uint16_t*)bank_b);
+  TD_CHECK_LAUNCH();
   return TD_OK;
 }
 
@@ -276,8 +430,9 @@ extern "C" int td_lora_add(const void* x, int64_t ldx, const void* y, int64_t ld
   TD_REQUIRE(max_rank > 0 && max_rank <= LR_MAX_RANK, TD_ERR_UNSUPPORTED, "td_lora_add: rank %d (at most %d)", max_rank, LR_MAX_RANK);
   TD_REQUIRE(counts[4] <= num_adapters, TD_ERR_INVALID, "td_lora_add: the plan names adapter %lld of %d", (long long)counts[4] - 1, num_adapters);
   TD_REQUIRE(counts[0] >= 0 && counts[1] >= 0 && counts[0] + counts[1] < (1 << 28), TD_ERR_INVALID, "td_lora_add: counts");
+  TD_REQUIRE(counts[5] == LR_WIDE || counts[5] == LR_NARROW, TD_ERR_INVALID, "td_lora_add: counts");
   TD_REQUIRE(counts[3] == 0 || ws, TD_ERR_INVALID, "td_lora_add: null workspace");
-  const LoraShape sh = lora_shape(counts[0], counts[3], k, max_rank);
+  const LoraShape sh = lora_shape(counts, k, max_rank);
   LoraParams p;
   p.x = (const uint16_t*)x; p.y = (const uint16_t*)y; p.out = (uint16_t*)out;
   p.ldx = ldx; p.ldy = ldy; p.ldo = ldo;
@@ -288,17 +443,19 @@ extern "C" int td_lora_add(const void* x, int64_t ldx, const void* y, int64_t ld
   p.splits = sh.splits; p.steps = sh.steps;
   const int64_t tiles = counts[0] + (out == y ? 0 : counts[1]);
   if (tiles == 0) return TD_OK;
-  p.ntile = tiles >= 512 ? 1024 : tiles >= 32 ? 512 : 128;
+  p.ntile = sh.wide ? 1024 : tiles >= 64 ? 512 : 256;
   hipStream_t st = (hipStream_t)stream;
-  const dim3 gs((unsigned)(counts[0] * (sh.ks ? 4 : 1)), (unsigned)sh.splits), ge((unsigned)tiles, (unsigned)td_cdiv(n, p.ntile));
+  const dim3 gs((unsigned)counts[0], (unsigned)sh.splits), ge((unsigned)tiles, (unsigned)td_cdiv(n, p.ntile));
   TD_REQUIRE(ge.y <= 65535, TD_ERR_UNSUPPORTED, "td_lora_add: n = %lld", (long long)n);
 #define LR_GO(DT_, RJ_)                                                                        \
   {                                                                                            \
-    if (counts[0] > 0) {                                                                       \
-      if (sh.ks) lora_shrink_kernel<DT_, RJ_, true><<<gs, 256, 0, st>>>(p);                    \
-      else lora_shrink_kernel<DT_, RJ_, false><<<gs, 256, 0, st>>>(p);                         \
+    if (sh.wide) {                                                                             \
+      lora_shrink_kernel<DT_, RJ_, true><<<gs, 256, 0, st>>>(p);                               \
+      lora_expand_kernel<DT_, RJ_, true><<<ge, 256, 0, st>>>(p);                               \
+    } else {                                                                                   \
+      if (counts[0] > 0) lora_shrink_kernel<DT_, RJ_, false><<<gs, 256, 0, st>>>(p);           \
+      lora_expand_kernel<DT_, RJ_, false><<<ge, 256, 0, st>>>(p);                              \
     }                                                                                          \
-    lora_expand_kernel<DT_, RJ_><<<ge, 256, 0, st>>>(p);                                       \
   }
 #define LR_GO_DT(DT_)                                                                          \
   switch (sh.rj) {                                                                             \

@@ -13,7 +13,7 @@ import torch
 
 from . import _lib as L
 from .kernels import call, _f32c
-from ._lib import dt_code, ptr, require_gpu
+from ._lib import dt_code, ptr, require_gpu, stream_ptr
 
 
 def _lengths(lens, what):
@@ -165,6 +165,7 @@ class AdapterBank:
     1 to 256 that may differ; ``scales[i]`` (default 1) multiplies the update (the usual alpha / rank)."""
 
     MAX_RANK = 256
+    SPARE = 16384          # elements behind the last adapter that a call may read (td_lora_add)
 
     def __init__(self, pairs, scales=None, device="cuda"):
         pairs = list(pairs)
@@ -196,15 +197,16 @@ class AdapterBank:
         self.ranks = [a.shape[0] for a, _ in pairs]
         r8 = [-(-r // 8) * 8 for r in self.ranks]
         self.max_rank = max(r8)
+        k32, n32 = -(-self.k // 32) * 32, -(-self.n // 32) * 32
         with _guard(self.device):
-            self.data = torch.zeros(sum(r * (self.k + self.n) for r in r8), dtype=self.dtype, device=self.device)
+            self.data = torch.empty(sum(r * (k32 + n32) for r in r8) + self.SPARE, dtype=self.dtype, device=self.device)
             meta = torch.zeros(len(pairs), 3, dtype=torch.int64)
-            off = 0
+            off, st = 0, stream_ptr()
             for i, ((a, b), r, r_) in enumerate(zip(pairs, self.ranks, r8)):
-                oa, ob = off, off + r_ * self.k
-                off = ob + self.n * r_
-                self.data[oa:ob].view(r_, self.k)[:r] = a.detach()
-                self.data[ob:off].view(self.n, r_)[:, :r] = b.detach()
+                oa, ob = off, off + r_ * k32
+                off = ob + n32 * r_
+                a, b = (t.detach().to(self.device).contiguous() for t in (a, b))
+                call("td_lora_pack", ptr(a), self.k, ptr(b), r, r, self.k, self.n, ptr(self.data[oa:]), ptr(self.data[ob:]), st)
                 meta[i, 0], meta[i, 1] = oa, ob
                 words = meta[i, 2:].view(torch.int32)
                 words[0] = r_
@@ -224,7 +226,7 @@ class AdapterPlan(_Plan):
         if len(self.lens) != len(self.ids):
             raise ValueError(f"AdapterPlan: {len(self.lens)} lengths, {len(self.ids)} adapter ids")
         args = (_i64_array(self.lens), _i64_array(self.ids), len(self.lens))
-        self._counts = (ctypes.c_int64 * 5)()
+        self._counts = (ctypes.c_int64 * 6)()
         L.call("td_lora_plan", *args, None, 0, self._counts)
         n = 4 * (self._counts[0] + self._counts[1]) + self._counts[2]
         host = torch.zeros(max(1, n), dtype=torch.int32)
