@@ -139,7 +139,7 @@ def test_adapter_refusals():
 
 def test_adapter_workspace_of_every_plan():
     """no rows with an adapter need no workspace; otherwise at least one fp32 part of every such row"""
-    for tiles, rows, tile in ((0, 0, 32), (1, 1, 32), (5, 150, 32), (64, 8192, 128), (600, 600 * 128, 128)):
+    for tiles, rows, tile in ((0, 0, 32), (1, 1, 32), (5, 150, 32), (32, 8192, 256), (600, 600 * 256, 256)):
         c = (ctypes.c_int64 * 6)(tiles, 0, rows, rows, 1, tile)
         for k in (8, 64, 4096, 10240):
             for rank in (8, 16, 24, 256):

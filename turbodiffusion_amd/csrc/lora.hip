@@ -5,12 +5,11 @@
 // x [rows, K], y / out [rows, N], A_i [rank_i, K], B_i [N, rank_i], 16-bit.  The rows are taken adapter by adapter (a permutation
 // made by the plan), in tiles of one adapter, so an adapter is read for all of its rows at once however its requests lie.
 //
-//   shrink   S = A_i x by MFMA 16x16x32, fp32.  x streams from memory straight into fragments.
+//   shrink   S = A_i x by MFMA 16x16x32, fp32.  x streams from memory straight into fragments.  A workgroup takes 32 rows, its
+//            four waves split K; with few rows K is split over workgroups too and expand adds the fp32 parts in order.
 //   expand   out = y + B_i (s_i S): S is scaled in fp32 and rounded once to the operands' type (half a step of the update only:
 //            it stays below the rounding of the output wherever the update is not many times larger than the output itself).
-// A wave works on 32 rows.  WIDE tiles (many rows): 128 rows, 32 per wave, the waves share the adapter through the CU's L1.  Narrow
-// tiles: 32 rows; shrink's waves split K, and K is split over workgroups too (expand adds the fp32 parts in order), expand's waves
-// split the columns.
+//            A wave keeps B_i of 64 columns in registers and walks the tile's rows, 16 at a time.
 // The bank holds A and B in fragment order (td_lora_pack): every load of them is a contiguous kilobyte, ranks are padded to 8
 // only.  Memory-bound: y and out dominate, then x; 2 rank flops per byte of them.
 #include "td_common.h"
@@ -18,8 +17,8 @@
 #include <new>
 #include <vector>
 
-#define LR_WIDE 128
-#define LR_NARROW 32
+#define LR_WIDE 256       // rows per tile: many rows (B_i is read once per tile and column set) ...
+#define LR_NARROW 32      // ... and few
 #define LR_MAX_RANK 256
 
 struct LoraTile { int32_t perm0, rows, adapter, pad; };
@@ -33,7 +32,7 @@ struct LoraParams {
   void* s;                  // splits == 1: 16-bit, scaled [rows][RS]; else f32 parts [splits][rows][RS]
   int64_t rows, K, N;
   int splits, steps;        // K splits over workgroups, K steps of 32 per split
-  int ntile;                // columns per workgroup of expand
+  int subs;                 // 32-row groups of a full tile
 };
 
 template <int DT> struct lr_mma;
@@ -123,13 +122,13 @@ __device__ __forceinline__ void lr_shrink(v4f (&acc)[2][RJ], const uint16_t* x0,
 }
 
 // RJ: 16-rank blocks of the largest adapter (1, 2, 4, 8, 16); an adapter takes the smallest of these that holds its rank
-template <int DT, int RJ, bool WIDE>
-__global__ __launch_bounds__(256) void lora_shrink_kernel(const LoraParams p) {
+template <int DT, int RJ>
+__global__ __launch_bounds__(256, RJ <= 8 ? 2 : 1) void lora_shrink_kernel(const LoraParams p) {
   constexpr int RS = 16 * RJ;
   const int lane = threadIdx.x & 63, l16 = lane & 15, lq = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const LoraTile t = p.tiles[blockIdx.x];
-  const int row0 = WIDE ? 32 * wave : 0;
+  const LoraTile t = p.tiles[blockIdx.x / p.subs];
+  const int row0 = 32 * (blockIdx.x % p.subs);
   if (row0 >= t.rows) return;
   const LoraAdapter ad = p.adapters[t.adapter];
   const uint16_t* xp[2];
@@ -139,12 +138,8 @@ __global__ __launch_bounds__(256) void lora_shrink_kernel(const LoraParams p) {
   const uint16_t* ap = p.bank + ad.a_off + (l16 * 4 + lq) * 8;
   const int64_t astep = 32 * ad.rank8;
   const int nsteps = (int)((p.K + 31) / 32);
-  int s0 = blockIdx.y * p.steps, s1 = min(nsteps, s0 + p.steps);
-  if constexpr (!WIDE) {
-    const int per = (p.steps + 3) / 4;
-    s0 += wave * per;
-    s1 = min(s1, s0 + per);
-  }
+  const int per = (p.steps + 3) / 4;
+  const int s0 = blockIdx.y * p.steps + wave * per, s1 = min(min(nsteps, (int)(blockIdx.y + 1) * p.steps), s0 + per);
   v4f acc[2][RJ];
 #pragma unroll
   for (int g = 0; g < 2; ++g)
@@ -163,171 +158,140 @@ __global__ __launch_bounds__(256) void lora_shrink_kernel(const LoraParams p) {
     }
   }
 #undef LR_SHRINK
-  // acc[g][j][r] is row 16 g + l16, rank 16 j + 4 lq + r
-  if constexpr (!WIDE) {
-    __shared__ float4 red[3][2][RJ][64];
-    if (wave > 0) {
+  // acc[g][j][r] is row 16 g + l16, rank 16 j + 4 lq + r; the four waves' parts are added in order, each wave a share of them
+  __shared__ float4 red[4][2 * RJ][64];
 #pragma unroll
-      for (int g = 0; g < 2; ++g)
+  for (int g = 0; g < 2; ++g)
 #pragma unroll
-        for (int j = 0; j < RJ; ++j) red[wave - 1][g][j][lane] = make_float4(acc[g][j][0], acc[g][j][1], acc[g][j][2], acc[g][j][3]);
+    for (int j = 0; j < RJ; ++j) red[wave][g * RJ + j][lane] = make_float4(acc[g][j][0], acc[g][j][1], acc[g][j][2], acc[g][j][3]);
+  __syncthreads();
+  for (int i = wave; i < 2 * RJ; i += 4) {
+    const int g = i / RJ, j = i % RJ, r = row0 + 16 * g + l16;
+    if (16 * j >= ad.rank8 || r >= t.rows) continue;
+    float4 v = red[0][i][lane];
+#pragma unroll
+    for (int w = 1; w < 4; ++w) {
+      const float4 o = red[w][i][lane];
+      v.x += o.x; v.y += o.y; v.z += o.z; v.w += o.w;
     }
-    __syncthreads();
-    if (wave > 0) return;
-#pragma unroll
-    for (int w = 0; w < 3; ++w)
-#pragma unroll
-      for (int g = 0; g < 2; ++g)
-#pragma unroll
-        for (int j = 0; j < RJ; ++j) {
-          const float4 o = red[w][g][j][lane];
-          acc[g][j][0] += o.x; acc[g][j][1] += o.y; acc[g][j][2] += o.z; acc[g][j][3] += o.w;
-        }
-  }
-#pragma unroll
-  for (int g = 0; g < 2; ++g) {
-    const int r = row0 + 16 * g + l16;
-    if (r < t.rows) {
-      const int64_t pr = t.perm0 + r;
-      if (p.splits == 1) {
-        uint16_t* sp = reinterpret_cast<uint16_t*>(p.s) + pr * RS + 4 * lq;
-#pragma unroll
-        for (int j = 0; j < RJ; ++j)
-          if (16 * j < ad.rank8)
-            *reinterpret_cast<uint2*>(sp + 16 * j) = make_uint2(pack2<DT>(acc[g][j][0] * ad.scale, acc[g][j][1] * ad.scale),
-                                                                pack2<DT>(acc[g][j][2] * ad.scale, acc[g][j][3] * ad.scale));
-      } else {
-        float* sp = reinterpret_cast<float*>(p.s) + ((int64_t)blockIdx.y * p.rows + pr) * RS + 4 * lq;
-#pragma unroll
-        for (int j = 0; j < RJ; ++j)
-          if (16 * j < ad.rank8)
-            *reinterpret_cast<float4*>(sp + 16 * j) = make_float4(acc[g][j][0], acc[g][j][1], acc[g][j][2], acc[g][j][3]);
-      }
-    }
+    const int64_t pr = t.perm0 + r;
+    if (p.splits == 1)
+      *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(p.s) + pr * RS + 16 * j + 4 * lq) =
+          make_uint2(pack2<DT>(v.x * ad.scale, v.y * ad.scale), pack2<DT>(v.z * ad.scale, v.w * ad.scale));
+    else
+      *reinterpret_cast<float4*>(reinterpret_cast<float*>(p.s) + ((int64_t)blockIdx.y * p.rows + pr) * RS + 16 * j + 4 * lq) = v;
   }
 }
 
-struct LrRows {          // what a lane of expand holds: rows l16 and 16 + l16 of the wave's 32
-  const uint16_t* y[2];  // at column 8 lq
-  uint16_t* o[2];
-  bool in[2];
-};
-
-// columns n, n + step, .. < n1 of the wave's rows, ranks [0, 32 NK); 64 columns a round: both 64-byte halves of a row's line
-// are read and written together, and the next round's y is on its way while this one multiplies
-template <int DT, int NK, int KK>
-__device__ __forceinline__ void lr_expand(const v4i (&sf)[2][KK], const LrRows& w, const uint16_t* bp, int rank8, int64_t n, int64_t n1, int step,
-                                          int64_t N, int lq) {
-  uint4 yv[2][2], yc[2][2];
-  auto load_y = [&](int64_t c) {
+// 64 columns from n of the tile's rows, ranks [0, 32 NK): B stays in registers, y and S of the next 16 rows are on their way
+// while these multiply.  sb / srs: the tile's S (16-bit, scaled) and its row stride; prow: its rows' numbers (LDS).
+template <int DT, int NK>
+__device__ __forceinline__ void lr_expand(const LoraParams& p, const uint16_t* sb, int srs, const int32_t* prow, int rows, const uint16_t* bp,
+                                          int rank8, int64_t n, int l16, int lq) {
+  v4i bf[2][2][NK];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int64_t cc = min(c + 32 * h, N - 8 - 8 * lq);   // columns past the end: re-read, not stored
+  for (int h = 0; h < 2; ++h) {
+    const uint16_t* bh = bp + min(n / 32 + h, (p.N - 1) / 32) * 32 * rank8;
 #pragma unroll
-      for (int g = 0; g < 2; ++g) yv[g][h] = *reinterpret_cast<const uint4*>(w.y[g] + cc);
+    for (int kk = 0; kk < NK; ++kk)
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        const int quads = min(4, max(0, rank8 / 8 - 4 * kk));
+        v4i f = *reinterpret_cast<const v4i*>(bh + kk * 1024 + b * quads * 128);
+        const int keep = lq < quads ? -1 : 0;                   // what lies behind the rank's last quad is not B's
+        bf[h][b][kk] = f & (v4i){keep, keep, keep, keep};
+      }
+  }
+  const int64_t col = n + 8 * lq;
+  const bool c0 = col < p.N, c1 = col + 32 < p.N;
+  // columns past the end: re-read the last ones, not stored
+  const uint16_t* y0 = p.y + min(col, p.N - 8);
+  const uint16_t* y1 = p.y + min(col + 32, p.N - 8);
+  uint4 ya, yb;
+  v4i sf[NK];
+  int64_t row;
+  auto load = [&](int g) {
+    const int r = min(g + l16, rows - 1);
+    row = prow[r];
+    ya = *reinterpret_cast<const uint4*>(y0 + row * p.ldy);
+    yb = *reinterpret_cast<const uint4*>(y1 + row * p.ldy);
+#pragma unroll
+    for (int kk = 0; kk < NK; ++kk) {
+      const int r0 = min(32 * kk + 8 * lq, rank8 - 8);           // past the rank: any value, B is zero there
+      sf[kk] = *reinterpret_cast<const v4i*>(sb + (int64_t)r * srs + r0);
     }
   };
-  load_y(n);
-  for (; n < n1; n += step) {
-    v4i bf[2][2][NK];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const uint16_t* bh = bp + min(n / 32 + h, (N - 1) / 32) * 32 * rank8;
-#pragma unroll
-      for (int kk = 0; kk < NK; ++kk)
-#pragma unroll
-        for (int b = 0; b < 2; ++b) {
-          const int quads = min(4, max(0, rank8 / 8 - 4 * kk));
-          bf[h][b][kk] = *reinterpret_cast<const v4i*>(bh + kk * 1024 + b * quads * 128);
-        }
-    }
-#pragma unroll
-    for (int g = 0; g < 2; ++g)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) yc[g][h] = yv[g][h];
-    if (n + step < n1) load_y(n + step);
-    v4f acc[2][2][2];
+  load(0);
+  for (int g = 0; g < rows; g += 16) {
+    v4f acc[2][2];
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
-        acc[0][h][b] = acc[1][h][b] = (v4f){0.f, 0.f, 0.f, 0.f};
+        acc[h][b] = (v4f){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int kk = 0; kk < NK; ++kk) {
-          v4i f = bf[h][b][kk];
-          const int keep = lq < rank8 / 8 - 4 * kk ? -1 : 0;   // what lies behind the rank's last quad is not B's
-          f &= (v4i){keep, keep, keep, keep};
-          acc[0][h][b] = lr_mma<DT>::run(f, sf[0][kk], acc[0][h][b]);
-          acc[1][h][b] = lr_mma<DT>::run(f, sf[1][kk], acc[1][h][b]);
-        }
+        for (int kk = 0; kk < NK; ++kk) acc[h][b] = lr_mma<DT>::run(bf[h][b][kk], sf[kk], acc[h][b]);
       }
+    const uint4 va = ya, vb = yb;
+    const bool in = g + l16 < rows;
+    uint16_t* o = p.out + row * p.ldo + col;
+    if (g + 16 < rows) load(g + 16);
+    float f[8];
+    unpack8<DT>(va, f);
 #pragma unroll
-    for (int g = 0; g < 2; ++g)
+    for (int e = 0; e < 8; ++e) f[e] += acc[0][e >> 2][e & 3];
+    if (in && c0) *reinterpret_cast<uint4*>(o) = pack8<DT>(f);
+    unpack8<DT>(vb, f);
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
-        if (w.in[g] && n + 32 * h + 8 * lq < n1) {
-          float f[8];
-          unpack8<DT>(yc[g][h], f);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) f[e] += acc[g][h][e >> 2][e & 3];
-          *reinterpret_cast<uint4*>(w.o[g] + n + 32 * h) = pack8<DT>(f);
-        }
+    for (int e = 0; e < 8; ++e) f[e] += acc[1][e >> 2][e & 3];
+    if (in && c1) *reinterpret_cast<uint4*>(o + 32) = pack8<DT>(f);
   }
 }
 
-template <int DT, int RJ, bool WIDE>
-__global__ __launch_bounds__(256) void lora_expand_kernel(const LoraParams p) {
+// S past the rank must be finite where B is zero: shrink leaves the ranks of a last half block (rank8 % 16 == 8) as whatever
+// lies behind the adapter in the bank, so nothing past rank8 is read
+template <int DT, int RJ>
+__global__ __launch_bounds__(256, RJ <= 8 ? 2 : 1) void lora_expand_kernel(const LoraParams p) {
   constexpr int RS = 16 * RJ, KK = (RJ + 1) / 2;
   const int lane = threadIdx.x & 63, l16 = lane & 15, lq = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const LoraTile t = p.tiles[blockIdx.x];
-  const int64_t n0 = (int64_t)blockIdx.y * p.ntile, n1 = min(p.N, n0 + p.ntile);
+  const int64_t n = (int64_t)blockIdx.y * 256 + 64 * wave;
+  __shared__ int32_t prow[LR_WIDE];
+  if (threadIdx.x < t.rows) prow[threadIdx.x] = p.perm[t.perm0 + threadIdx.x];
   if (t.adapter < 0) {            // rows without an adapter: copy
-    for (int r = wave; r < t.rows; r += 4) {
-      const int64_t row = p.perm[t.perm0 + r];
-      for (int64_t n = n0 + 8 * lane; n < n1; n += 512)
-        *reinterpret_cast<uint4*>(p.out + row * p.ldo + n) = *reinterpret_cast<const uint4*>(p.y + row * p.ldy + n);
-    }
+    __syncthreads();
+    const int64_t c = (int64_t)blockIdx.y * 256 + 8 * (lane & 31);
+    if (c < p.N)
+      for (int r = 2 * wave + (lane >> 5); r < t.rows; r += 8)
+        *reinterpret_cast<uint4*>(p.out + prow[r] * p.ldo + c) = *reinterpret_cast<const uint4*>(p.y + prow[r] * p.ldy + c);
     return;
   }
-  const int row0 = WIDE ? 32 * wave : 0;
-  const int64_t n = n0 + (WIDE ? 0 : 64 * wave);
-  if (row0 >= t.rows || n >= n1) return;
   const LoraAdapter ad = p.adapters[t.adapter];
-  const v4i zero = {0, 0, 0, 0};
-  // S fragments: B operand, lane = row l16 of group g, 8 ranks from 32 kk + 8 lq
-  v4i sf[2][KK];
-  LrRows w;
-#pragma unroll
-  for (int g = 0; g < 2; ++g) {
-    const int r = row0 + 16 * g + l16;
-    w.in[g] = r < t.rows;
-    const int64_t pr = t.perm0 + min(r, t.rows - 1);
-    const int64_t row = p.perm[pr];
-    w.y[g] = p.y + row * p.ldy + 8 * lq;
-    w.o[g] = p.out + row * p.ldo + 8 * lq;
-#pragma unroll
-    for (int kk = 0; kk < KK; ++kk) {
-      const int r0 = 32 * kk + 8 * lq;
-      if (r0 >= ad.rank8) sf[g][kk] = zero;
-      else if (p.splits == 1) sf[g][kk] = *reinterpret_cast<const v4i*>(reinterpret_cast<const uint16_t*>(p.s) + pr * RS + r0);
-      else {
-        float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        const float* sp = reinterpret_cast<const float*>(p.s) + pr * RS + r0;
+  const uint16_t* sb = reinterpret_cast<const uint16_t*>(p.s) + (int64_t)t.perm0 * RS;
+  int srs = RS;
+  __shared__ __attribute__((aligned(16))) uint16_t ssum[LR_NARROW * (RS + 8)];
+  if (p.splits > 1) {             // add the parts of S, scale, round (narrow tiles only)
+    const float* sp = reinterpret_cast<const float*>(p.s) + (int64_t)t.perm0 * RS;
+    const int quads = ad.rank8 / 4;
+    for (int i = threadIdx.x; i < t.rows * quads; i += 256) {
+      const int r = i / quads, c = 4 * (i - r * quads);
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 8
-        for (int s = 0; s < p.splits; ++s) {
-          const float4 a = *reinterpret_cast<const float4*>(sp + s * p.rows * RS), b = *reinterpret_cast<const float4*>(sp + s * p.rows * RS + 4);
-          f[0] += a.x; f[1] += a.y; f[2] += a.z; f[3] += a.w; f[4] += b.x; f[5] += b.y; f[6] += b.z; f[7] += b.w;
-        }
-#pragma unroll
-        for (int e = 0; e < 8; ++e) f[e] *= ad.scale;
-        sf[g][kk] = __builtin_bit_cast(v4i, pack8<DT>(f));
+      for (int s = 0; s < p.splits; ++s) {
+        const float4 o = *reinterpret_cast<const float4*>(sp + (s * p.rows + r) * RS + c);
+        v.x += o.x; v.y += o.y; v.z += o.z; v.w += o.w;
       }
+      *reinterpret_cast<uint2*>(ssum + r * (RS + 8) + c) =
+          make_uint2(pack2<DT>(v.x * ad.scale, v.y * ad.scale), pack2<DT>(v.z * ad.scale, v.w * ad.scale));
     }
+    sb = ssum;
+    srs = RS + 8;
   }
-  const int step = WIDE ? 64 : 256;
+  __syncthreads();
+  if (n >= p.N) return;
   const uint16_t* bp = p.bank + ad.b_off + lane * 8;
-#define LR_EXPAND(NK_) lr_expand<DT, NK_, KK>(sf, w, bp, ad.rank8, n, n1, step, p.N, lq)
+#define LR_EXPAND(NK_) lr_expand<DT, NK_>(p, sb, srs, prow, t.rows, bp, ad.rank8, n, l16, lq)
   if (ad.rank8 <= 32) LR_EXPAND(1);
   else if constexpr (KK > 1) {
     if (ad.rank8 <= 64) LR_EXPAND(2);
@@ -381,14 +345,13 @@ extern "C" int td_lora_plan(const int64_t* lens, const int64_t* ids, int64_t nse
   return TD_OK;
 }
 
-struct LoraShape { int rj, splits, steps; bool wide; };
-// 256 CUs: K is split over workgroups until there are about 512 of them, at least 512 of K each
+struct LoraShape { int rj, splits, steps; };
+// 256 CUs: K is split over workgroups until there are about 256 of them (at most 8 parts, 512 of K each or more)
 static LoraShape lora_shape(const int64_t* counts, int64_t k, int max_rank) {
   LoraShape s;
   s.rj = max_rank <= 16 ? 1 : max_rank <= 32 ? 2 : max_rank <= 64 ? 4 : max_rank <= 128 ? 8 : 16;
-  s.wide = counts[5] == LR_WIDE;
   const int64_t nsteps = td_cdiv(k, 32), tiles = std::max<int64_t>(counts[0], 1);
-  const int64_t want = s.wide ? 1 : std::max<int64_t>(1, std::min<int64_t>(td_cdiv(512, tiles), nsteps / 16));
+  const int64_t want = counts[5] == LR_WIDE ? 1 : std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(8, td_cdiv(256, tiles)), nsteps / 16));
   s.steps = (int)td_cdiv(nsteps, want);
   s.splits = (int)td_cdiv(nsteps, s.steps);
   return s;
@@ -443,19 +406,14 @@ extern "C" int td_lora_add(const void* x, int64_t ldx, const void* y, int64_t ld
   p.splits = sh.splits; p.steps = sh.steps;
   const int64_t tiles = counts[0] + (out == y ? 0 : counts[1]);
   if (tiles == 0) return TD_OK;
-  p.ntile = sh.wide ? 1024 : tiles >= 64 ? 512 : 256;
+  p.subs = (int)(counts[5] / 32);
   hipStream_t st = (hipStream_t)stream;
-  const dim3 gs((unsigned)counts[0], (unsigned)sh.splits), ge((unsigned)tiles, (unsigned)td_cdiv(n, p.ntile));
+  const dim3 gs((unsigned)(counts[0] * p.subs), (unsigned)sh.splits), ge((unsigned)tiles, (unsigned)td_cdiv(n, 256));
   TD_REQUIRE(ge.y <= 65535, TD_ERR_UNSUPPORTED, "td_lora_add: n = %lld", (long long)n);
 #define LR_GO(DT_, RJ_)                                                                        \
   {                                                                                            \
-    if (sh.wide) {                                                                             \
-      lora_shrink_kernel<DT_, RJ_, true><<<gs, 256, 0, st>>>(p);                               \
-      lora_expand_kernel<DT_, RJ_, true><<<ge, 256, 0, st>>>(p);                               \
-    } else {                                                                                   \
-      if (counts[0] > 0) lora_shrink_kernel<DT_, RJ_, false><<<gs, 256, 0, st>>>(p);           \
-      lora_expand_kernel<DT_, RJ_, false><<<ge, 256, 0, st>>>(p);                              \
-    }                                                                                          \
+    if (counts[0] > 0) lora_shrink_kernel<DT_, RJ_><<<gs, 256, 0, st>>>(p);                    \
+    lora_expand_kernel<DT_, RJ_><<<ge, 256, 0, st>>>(p);                                       \
   }
 #define LR_GO_DT(DT_)                                                                          \
   switch (sh.rj) {                                                                             \
