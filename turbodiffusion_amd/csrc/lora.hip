@@ -19,6 +19,7 @@
 
 #define LR_WIDE 256       // rows per tile: many rows (B_i is read once per tile and column set) ...
 #define LR_NARROW 32      // ... and few
+#define LR_TURN 68        // floats per row of a wave's 16 x 64 update in LDS
 #define LR_MAX_RANK 256
 
 struct LoraTile { int32_t perm0, rows, adapter, pad; };
@@ -31,7 +32,7 @@ struct LoraParams {
   const LoraTile* tiles; const int32_t* perm;
   void* s;                  // splits == 1: 16-bit, scaled [rows][RS]; else f32 parts [splits][rows][RS]
   int64_t rows, K, N;
-  int splits, steps;        // K splits over workgroups, K steps of 32 per split
+  int splits, chunks;       // K splits over workgroups, K chunks of 64 per split
   int subs;                 // 32-row groups of a full tile
 };
 
@@ -80,44 +81,45 @@ __global__ __launch_bounds__(256) void lora_pack_kernel(const uint16_t* a, int64
   }
 }
 
-// K steps [s0, s1) of 32 rows, ranks [0, 16 NJ) of one adapter.  No load sits behind a branch: the last fragment of a rank that is
-// no multiple of 16 brings ranks of whatever lies behind it in the bank (it ends with a spare kilobyte), which nothing reads.
+// K chunks [c0, c1) of 64 of 32 rows, ranks [0, 16 NJ) of one adapter.  x: 8 lanes take a row's 128 bytes (a full line) and hand
+// them over as fragments through the wave's own LDS (4 KB a chunk, 16-byte pieces XOR-permuted against bank conflicts).  No load
+// sits behind a branch: the last fragment of a rank that is no multiple of 16 brings ranks of whatever lies behind it in the
+// bank (it ends with spare elements), which nothing reads.
 template <int DT, int NJ, int RJ>
-__device__ __forceinline__ void lr_shrink(v4f (&acc)[2][RJ], const uint16_t* x0, const uint16_t* x1, const uint16_t* ap, int64_t astep,
-                                          int s0, int s1, int64_t K, int lq) {
-  constexpr int U = NJ <= 2 ? 8 : NJ <= 4 ? 4 : 2;
-  const int full = min(s1, (int)(K / 32));
-  int s = s0;
-  for (; s + U <= full; s += U) {
-    v4i xf[U][2], af[U][NJ];
+__device__ __forceinline__ void lr_shrink(v4f (&acc)[2][RJ], const uint16_t* const (&x)[4], const uint16_t* ap, int64_t astep, int c0, int c1,
+                                          int64_t K, char* turn, int lane) {
+  const int l16 = lane & 15, lq = lane >> 4, lr = lane >> 3, lc = lane & 7;
+  const int last = (int)((K + 31) / 32) - 1;
+  const v4i zero = {0, 0, 0, 0};
+  for (int c = c0; c < c1; ++c) {
+    const int64_t k = 64 * (int64_t)c + 8 * lc;
+    v4i xv[4], af[2][NJ];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      xf[u][0] = *reinterpret_cast<const v4i*>(x0 + 32 * (int64_t)(s + u));
-      xf[u][1] = *reinterpret_cast<const v4i*>(x1 + 32 * (int64_t)(s + u));
+    for (int i = 0; i < 4; ++i) {
+      const v4i v = *reinterpret_cast<const v4i*>(x[i] + min(k, K - 8));
+      xv[i] = k < K ? v : zero;
     }
 #pragma unroll
-    for (int u = 0; u < U; ++u)
+    for (int h = 0; h < 2; ++h)
 #pragma unroll
-      for (int j = 0; j < NJ; ++j) af[u][j] = *reinterpret_cast<const v4i*>(ap + (s + u) * astep + 512 * j);
+      for (int j = 0; j < NJ; ++j) af[h][j] = *reinterpret_cast<const v4i*>(ap + min(2 * c + h, last) * astep + 512 * j);
 #pragma unroll
-    for (int u = 0; u < U; ++u)
+    for (int i = 0; i < 4; ++i) {
+      const int r = 8 * i + lr;
+      *reinterpret_cast<v4i*>(turn + r * 128 + ((lc ^ ((r >> 1) & 7)) << 4)) = xv[i];
+    }
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const char* f = turn + l16 * 128 + (((4 * h + lq) ^ ((l16 >> 1) & 7)) << 4);
+      const v4i x0 = *reinterpret_cast<const v4i*>(f), x1 = *reinterpret_cast<const v4i*>(f + 2048);
 #pragma unroll
       for (int j = 0; j < NJ; ++j) {
-        acc[0][j] = lr_mma<DT>::run(af[u][j], xf[u][0], acc[0][j]);
-        acc[1][j] = lr_mma<DT>::run(af[u][j], xf[u][1], acc[1][j]);
+        acc[0][j] = lr_mma<DT>::run(af[h][j], x0, acc[0][j]);
+        acc[1][j] = lr_mma<DT>::run(af[h][j], x1, acc[1][j]);
       }
-  }
-  const v4i zero = {0, 0, 0, 0};
-  for (; s < s1; ++s) {
-    const bool in = 32 * (int64_t)s + 8 * lq < K;
-    const v4i xf0 = in ? *reinterpret_cast<const v4i*>(x0 + 32 * (int64_t)s) : zero;
-    const v4i xf1 = in ? *reinterpret_cast<const v4i*>(x1 + 32 * (int64_t)s) : zero;
-#pragma unroll
-    for (int j = 0; j < NJ; ++j) {
-      const v4i af = *reinterpret_cast<const v4i*>(ap + s * astep + 512 * j);
-      acc[0][j] = lr_mma<DT>::run(af, xf0, acc[0][j]);
-      acc[1][j] = lr_mma<DT>::run(af, xf1, acc[1][j]);
     }
+    __builtin_amdgcn_wave_barrier();
   }
 }
 
@@ -131,21 +133,23 @@ __global__ __launch_bounds__(256, RJ <= 8 ? 2 : 1) void lora_shrink_kernel(const
   const int row0 = 32 * (blockIdx.x % p.subs);
   if (row0 >= t.rows) return;
   const LoraAdapter ad = p.adapters[t.adapter];
-  const uint16_t* xp[2];
+  const uint16_t* xp[4];
 #pragma unroll
-  for (int g = 0; g < 2; ++g)                                     // rows past the tile repeat its last one
-    xp[g] = p.x + (int64_t)p.perm[t.perm0 + min(row0 + 16 * g + l16, t.rows - 1)] * p.ldx + 8 * lq;
+  for (int i = 0; i < 4; ++i)                                     // rows past the tile repeat its last one
+    xp[i] = p.x + (int64_t)p.perm[t.perm0 + min(row0 + 8 * i + (lane >> 3), t.rows - 1)] * p.ldx;
   const uint16_t* ap = p.bank + ad.a_off + (l16 * 4 + lq) * 8;
   const int64_t astep = 32 * ad.rank8;
-  const int nsteps = (int)((p.K + 31) / 32);
-  const int per = (p.steps + 3) / 4;
-  const int s0 = blockIdx.y * p.steps + wave * per, s1 = min(min(nsteps, (int)(blockIdx.y + 1) * p.steps), s0 + per);
+  const int nchunks = (int)((p.K + 63) / 64);
+  const int per = (p.chunks + 3) / 4;
+  const int c0 = blockIdx.y * p.chunks + wave * per, c1 = min(min(nchunks, (int)(blockIdx.y + 1) * p.chunks), c0 + per);
+  constexpr int RED = 4 * 2 * RJ * 64 * 16;
+  __shared__ __attribute__((aligned(16))) char smem[RED > 16384 ? RED : 16384];
   v4f acc[2][RJ];
 #pragma unroll
   for (int g = 0; g < 2; ++g)
 #pragma unroll
     for (int j = 0; j < RJ; ++j) acc[g][j] = (v4f){0.f, 0.f, 0.f, 0.f};
-#define LR_SHRINK(NJ_) lr_shrink<DT, NJ_, RJ>(acc, xp[0], xp[1], ap, astep, s0, s1, p.K, lq)
+#define LR_SHRINK(NJ_) lr_shrink<DT, NJ_, RJ>(acc, xp, ap, astep, c0, c1, p.K, smem + wave * 4096, lane)
   if (ad.rank8 <= 16) LR_SHRINK(1);
   else if constexpr (RJ > 1) {
     if (ad.rank8 <= 32) LR_SHRINK(2);
@@ -159,7 +163,8 @@ __global__ __launch_bounds__(256, RJ <= 8 ? 2 : 1) void lora_shrink_kernel(const
   }
 #undef LR_SHRINK
   // acc[g][j][r] is row 16 g + l16, rank 16 j + 4 lq + r; the four waves' parts are added in order, each wave a share of them
-  __shared__ float4 red[4][2 * RJ][64];
+  float4 (*red)[2 * RJ][64] = reinterpret_cast<float4 (*)[2 * RJ][64]>(smem);
+  __syncthreads();
 #pragma unroll
   for (int g = 0; g < 2; ++g)
 #pragma unroll
@@ -184,10 +189,11 @@ __global__ __launch_bounds__(256, RJ <= 8 ? 2 : 1) void lora_shrink_kernel(const
 }
 
 // 64 columns from n of the tile's rows, ranks [0, 32 NK): B stays in registers, y and S of the next 16 rows are on their way
-// while these multiply.  sb / srs: the tile's S (16-bit, scaled) and its row stride; prow: its rows' numbers (LDS).
+// while these multiply.  sb / srs: the tile's S (16-bit, scaled) and its row stride; prow: its rows' numbers (LDS); turn: the
+// wave's own 16 x 64 floats of LDS.
 template <int DT, int NK>
 __device__ __forceinline__ void lr_expand(const LoraParams& p, const uint16_t* sb, int srs, const int32_t* prow, int rows, const uint16_t* bp,
-                                          int rank8, int64_t n, int l16, int lq) {
+                                          int rank8, int64_t n, int l16, int lq, float* turn) {
   v4i bf[2][2][NK];
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
@@ -202,23 +208,25 @@ __device__ __forceinline__ void lr_expand(const LoraParams& p, const uint16_t* s
         bf[h][b][kk] = f & (v4i){keep, keep, keep, keep};
       }
   }
-  const int64_t col = n + 8 * lq;
-  const bool c0 = col < p.N, c1 = col + 32 < p.N;
-  // columns past the end: re-read the last ones, not stored
-  const uint16_t* y0 = p.y + min(col, p.N - 8);
-  const uint16_t* y1 = p.y + min(col + 32, p.N - 8);
-  uint4 ya, yb;
+  // y and out: 8 lanes take a row's 128 bytes (a full line), two sets of 8 rows; the update comes to them through LDS
+  const int lr = (threadIdx.x & 63) >> 3;
+  const int64_t col = n + 8 * (threadIdx.x & 7);
+  const bool cin = col < p.N;
+  const uint16_t* yb = p.y + min(col, p.N - 8);                 // columns past the end: re-read the last ones, not stored
+  uint16_t* ob = p.out + col;
+  uint4 yv[2];
   v4i sf[NK];
-  int64_t row;
+  int64_t row[2];
   auto load = [&](int g) {
-    const int r = min(g + l16, rows - 1);
-    row = prow[r];
-    ya = *reinterpret_cast<const uint4*>(y0 + row * p.ldy);
-    yb = *reinterpret_cast<const uint4*>(y1 + row * p.ldy);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      row[i] = prow[min(g + 8 * i + lr, rows - 1)];
+      yv[i] = *reinterpret_cast<const uint4*>(yb + row[i] * p.ldy);
+    }
 #pragma unroll
     for (int kk = 0; kk < NK; ++kk) {
       const int r0 = min(32 * kk + 8 * lq, rank8 - 8);           // past the rank: any value, B is zero there
-      sf[kk] = *reinterpret_cast<const v4i*>(sb + (int64_t)r * srs + r0);
+      sf[kk] = *reinterpret_cast<const v4i*>(sb + (int64_t)min(g + l16, rows - 1) * srs + r0);
     }
   };
   load(0);
@@ -231,20 +239,22 @@ __device__ __forceinline__ void lr_expand(const LoraParams& p, const uint16_t* s
         acc[h][b] = (v4f){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int kk = 0; kk < NK; ++kk) acc[h][b] = lr_mma<DT>::run(bf[h][b][kk], sf[kk], acc[h][b]);
+        *reinterpret_cast<v4f*>(turn + l16 * LR_TURN + 32 * h + 8 * lq + 4 * b) = acc[h][b];
       }
-    const uint4 va = ya, vb = yb;
-    const bool in = g + l16 < rows;
-    uint16_t* o = p.out + row * p.ldo + col;
+    __builtin_amdgcn_wave_barrier();
+    const uint4 v[2] = {yv[0], yv[1]};
+    const int64_t r[2] = {row[0], row[1]};
     if (g + 16 < rows) load(g + 16);
-    float f[8];
-    unpack8<DT>(va, f);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) f[e] += acc[0][e >> 2][e & 3];
-    if (in && c0) *reinterpret_cast<uint4*>(o) = pack8<DT>(f);
-    unpack8<DT>(vb, f);
+    for (int i = 0; i < 2; ++i) {
+      float f[8];
+      unpack8<DT>(v[i], f);
+      const v4f* d = reinterpret_cast<const v4f*>(turn + (8 * i + lr) * LR_TURN + 8 * (threadIdx.x & 7));
+      const v4f d0 = d[0], d1 = d[1];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) f[e] += acc[1][e >> 2][e & 3];
-    if (in && c1) *reinterpret_cast<uint4*>(o + 32) = pack8<DT>(f);
+      for (int e = 0; e < 4; ++e) { f[e] += d0[e]; f[4 + e] += d1[e]; }
+      if (cin && g + 8 * i + lr < rows) *reinterpret_cast<uint4*>(ob + r[i] * p.ldo) = pack8<DT>(f);
+    }
   }
 }
 
@@ -258,6 +268,7 @@ __global__ __launch_bounds__(256, RJ <= 8 ? 2 : 1) void lora_expand_kernel(const
   const LoraTile t = p.tiles[blockIdx.x];
   const int64_t n = (int64_t)blockIdx.y * 256 + 64 * wave;
   __shared__ int32_t prow[LR_WIDE];
+  __shared__ __attribute__((aligned(16))) float turn[4][16 * LR_TURN];
   if (threadIdx.x < t.rows) prow[threadIdx.x] = p.perm[t.perm0 + threadIdx.x];
   if (t.adapter < 0) {            // rows without an adapter: copy
     __syncthreads();
@@ -291,7 +302,7 @@ __global__ __launch_bounds__(256, RJ <= 8 ? 2 : 1) void lora_expand_kernel(const
   __syncthreads();
   if (n >= p.N) return;
   const uint16_t* bp = p.bank + ad.b_off + lane * 8;
-#define LR_EXPAND(NK_) lr_expand<DT, NK_>(p, sb, srs, prow, t.rows, bp, ad.rank8, n, l16, lq)
+#define LR_EXPAND(NK_) lr_expand<DT, NK_>(p, sb, srs, prow, t.rows, bp, ad.rank8, n, l16, lq, turn[wave])
   if (ad.rank8 <= 32) LR_EXPAND(1);
   else if constexpr (KK > 1) {
     if (ad.rank8 <= 64) LR_EXPAND(2);
@@ -345,15 +356,15 @@ extern "C" int td_lora_plan(const int64_t* lens, const int64_t* ids, int64_t nse
   return TD_OK;
 }
 
-struct LoraShape { int rj, splits, steps; };
+struct LoraShape { int rj, splits, chunks; };
 // 256 CUs: K is split over workgroups until there are about 256 of them (at most 8 parts, 512 of K each or more)
 static LoraShape lora_shape(const int64_t* counts, int64_t k, int max_rank) {
   LoraShape s;
   s.rj = max_rank <= 16 ? 1 : max_rank <= 32 ? 2 : max_rank <= 64 ? 4 : max_rank <= 128 ? 8 : 16;
-  const int64_t nsteps = td_cdiv(k, 32), tiles = std::max<int64_t>(counts[0], 1);
-  const int64_t want = counts[5] == LR_WIDE ? 1 : std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(8, td_cdiv(256, tiles)), nsteps / 16));
-  s.steps = (int)td_cdiv(nsteps, want);
-  s.splits = (int)td_cdiv(nsteps, s.steps);
+  const int64_t nch = td_cdiv(k, 64), tiles = std::max<int64_t>(counts[0], 1);
+  const int64_t want = counts[5] == LR_WIDE ? 1 : std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(8, td_cdiv(256, tiles)), nch / 8));
+  s.chunks = (int)td_cdiv(nch, want);
+  s.splits = (int)td_cdiv(nch, s.chunks);
   return s;
 }
 
@@ -403,7 +414,7 @@ extern "C" int td_lora_add(const void* x, int64_t ldx, const void* y, int64_t ld
   p.tiles = reinterpret_cast<const LoraTile*>(table);
   p.perm = table + 4 * (counts[0] + counts[1]);
   p.s = ws; p.rows = counts[3]; p.K = k; p.N = n;
-  p.splits = sh.splits; p.steps = sh.steps;
+  p.splits = sh.splits; p.chunks = sh.chunks;
   const int64_t tiles = counts[0] + (out == y ? 0 : counts[1]);
   if (tiles == 0) return TD_OK;
   p.subs = (int)(counts[5] / 32);
