@@ -508,18 +508,17 @@ int td_sla_linear_kv_final_packed(const float* ws_kv, const float* ws_ks, int nc
 /* ---- attention over packed sequences (csrc/attn_packed.hip) ----
  * o[i, h] = sum_j softmax_j(scale q[i, h] . k[j, h / G] + bias[h, clamp(j - pos_i, -bias_range, bias_range) + bias_range]) v[j, h / G]
  * over the keys of row i's own sequence; G = heads / kv_heads; pos_i = i + k_len - q_len; only j <= pos_i when causal.  A row with
- * nothing to attend to is 0.  q, k, v, o: 16-bit (TD_F16 | TD_BF16), head_dim 64 or 128 contiguous, token / head strides in elements
- * (multiples of 8; pointers 16-byte aligned).  bias: f32 [heads, 2 bias_range + 1] or NULL, at most 32 KB per key head.
+ * nothing to attend to is 0.  q, k, v, o: 16-bit (TD_F16 | TD_BF16), head_dim 64 or 128 contiguous; strides[8] = token and
+ * head strides of q, k, v, o in elements (multiples of 8; pointers 16-byte aligned).  bias: f32 [heads, 2 bias_range + 1] or NULL, at most 32 KB per key head.
  * td_attn_packed_plan (host only): the lengths of the sequences -> work table (records of 8 int32; call with table = NULL for
  * counts = {tile items, few-row items, joins, partial rows, query tokens, key tokens}; records = the first three added up).  The
  * table goes to the device unchanged and is valid for every call with these lengths, heads and causality.  td_attn_packed trusts
  * it: q / k / v / o must hold the planned tokens.  ws: f32 [kv_heads * partial rows * (head_dim + 2)] (NULL when that is 0). */
 int td_attn_packed_plan(const int64_t* lens_q, const int64_t* lens_k, int64_t nseq, int heads, int kv_heads, int causal, int32_t* table,
                         int64_t capacity, int64_t* counts);
-int td_attn_packed(const void* q, int64_t q_ts, int64_t q_hs, const void* k, int64_t k_ts, int64_t k_hs, const void* v, int64_t v_ts,
-                   int64_t v_hs, void* o, int64_t o_ts, int64_t o_hs, int dtype, int heads, int kv_heads, int head_dim, float scale,
-                   int causal, const float* bias, int bias_range, const int32_t* table, const int64_t* counts, float* ws,
-                   td_stream_t stream);
+int td_attn_packed(const void* q, const void* k, const void* v, void* o, const int64_t* strides, int dtype, int heads, int kv_heads,
+                   int head_dim, float scale, int causal, const float* bias, int bias_range, const int32_t* table, const int64_t* counts,
+                   float* ws, td_stream_t stream);
 
 /* ---- low-rank adapters of many requests (csrc/lora.hip) ----
  * out[r] = y[r] + scale_i B_i (A_i x[r]) for rows r of a request with adapter i; out[r] = y[r] for one without (id -1; not touched

@@ -78,7 +78,7 @@ def test_attention_plan_refusals():
 
 def test_attention_refuses_cpu_tensors():
     class Plan:
-        heads, kv_heads, head_dim = 2, 2, 64
+        heads, kv_heads, head_dim, device = 2, 2, 64, torch.device("cuda", 0)
     q = torch.zeros(3, 2, 64, dtype=torch.bfloat16)
     with pytest.raises(L.TurboDiffusionAMDError):
         ops.packed_attention(q, q, q, Plan())

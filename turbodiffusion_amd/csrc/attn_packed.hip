@@ -462,17 +462,16 @@ static void ap_launch(const ApParams& p, int64_t n, int bias_bytes, hipStream_t 
   attn_packed_kernel<DT, D, FEW, BIAS><<<(unsigned)(n * p.Hkv), 256, tiles + bias_bytes, st>>>(p);
 }
 
-extern "C" int td_attn_packed(const void* q, int64_t q_ts, int64_t q_hs, const void* k, int64_t k_ts, int64_t k_hs, const void* v,
-                              int64_t v_ts, int64_t v_hs, void* o, int64_t o_ts, int64_t o_hs, int dtype, int heads, int kv_heads,
+extern "C" int td_attn_packed(const void* q, const void* k, const void* v, void* o, const int64_t* strides, int dtype, int heads, int kv_heads,
                               int head_dim, float scale, int causal, const float* bias, int bias_range, const int32_t* table,
                               const int64_t* counts, float* ws, td_stream_t stream) {
-  TD_REQUIRE(q && o && counts && table, TD_ERR_INVALID, "td_attn_packed: null pointer");
+  TD_REQUIRE(q && o && counts && table && strides, TD_ERR_INVALID, "td_attn_packed: null pointer");
   TD_REQUIRE(dtype == TD_BF16 || dtype == TD_F16, TD_ERR_UNSUPPORTED, "td_attn_packed: dtype %d", dtype);
   TD_REQUIRE(head_dim == 64 || head_dim == 128, TD_ERR_UNSUPPORTED, "td_attn_packed: head_dim = %d (64 or 128)", head_dim);
   TD_REQUIRE(kv_heads > 0 && heads > 0 && heads % kv_heads == 0, TD_ERR_INVALID, "td_attn_packed: %d heads over %d key heads", heads, kv_heads);
-  const int64_t st_[8] = {q_ts, q_hs, k_ts, k_hs, v_ts, v_hs, o_ts, o_hs};
-  for (int64_t s : st_) TD_REQUIRE(s >= 0 && s % 8 == 0, TD_ERR_UNSUPPORTED, "td_attn_packed: stride %lld (a multiple of 8 elements)", (long long)s);
-  TD_REQUIRE(k_ts < (1 << 24) && v_ts < (1 << 24), TD_ERR_UNSUPPORTED, "td_attn_packed: key / value token stride of 2^24 elements or more");
+  for (int i = 0; i < 8; ++i)
+    TD_REQUIRE(strides[i] >= 0 && strides[i] % 8 == 0, TD_ERR_UNSUPPORTED, "td_attn_packed: stride %lld (a multiple of 8 elements)", (long long)strides[i]);
+  TD_REQUIRE(strides[2] < (1 << 24) && strides[4] < (1 << 24), TD_ERR_UNSUPPORTED, "td_attn_packed: key / value token stride of 2^24 elements or more");
   TD_REQUIRE((((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)o | (uintptr_t)ws) & 15) == 0, TD_ERR_UNSUPPORTED,
              "td_attn_packed: pointers must be 16-byte aligned");
   TD_REQUIRE(scale > 0.f && scale <= 3.0e38f, TD_ERR_INVALID, "td_attn_packed: scale must be positive and finite");
@@ -490,7 +489,8 @@ extern "C" int td_attn_packed(const void* q, int64_t q_ts, int64_t q_hs, const v
   }
   ApParams p;
   p.q = (const uint16_t*)q; p.k = (const uint16_t*)k; p.v = (const uint16_t*)v; p.o = (uint16_t*)o;
-  p.q_ts = q_ts; p.q_hs = q_hs; p.k_ts = k_ts; p.k_hs = k_hs; p.v_ts = v_ts; p.v_hs = v_hs; p.o_ts = o_ts; p.o_hs = o_hs;
+  p.q_ts = strides[0]; p.q_hs = strides[1]; p.k_ts = strides[2]; p.k_hs = strides[3];
+  p.v_ts = strides[4]; p.v_hs = strides[5]; p.o_ts = strides[6]; p.o_hs = strides[7];
   p.bias = bias; p.R = bias_range; p.items = reinterpret_cast<const ApItem*>(table);
   p.po = ws; p.pml = ws ? ws + (int64_t)kv_heads * wr * head_dim : nullptr; p.ws_rows = wr;
   p.Hkv = kv_heads; p.G = G; p.causal = causal ? 1 : 0;

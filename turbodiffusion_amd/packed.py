@@ -16,6 +16,10 @@ from .kernels import call, _f32c
 from ._lib import dt_code, ptr, require_gpu, stream_ptr
 
 
+# torch.cuda.current_device / current_stream without the Python around them: 4 of a small call's 13 us
+_current_device, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+
+
 def _lengths(lens, what):
     if isinstance(lens, torch.Tensor):
         if lens.dim() != 1 or lens.is_floating_point() or lens.dtype == torch.bool:
@@ -33,7 +37,7 @@ def _i64_array(values):
 
 
 class _Plan:
-    """A host-made table of int32 records on ``device``; ``use()`` ties it to the stream a call runs on."""
+    """A host-made table of int32 records on ``device``."""
 
     def _upload(self, host, device):
         self.device = torch.device(device)
@@ -42,24 +46,31 @@ class _Plan:
         if self.device.index is None:
             self.device = torch.device("cuda", torch.cuda.current_device())
         with torch.cuda.device(self.device):
-            self._stream = torch.cuda.current_stream()
+            self._stream = torch.cuda.current_stream().cuda_stream
             self.table = host.to(self.device)          # synchronous: complete for every stream
 
-    def use(self):
-        s = torch.cuda.current_stream(self.device)
-        if s != self._stream:
-            self.table.record_stream(s)
-        return ctypes.c_void_p(s.cuda_stream)
+    def _launch(self, fn):
+        """``fn(stream)`` with the plan's device current; the table stays allocated while that stream needs it"""
+        if _current_device() != self.device.index:
+            with torch.cuda.device(self.device):
+                return self._launch(fn)
+        stream = _raw_stream(self.device.index)
+        if stream != self._stream:
+            self.table.record_stream(torch.cuda.current_stream())
+        fn(stream)
 
 
-def _guard(device):
-    """launch on ``device`` whatever the current device is"""
-    return torch.cuda.device(device)
-
-
-def _no_grad_inputs(*tensors):
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise RuntimeError("inference only: an input requires gradients (call under torch.no_grad() or detach it)")
+def _check_tensors(what, dev, *tensors):
+    """GPU tensors on ``dev`` that want no gradient (None: an argument left out)"""
+    grad = torch.is_grad_enabled()
+    for t in tensors:
+        if t is None:
+            continue
+        if t.device != dev:
+            require_gpu(t)
+            raise ValueError(f"{what}: the plan and every tensor must be on one device ({dev}, got {t.device})")
+        if grad and t.requires_grad:
+            raise RuntimeError(f"{what} is inference only: an input requires gradients (call under torch.no_grad() or detach it)")
 
 
 def _overlap(a, b):
@@ -95,16 +106,18 @@ class AttentionPlan(_Plan):
         host = torch.zeros(max(1, n), 8, dtype=torch.int32)
         L.call("td_attn_packed_plan", *args, ptr(host), n, self._counts)
         self.tokens, self.tokens_k = self._counts[4], self._counts[5]
+        self._strides = {}                             # stride tuples seen, as C arrays
         self.ws_floats = self._counts[3] * self.kv_heads * (self.head_dim + 2)
         self._upload(host, device)
 
 
 def _packed_strides(t, tokens, heads, head_dim, what):
-    if t.dim() != 3 or tuple(t.shape) != (tokens, heads, head_dim):
+    if t.shape != (tokens, heads, head_dim):
         raise ValueError(f"packed_attention: {what} is {tuple(t.shape)}, the plan wants ({tokens}, {heads}, {head_dim})")
-    if t.stride(2) != 1:
+    ts, hs, ds = t.stride()
+    if ds != 1:
         raise ValueError(f"packed_attention: the last dimension of {what} must be contiguous")
-    return (t.stride(0) if tokens > 1 else 0), (t.stride(1) if heads > 1 else 0)   # a stride that no second element uses is arbitrary
+    return (ts if tokens > 1 else 0), (hs if heads > 1 else 0)   # a stride that no second element uses is arbitrary
 
 
 def packed_attention(q, k, v, plan, scale=None, bias=None, out=None):
@@ -119,16 +132,12 @@ def packed_attention(q, k, v, plan, scale=None, bias=None, out=None):
     ``out``: written instead of a new tensor; it may not overlap the inputs.  Any stream, capturable; the plan must outlive a
     captured graph."""
     H, Hkv, D = plan.heads, plan.kv_heads, plan.head_dim
-    require_gpu(q, k, v, bias, out)
-    _no_grad_inputs(q, k, v, bias)
-    if not (q.dtype == k.dtype == v.dtype) or q.dtype not in (torch.bfloat16, torch.float16):
+    dev, dt = plan.device, q.dtype
+    _check_tensors("packed_attention", dev, q, k, v, bias, out)
+    if k.dtype != dt or v.dtype != dt or (dt != torch.bfloat16 and dt != torch.float16):
         raise TypeError(f"packed_attention: q, k, v must all be bf16 or all f16 (got {q.dtype}, {k.dtype}, {v.dtype})")
-    dev = plan.device
-    if any(t is not None and t.device != dev for t in (q, k, v, bias, out)):
-        raise ValueError(f"packed_attention: the plan and every tensor must be on one device ({dev})")
-    qs = _packed_strides(q, plan.tokens, H, D, "q")
-    ks = _packed_strides(k, plan.tokens_k, Hkv, D, "k")
-    vs = _packed_strides(v, plan.tokens_k, Hkv, D, "v")
+    strides = (*_packed_strides(q, plan.tokens, H, D, "q"), *_packed_strides(k, plan.tokens_k, Hkv, D, "k"),
+               *_packed_strides(v, plan.tokens_k, Hkv, D, "v"))
     R = 0
     if bias is not None:
         _f32c(bias, "bias")
@@ -139,24 +148,27 @@ def packed_attention(q, k, v, plan, scale=None, bias=None, out=None):
     if not 0.0 < scale < math.inf:
         raise ValueError(f"packed_attention: scale must be positive and finite, got {scale}")
     if out is None:
-        out = torch.empty((plan.tokens, H, D), dtype=q.dtype, device=dev)
-        os_ = (H * D, D)
+        out = torch.empty((plan.tokens, H, D), dtype=dt, device=dev)
+        strides += (H * D, D)
     else:
-        if out.dtype != q.dtype:
-            raise TypeError(f"packed_attention: out is {out.dtype}, the inputs {q.dtype}")
-        os_ = _packed_strides(out, plan.tokens, H, D, "out")
-        ts, hs = os_
+        if out.dtype != dt:
+            raise TypeError(f"packed_attention: out is {out.dtype}, the inputs {dt}")
+        ts, hs = _packed_strides(out, plan.tokens, H, D, "out")
         if not ((H == 1 or hs >= D) and (plan.tokens <= 1 or ts >= (H - 1) * hs + D)
                 or (plan.tokens <= 1 or ts >= D) and (H == 1 or hs >= (plan.tokens - 1) * ts + D)):
             raise ValueError("packed_attention: out overlaps itself")
         if any(_overlap(out, t) for t in (q, k, v)):
             raise ValueError("packed_attention: out overlaps an input")
+        strides += (ts, hs)
     if plan.tokens == 0:
         return out
-    with _guard(dev):
-        ws = torch.empty(plan.ws_floats, dtype=torch.float32, device=dev) if plan.ws_floats else None
-        call("td_attn_packed", ptr(q), *qs, ptr(k), *ks, ptr(v), *vs, ptr(out), *os_, dt_code(q.dtype), H, Hkv, D, scale,
-             1 if plan.causal else 0, ptr(bias), R, ptr(plan.table), plan._counts, ptr(ws), plan.use())
+    packed_strides = plan._strides.get(strides)
+    if packed_strides is None:
+        packed_strides = plan._strides[strides] = _i64_array(strides)
+    ws = torch.empty(plan.ws_floats, dtype=torch.float32, device=dev) if plan.ws_floats else None
+    plan._launch(lambda stream: call(
+        "td_attn_packed", q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), packed_strides, dt_code(dt), H, Hkv, D, scale, plan.causal,
+        None if bias is None else bias.data_ptr(), R, plan.table.data_ptr(), plan._counts, None if ws is None else ws.data_ptr(), stream))
     return out
 
 
@@ -198,7 +210,7 @@ class AdapterBank:
         r8 = [-(-r // 8) * 8 for r in self.ranks]
         self.max_rank = max(r8)
         k32, n32 = -(-self.k // 32) * 32, -(-self.n // 32) * 32
-        with _guard(self.device):
+        with torch.cuda.device(self.device):
             self.data = torch.empty(sum(r * (k32 + n32) for r in r8) + self.SPARE, dtype=self.dtype, device=self.device)
             meta = torch.zeros(len(pairs), 3, dtype=torch.int64)
             off, st = 0, stream_ptr()
@@ -246,11 +258,12 @@ class AdapterPlan(_Plan):
 
 
 def _rows(t, rows, cols, what):
-    if t.dim() != 2 or tuple(t.shape) != (rows, cols):
+    if t.shape != (rows, cols):
         raise ValueError(f"lora_add: {what} is {tuple(t.shape)}, wanted ({rows}, {cols})")
-    if t.stride(1) != 1:
+    ld, one = t.stride()
+    if one != 1:
         raise ValueError(f"lora_add: the last dimension of {what} must be contiguous")
-    return t.stride(0) if rows > 1 else 0
+    return ld if rows > 1 else 0
 
 
 def lora_add(y, x, bank, plan, out=None):
@@ -259,11 +272,8 @@ def lora_add(y, x, bank, plan, out=None):
     all requests share (``int8_linear``, ``Int8Linear``, a 16-bit GEMM).  ``out``: written instead of a new tensor; ``out=y`` adds
     in place; any other overlap is refused.  x A^T is summed in fp32 and, scaled, rounded once to the adapters' type; the update
     is added in fp32 and rounded with the result.  Any stream, capturable; bank and plan must outlive a captured graph."""
-    require_gpu(y, x, out)
-    _no_grad_inputs(y, x)
     dev = plan.device
-    if any(t is not None and t.device != dev for t in (y, x, out, bank.data)):
-        raise ValueError(f"lora_add: bank, plan and every tensor must be on one device ({dev})")
+    _check_tensors("lora_add", dev, y, x, out, bank.data)
     if x.dtype != bank.dtype or y.dtype != bank.dtype:
         raise TypeError(f"lora_add: x is {x.dtype}, y {y.dtype}, the adapters {bank.dtype}")
     if plan._counts[4] > len(bank):
@@ -282,9 +292,9 @@ def lora_add(y, x, bank, plan, out=None):
             raise ValueError("lora_add: out overlaps an input (out=y alone may)")
     if plan.rows == 0:
         return out
-    with _guard(dev):
-        n = plan.workspace(bank.k, bank.max_rank)
-        ws = torch.empty(n, dtype=torch.float32, device=dev) if n else None
-        call("td_lora_add", ptr(x), ldx, ptr(y), ldy, ptr(out), ldo, dt_code(y.dtype), bank.k, bank.n, ptr(bank.data), ptr(bank.meta),
-             len(bank), bank.max_rank, ptr(plan.table), plan._counts, ptr(ws), plan.use())
+    n = plan.workspace(bank.k, bank.max_rank)
+    ws = torch.empty(n, dtype=torch.float32, device=dev) if n else None
+    plan._launch(lambda stream: call(
+        "td_lora_add", x.data_ptr(), ldx, y.data_ptr(), ldy, out.data_ptr(), ldo, dt_code(y.dtype), bank.k, bank.n, bank.data.data_ptr(),
+        bank.meta.data_ptr(), len(bank), bank.max_rank, plan.table.data_ptr(), plan._counts, None if ws is None else ws.data_ptr(), stream))
     return out
