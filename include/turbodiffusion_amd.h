@@ -509,7 +509,7 @@ int td_sla_linear_kv_final_packed(const float* ws_kv, const float* ws_ks, int nc
  * o[i, h] = sum_j softmax_j(scale q[i, h] . k[j, h / G] + bias[h, clamp(j - pos_i, -bias_range, bias_range) + bias_range]) v[j, h / G]
  * over the keys of row i's own sequence; G = heads / kv_heads; pos_i = i + k_len - q_len; only j <= pos_i when causal.  A row with
  * nothing to attend to is 0.  q, k, v, o: 16-bit (TD_F16 | TD_BF16), head_dim 64 or 128 contiguous; strides[8] = token and
- * head strides of q, k, v, o in elements (multiples of 8; pointers 16-byte aligned).  bias: f32 [heads, 2 bias_range + 1] or NULL, at most 32 KB per key head.
+ * head strides of q, k, v, o in elements (multiples of 8; pointers 16-byte aligned).  bias: f32 [heads, 2 bias_range + 1] or NULL; G (2 bias_range + 193) <= 8192.
  * td_attn_packed_plan (host only): the lengths of the sequences -> work table (records of 8 int32; call with table = NULL for
  * counts = {tile items, few-row items, joins, partial rows, query tokens, key tokens}; records = the first three added up).  The
  * table goes to the device unchanged and is valid for every call with these lengths, heads and causality.  td_attn_packed trusts

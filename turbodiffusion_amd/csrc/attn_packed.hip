@@ -30,6 +30,8 @@ typedef __attribute__((address_space(3))) ap_v4s* ap_trptr_t;
 
 #define AP_ROWS 128        // rows of a tile item
 #define AP_FEW 32          // rows of a few item
+#define AP_FEW_KEYS 128    // ... of sequences with more keys than this; with fewer the four waves would not all have a tile
+#define AP_PAD 96          // the bias table repeats its ends: distances within a key tile of the range need no clamp
 #define AP_TAU 8.0f        // the reference maximum moves only when exceeded by 2^8: P <= 256 fits f16 / bf16 and the fp32 sum
 
 struct ApItem {            // one workgroup's work per key head: rows [row0, ..) of a sequence over keys [key0, key1)
@@ -44,6 +46,7 @@ struct ApParams {
   const ApItem* items;
   float* po; float* pml; int64_t ws_rows;                    // partials [Hkv][ws_rows][D], [Hkv][ws_rows][2] (max, sum)
   int Hkv, G, causal;
+  uint32_t gmagic;                                           // ceil(2^32 / G): x / G = mulhi(x, gmagic) for x G < 2^32 (G > 1)
   float c;                                                   // scale * log2(e)
 };
 
@@ -76,6 +79,10 @@ __device__ __forceinline__ void ap_dma(const void* base, uint32_t bytes, char* l
   __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (ap_lptr_t)lds, 16, off, 0, 0, 0);
 }
 
+__device__ __forceinline__ void ap_dma_ptr(const void* src, char* lds) {   // the same from an address per lane
+  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src, (ap_lptr_t)lds, 16, 0, 0);
+}
+
 template <int DT, int D, bool FEW, bool BIAS>
 __global__ __launch_bounds__(256, FEW ? 1 : 2) void attn_packed_kernel(const ApParams p) {
   constexpr int NB = FEW && D == 128 ? 1 : 2;       // 32-key blocks per tile
@@ -96,10 +103,18 @@ __global__ __launch_bounds__(256, FEW ? 1 : 2) void attn_packed_kernel(const ApP
   // ---- this lane's row ----
   const int nrows = it.q_len * p.G;
   const int wrow0 = it.row0 + (FEW ? 0 : 32 * wave);
+  const int q_first = it.row0 / p.G, g_first = it.row0 - q_first * p.G;
+  // query and head of row it.row0 + x: x is less than a tile, so the division is one multiplication
+  auto split_row = [&](int x, int& q, int& h) {
+    const int y = g_first + min(x, nrows - 1 - it.row0);
+    const int d = p.G > 1 ? (int)__umulhi((uint32_t)y, p.gmagic) : y;
+    q = q_first + d;
+    h = y - d * p.G;
+  };
   const int row = wrow0 + (lane & 31);
   const bool valid = row < nrows;
-  const int rc = min(row, nrows - 1);
-  const int qi = rc / p.G, g = rc - qi * p.G;
+  int qi, g;
+  split_row(row - it.row0, qi, g);
   const int shift = it.k_len - it.q_len;
   const int pos = qi + shift;
   const int kmax = p.causal ? min(it.key1, pos + 1) : it.key1;         // keys [key0, kmax) of this row
@@ -110,23 +125,34 @@ __global__ __launch_bounds__(256, FEW ? 1 : 2) void attn_packed_kernel(const ApP
   const int wmin = p.causal ? min(it.key1, wfirst + 1) : it.key1;
   const int wmax = wrow0 >= nrows ? 0 : (p.causal ? min(it.key1, wlast + 1) : it.key1);
 
-  // ---- Q^T fragments: B operand, lane = row, 8 consecutive d per register quad ----
-  v4i qf[KK];
-  {
-    const uint16_t* qp = p.q + (int64_t)(it.q_begin + qi) * p.q_ts + (int64_t)(kvh * p.G + g) * p.q_hs + 8 * half;
+  const uint16_t* const qhead = p.q + (int64_t)it.q_begin * p.q_ts + (int64_t)kvh * p.G * p.q_hs;
+  char* const qstage = smem + STAGE + wave * 32 * ROWB;                // tile kernel: the wave's 32 rows, in stage 1 until tile 1 comes
+  v4i qf[KK];                                                          // Q^T fragments: B operand, lane = row, 8 consecutive d each
+  if constexpr (FEW) {
+    const uint16_t* qp = qhead + qi * p.q_ts + g * p.q_hs + 8 * half;
 #pragma unroll
     for (int kk = 0; kk < KK; ++kk) qf[kk] = *reinterpret_cast<const v4i*>(qp + 16 * kk);
+  } else {                                                             // whole rows at a time: memory likes full lines
+    constexpr int RP = 1024 / ROWB;
+#pragma unroll
+    for (int t = 0; t < 32 / RP; ++t) {
+      const int x = RP * t + lane / (ROWB / 16);
+      int q2, g2;
+      split_row(wrow0 - it.row0 + x, q2, g2);
+      ap_dma_ptr(qhead + q2 * p.q_ts + g2 * p.q_hs + 8 * ((lane & (ROWB / 16 - 1)) ^ ap_kx<D>(x)), qstage + t * 1024);
+    }
   }
+  const int bn = 2 * p.R + 1 + 2 * AP_PAD;
   if constexpr (BIAS) {   // exp2 domain; the type's lowest values as a finite low (a row of nothing else stays a uniform row)
-    const int n = p.G * (2 * p.R + 1);
-    const float* b = p.bias + (int64_t)kvh * n;
-    for (int i = tid; i < n; i += 256) {
-      const float x = b[i];
+    const float* b = p.bias + (int64_t)kvh * p.G * (2 * p.R + 1);
+    for (int i = tid; i < p.G * bn; i += 256) {
+      const int h = i / bn, d = max(0, min(2 * p.R, i - h * bn - AP_PAD));
+      const float x = b[h * (2 * p.R + 1) + d];
       lbias[i] = fabsf(x) > 1e37f && fabsf(x) < INFINITY ? copysignf(1e37f, x) : x * 1.4426950408889634f;
     }
     __syncthreads();
   }
-  const float* const lb = lbias + (BIAS ? g * (2 * p.R + 1) + p.R : 0);
+  const float* const lb = lbias + (BIAS ? g * bn + p.R + AP_PAD : 0);   // lb[key - position]
   const float b_far_past = BIAS ? lb[-p.R] : 0.f, b_far_next = BIAS ? lb[p.R] : 0.f;
 
   // ---- LDS-DMA: piece t of this wave; rows past the range re-read the last one (finite, masked) ----
@@ -188,7 +214,12 @@ __global__ __launch_bounds__(256, FEW ? 1 : 2) void attn_packed_kernel(const ApP
   const int kend = key_end;
   if (kt < kend) fetch(kt, 0);
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-  if constexpr (!FEW) __syncthreads();
+  if constexpr (!FEW) {
+    const uint32_t r = lane & 31;
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk) qf[kk] = *reinterpret_cast<const v4i*>(qstage + r * ROWB + (((half ^ ap_kx<D>(r)) << 4) ^ (kk << 5)));
+    __syncthreads();
+  }
   for (int buf = 0; kt < kend; kt += step, buf ^= 1) {
     if (kt + step < kend) fetch(kt + step, buf ^ 1);
     if (FEW || kt < wmax) {
@@ -196,31 +227,35 @@ __global__ __launch_bounds__(256, FEW ? 1 : 2) void attn_packed_kernel(const ApP
       const char* sv = sk + TILE;
       v16f s[NB];
 #pragma unroll
-      for (int b = 0; b < NB; ++b) {
+      for (int b = 0; b < NB; ++b)
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[b][r] = 0.f;
 #pragma unroll
-        for (int kk = 0; kk < KK; ++kk) {
+      for (int kk = 0; kk < KK; ++kk)     // the blocks in turn: two MFMAs in a row do not depend on each other
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
           const v4i kf = *reinterpret_cast<const v4i*>(sk + b * 32 * ROWB + krow + (kxor ^ (kk << 5)));
           s[b] = ap_mma<DT>::run(kf, qf[kk], s[b]);
         }
-      }
       // register r of block b is key kt + 32 b + 16 (r >> 3) + 8 half + (r & 7)
       if constexpr (BIAS) {
-        float far = 0.f; bool isfar = false;
-        if (kt - wlast >= p.R) { far = b_far_next; isfar = true; }
-        else if (kt + BK - 1 - wfirst <= -p.R) { far = b_far_past; isfar = true; }
-        const int d0 = kt + 8 * half - pos;
+        const bool next = kt - wlast >= p.R, past = kt + BK - 1 - wfirst <= -p.R;
+        if (next || past) {                                     // the whole tile lies beyond the range: one value a row
+          const float far = next ? b_far_next : b_far_past;
 #pragma unroll
-        for (int b = 0; b < NB; ++b)
+          for (int b = 0; b < NB; ++b)
 #pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            float bb = far;
-            if (!isfar) bb = lb[max(-p.R, min(p.R, d0 + 32 * b + 16 * (r >> 3) + (r & 7)))];
-            s[b][r] = fmaf(s[b][r], p.c, bb);
-          }
+            for (int r = 0; r < 16; ++r) s[b][r] = fmaf(s[b][r], p.c, far);
+        } else {                                                // |key - position| < R + 96 everywhere in the tile
+          const float* d = lb + (kt + 8 * half - pos);
+#pragma unroll
+          for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[b][r] = fmaf(s[b][r], p.c, d[32 * b + 16 * (r >> 3) + (r & 7)]);
+        }
       }
       if (kt + BK > wmin) {
+        asm volatile("");                 // a branch: as selects the mask would cost every tile 96 instructions
         const int lim = kmax - kt - 8 * half;
 #pragma unroll
         for (int b = 0; b < NB; ++b)
@@ -326,8 +361,8 @@ __global__ __launch_bounds__(256, FEW ? 1 : 2) void attn_packed_kernel(const ApP
       }
     }
   } else {
-    if (!valid) return;
     if (it.slot >= 0) {
+      if (!valid) return;
       const int64_t pr = (int64_t)kvh * p.ws_rows + it.slot + 32 * wave + (lane & 31);
 #pragma unroll
       for (int d = 0; d < DB; ++d)
@@ -335,9 +370,10 @@ __global__ __launch_bounds__(256, FEW ? 1 : 2) void attn_packed_kernel(const ApP
         for (int r = 0; r < 16; r += 4)
           *reinterpret_cast<float4*>(p.po + pr * D + 32 * d + 2 * r + 4 * half) = make_float4(acc[d][r], acc[d][r + 1], acc[d][r + 2], acc[d][r + 3]);
       if (half == 0) { p.pml[pr * 2] = m; p.pml[pr * 2 + 1] = l; }
-    } else {
+    } else {   // through the wave's own 32 rows of LDS (every wave is done with the stages): whole rows go out
       const float inv = l == 0.f ? 0.f : 1.0f / l;
-      uint16_t* op = p.o + (int64_t)(it.q_begin + qi) * p.o_ts + (int64_t)(kvh * p.G + g) * p.o_hs + 8 * half;
+      char* const ost = smem + wave * 32 * ROWB;
+      const uint32_t r32 = lane & 31;
 #pragma unroll
       for (int d = 0; d < DB; ++d)
 #pragma unroll
@@ -347,8 +383,19 @@ __global__ __launch_bounds__(256, FEW ? 1 : 2) void attn_packed_kernel(const ApP
           const uint32_t b0 = pack2<DT>(acc[d][r + 4] * inv, acc[d][r + 5] * inv), b1 = pack2<DT>(acc[d][r + 6] * inv, acc[d][r + 7] * inv);
           const auto s0 = __builtin_amdgcn_permlane32_swap(a0, b0, false, false);
           const auto s1 = __builtin_amdgcn_permlane32_swap(a1, b1, false, false);
-          *reinterpret_cast<uint4*>(op + 32 * d + 16 * j) = make_uint4(s0[0], s1[0], s0[1], s1[1]);
+          *reinterpret_cast<uint4*>(ost + r32 * ROWB + (((4 * d + 2 * j + half) ^ ap_kx<D>(r32)) << 4)) = make_uint4(s0[0], s1[0], s0[1], s1[1]);
         }
+      __builtin_amdgcn_wave_barrier();
+      uint16_t* const ohead = p.o + (int64_t)it.q_begin * p.o_ts + (int64_t)kvh * p.G * p.o_hs;
+      constexpr int RP = 1024 / ROWB;
+#pragma unroll
+      for (int t = 0; t < 32 / RP; ++t) {
+        const uint32_t x = RP * t + lane / (ROWB / 16), c = lane & (ROWB / 16 - 1);
+        int q2, g2;
+        split_row(wrow0 - it.row0 + x, q2, g2);
+        const uint4 v = *reinterpret_cast<const uint4*>(ost + x * ROWB + ((c ^ ap_kx<D>(x)) << 4));
+        if (wrow0 + (int)x < nrows) *reinterpret_cast<uint4*>(ohead + q2 * p.o_ts + g2 * p.o_hs + 8 * c) = v;
+      }
     }
   }
 }
@@ -401,13 +448,20 @@ extern "C" int td_attn_packed_plan(const int64_t* lens_q, const int64_t* lens_k,
     std::vector<Work> work[2];
     std::vector<ApJoin> joins;
     int64_t keys_total[2] = {0, 0};
+    // few rows over few keys go with whatever kernel the others need
+    bool few_short = false, any_tile = false;
+    for (int64_t s = 0; s < nseq; ++s) {
+      any_tile |= lens_q[s] * G > AP_FEW;
+      few_short |= lens_q[s] > 0 && lens_q[s] * G <= AP_FEW && lens_k[s] > AP_FEW_KEYS;
+    }
+    few_short &= !any_tile;
     // pass 0 counts the keys each kernel reads, pass 1 emits items of at most `chunk` keys
     int64_t chunk[2] = {0, 0}, ws_rows = 0;
     for (int pass = 0; pass < 2; ++pass) {
       int64_t q0 = 0, k0 = 0;
       for (int64_t s = 0; s < nseq; ++s) {
         const int64_t ql = lens_q[s], kl = lens_k[s], rows = ql * G;
-        const int few = rows <= AP_FEW;
+        const int few = rows <= AP_FEW && (kl > AP_FEW_KEYS || few_short);
         const int64_t tr = few ? AP_FEW : AP_ROWS;
         for (int64_t r0 = 0; r0 < rows; r0 += tr) {
           const int64_t last = std::min(r0 + tr, rows) - 1;
@@ -481,11 +535,12 @@ extern "C" int td_attn_packed(const void* q, const void* k, const void* v, void*
   TD_REQUIRE(nt * kv_heads < (1ll << 31) && nf * kv_heads < (1ll << 31) && nj < (1ll << 31) && kv_heads <= 65535, TD_ERR_UNSUPPORTED,
              "td_attn_packed: more than 2^31 workgroups");
   const int G = heads / kv_heads;
+  TD_REQUIRE(G <= 16384, TD_ERR_UNSUPPORTED, "td_attn_packed: %d heads share a key head", G);
   int bias_bytes = 0;
   if (bias) {
-    TD_REQUIRE(bias_range >= 0 && bias_range < 8192 && (int64_t)G * (2 * bias_range + 1) * 4 <= 32768, TD_ERR_UNSUPPORTED,
+    TD_REQUIRE(bias_range >= 0 && bias_range < 8192 && (int64_t)G * (2 * bias_range + 1 + 2 * AP_PAD) * 4 <= 32768, TD_ERR_UNSUPPORTED,
                "td_attn_packed: bias of range %d for %d heads per key head exceeds 32 KB", bias_range, G);
-    bias_bytes = G * (2 * bias_range + 1) * 4;
+    bias_bytes = G * (2 * bias_range + 1 + 2 * AP_PAD) * 4;
   }
   ApParams p;
   p.q = (const uint16_t*)q; p.k = (const uint16_t*)k; p.v = (const uint16_t*)v; p.o = (uint16_t*)o;
@@ -494,6 +549,7 @@ extern "C" int td_attn_packed(const void* q, const void* k, const void* v, void*
   p.bias = bias; p.R = bias_range; p.items = reinterpret_cast<const ApItem*>(table);
   p.po = ws; p.pml = ws ? ws + (int64_t)kv_heads * wr * head_dim : nullptr; p.ws_rows = wr;
   p.Hkv = kv_heads; p.G = G; p.causal = causal ? 1 : 0;
+  p.gmagic = G > 1 ? (uint32_t)(((1ull << 32) + G - 1) / G) : 0;
   p.c = scale * 1.4426950408889634f;
   hipStream_t st = (hipStream_t)stream;
   for (int few = 0; few < 2; ++few) {
