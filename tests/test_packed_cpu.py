@@ -30,15 +30,15 @@ def test_attention_plan_covers_every_visible_key_once(seed):
         causal = rng.randint(0, 1)
         t, (tiles, few, joins, ws_rows, tq, tk) = attention_table(lq, lk, kv * G, kv, causal)
         assert (tq, tk) == (sum(lq), sum(lk))
-        starts = {}
-        for s in range(ns):
-            if lq[s]:
-                starts[sum(lq[:s])] = s
+        starts = {sum(lq[:s]): s for s in range(ns) if lq[s]}
         seen = {}
-        for i, (qb, kb, ql, kl, row0, a, b, slot) in enumerate(t[:tiles + few]):
+        for i, (token, head0, rows, pos, kb, a, b, slot) in enumerate(t[:tiles + few]):
+            qb = max(x for x in starts if x <= token)
             s = starts[qb]
-            assert (kb, ql, kl) == (sum(lk[:s]), lq[s], lk[s]) and 0 <= a <= b <= kl
-            for row in range(row0, min(row0 + (128 if i < tiles else 32), ql * G)):
+            row0 = (token - qb) * G + head0
+            assert kb == sum(lk[:s]) and 0 <= head0 < G and pos == token - qb + lk[s] - lq[s] and 0 <= a <= b <= lk[s]
+            assert rows == min(128 if i < tiles else 32, lq[s] * G - row0) > 0
+            for row in range(row0, row0 + rows):
                 seen.setdefault((s, row), []).append((a, b, slot))
         for s in range(ns):
             for row in range(lq[s] * G):
@@ -49,8 +49,8 @@ def test_attention_plan_covers_every_visible_key_once(seed):
                     at = b
                 assert end <= at <= lk[s]
         assert not seen
-        slots = [j[4] + i * j[6] for j in t[tiles + few:] for i in range(j[5])]
-        rows = [x + r for j in t[tiles + few:] for x in range(j[4], j[4] + j[5] * j[6], j[6]) for r in range(j[6])]
+        slots = [j[3] + i * j[5] for j in t[tiles + few:] for i in range(j[4])]
+        rows = [x + r for j in t[tiles + few:] for x in range(j[3], j[3] + j[4] * j[5], j[5]) for r in range(j[5])]
         assert sorted(slots) == sorted(x[7] for x in t[:tiles + few] if x[7] >= 0)
         assert len(set(rows)) == len(rows) and (not rows or max(rows) < ws_rows)
 

@@ -34,16 +34,17 @@ typedef __attribute__((address_space(3))) ap_v4s* ap_trptr_t;
 #define AP_PAD 96          // the bias table repeats its ends: distances within a key tile of the range need no clamp
 #define AP_TAU 8.0f        // the reference maximum moves only when exceeded by 2^8: P <= 256 fits f16 / bf16 and the fp32 sum
 
-struct ApItem {            // one workgroup's work per key head: rows [row0, ..) of a sequence over keys [key0, key1)
-  int32_t q_begin, k_begin, q_len, k_len, row0, key0, key1, slot;   // slot: row in the partial buffer, -1 = writes o
-};
-struct ApJoin { int32_t q_begin, q_len, row0, rows, slot, splits, tile_rows, pad; };
+// One workgroup's work per key head: `rows` rows from head `head0` of query token `token`, which stands at position `pos` of its
+// sequence, over keys [key0, key1) of the sequence whose first key token is k_begin.  slot: row in the partial buffer, -1 = writes o
+struct ApItem { int32_t token, head0, rows, pos, k_begin, key0, key1, slot; };
+struct ApJoin { int32_t token, head0, rows, slot, splits, tile_rows, pad0, pad1; };
+#define AP_GRID_Y 32768    // items per grid.z
 
 struct ApParams {
   const uint16_t *q, *k, *v; uint16_t* o;
   int64_t q_ts, q_hs, k_ts, k_hs, v_ts, v_hs, o_ts, o_hs;   // token / head strides, elements
   const float* bias; int R;                                  // [H, 2R + 1] or null
-  const ApItem* items;
+  const ApItem* items; int n_items;
   float* po; float* pml; int64_t ws_rows;                    // partials [Hkv][ws_rows][D], [Hkv][ws_rows][2] (max, sum)
   int Hkv, G, causal;
   uint32_t gmagic;                                           // ceil(2^32 / G): x / G = mulhi(x, gmagic) for x G < 2^32 (G > 1)
@@ -83,116 +84,234 @@ __device__ __forceinline__ void ap_dma_ptr(const void* src, char* lds) {   // th
   __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src, (ap_lptr_t)lds, 16, 0, 0);
 }
 
-template <int DT, int D, bool FEW, bool BIAS>
-__global__ __launch_bounds__(256, FEW ? 1 : 2) void attn_packed_kernel(const ApParams p) {
-  constexpr int NB = FEW && D == 128 ? 1 : 2;       // 32-key blocks per tile
-  constexpr int BK = 32 * NB;
-  constexpr int ROWB = 2 * D;
-  constexpr int TILE = BK * ROWB;                   // bytes of a K or V tile
-  constexpr int STAGE = 2 * TILE;
-  constexpr int PIECES = TILE / 1024 / (FEW ? 1 : 4);   // 1 KB LDS-DMA pieces per wave, K and V each
-  constexpr int RPP = 1024 / ROWB;                  // rows per piece
-  constexpr int KK = D / 16, DB = D / 32;
+// query token (from the item's) and head of a row: rows run over the heads of a token first; x is less than a tile, so the
+// division is one multiplication
+__device__ __forceinline__ void ap_split(const ApParams& p, const ApItem& it, int x, int& q, int& h) {
+  const int y = it.head0 + x;
+  q = p.G > 1 ? (int)__umulhi((uint32_t)y, p.gmagic) : y;
+  h = y - q * p.G;
+}
+// Whole rows between memory and LDS, 16 bytes a lane: lane / (ROWB / 16) of each group of rows.  The pointer steps from group to
+// group: a step is a fixed number of tokens and heads, but for the carry from the last head to the next token.
+template <int D> struct ApRowWalk {
+  static constexpr int LPR = D / 8, RP = 64 / LPR;          // lanes per row, rows per group
+  int64_t at; int h;                                        // element offset from the item's first token and this key head's first head
+  int64_t step, carry; int dh, G;
+  __device__ __forceinline__ ApRowWalk(const ApParams& p, const ApItem& it, int x, int64_t ts, int64_t hs) : G(p.G) {
+    int q;
+    ap_split(p, it, x, q, h);
+    at = q * ts + h * hs;
+    const int dq = G > 1 ? (int)__umulhi((uint32_t)RP, p.gmagic) : RP;
+    dh = RP - dq * G;
+    step = dq * ts + dh * hs;
+    carry = ts - G * hs;
+  }
+  __device__ __forceinline__ void next() {
+    at += step;
+    h += dh;
+    if (h >= G) { h -= G; at += carry; }
+  }
+};
+
+// exp2 domain; the type's lowest values as a finite low (a row of nothing else stays a uniform row)
+__device__ __forceinline__ void ap_load_bias(const ApParams& p, int kvh, int bn, float* lbias) {
+  const float* b = p.bias + (int64_t)kvh * p.G * (2 * p.R + 1);
+  for (int h = 0; h < p.G; ++h)
+    for (int i = threadIdx.x; i < bn; i += 256) {
+      const float x = b[h * (2 * p.R + 1) + max(0, min(2 * p.R, i - AP_PAD))];
+      lbias[h * bn + i] = fabsf(x) > 1e37f && fabsf(x) < INFINITY ? copysignf(1e37f, x) : x * 1.4426950408889634f;
+    }
+}
+
+// scores of 32 N keys from kb, registers s[b][r] = key kb + 32 b + 16 (r >> 3) + 8 half + (r & 7) of this lane's row: bias, mask, maximum
+struct ApScore {
+  float c; int R; const float* lb;          // lb[key - position]
+  float far_past, far_next;
+  int pos, kmax, half;                      // this row's position and end
+  int wfirst, wlast, wmin, wmax;            // the wave's first and last position, smallest and largest end
+  template <bool BIAS, int N> __device__ __forceinline__ float finish(v16f (&s)[N], int kb) const {
+    if constexpr (BIAS) {
+      const bool next = kb - wlast >= R, past = kb + 32 * N - 1 - wfirst <= -R;
+      if (next || past) {                                     // all of it lies beyond the range: one value a row
+        const float far = next ? far_next : far_past;
+#pragma unroll
+        for (int b = 0; b < N; ++b)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[b][r] = fmaf(s[b][r], c, far);
+      } else {                                                // |key - position| < R + 96 everywhere
+        const float* d = lb + (kb + 8 * half - pos);
+#pragma unroll
+        for (int b = 0; b < N; ++b)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[b][r] = fmaf(s[b][r], c, d[32 * b + 16 * (r >> 3) + (r & 7)]);
+      }
+    }
+    if (kb + 32 * N > wmin) {
+      asm volatile("");                     // a branch: as selects the mask would cost every block three instructions a score
+      const int lim = kmax - kb - 8 * half;
+#pragma unroll
+      for (int b = 0; b < N; ++b)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[b][r] = 32 * b + 16 * (r >> 3) + (r & 7) < lim ? s[b][r] : -INFINITY;
+    }
+    float mx = s[0][0];
+#pragma unroll
+    for (int b = 0; b < N; ++b)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[b][r]);
+    mx = ap_other_half(mx, true);
+    return BIAS ? mx : mx * c;
+  }
+};
+
+// x0: the wave's first row within the item; this lane's row is x0 + (lane & 31), past the end the last one
+template <bool BIAS>
+__device__ __forceinline__ ApScore ap_score(const ApParams& p, const ApItem& it, int x0, int lane, const float* lbias, int bn) {
+  ApScore sc;
+  int q, h;
+  ap_split(p, it, min(x0, it.rows - 1), q, h);
+  sc.wfirst = it.pos + q;
+  ap_split(p, it, min(x0 + 31, it.rows - 1), q, h);
+  sc.wlast = it.pos + q;
+  ap_split(p, it, min(x0 + (lane & 31), it.rows - 1), q, h);
+  sc.c = p.c; sc.R = p.R; sc.half = lane >> 5;
+  sc.pos = it.pos + q;
+  sc.kmax = p.causal ? min(it.key1, sc.pos + 1) : it.key1;             // keys [key0, kmax) of this row
+  sc.wmin = p.causal ? min(it.key1, sc.wfirst + 1) : it.key1;
+  sc.wmax = p.causal ? min(it.key1, sc.wlast + 1) : it.key1;
+  sc.lb = lbias + (BIAS ? h * bn + p.R + AP_PAD : 0);
+  sc.far_past = BIAS ? sc.lb[-p.R] : 0.f;
+  sc.far_next = BIAS ? sc.lb[p.R] : 0.f;
+  return sc;
+}
+
+// One key tile of 32 NB keys from kt for a wave's 32 rows: scores, running maximum and sum, P V
+template <int DT, int D, int NB, bool BIAS>
+__device__ __forceinline__ void ap_tile(const ApParams& p, const ApScore& score, const char* sk, const char* sv, uint32_t krow, uint32_t kxor,
+                                        uint32_t vrow, uint32_t vxor, int kt, const v4i (&qf)[D / 16], v16f (&acc)[D / 32], float& m, float& mref,
+                                        float& l) {
+  constexpr int ROWB = 2 * D, KK = D / 16, DB = D / 32;
+  v16f s[NB];
+#pragma unroll
+  for (int b = 0; b < NB; ++b)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[b][r] = 0.f;
+#pragma unroll
+  for (int kk = 0; kk < KK; ++kk)     // the blocks in turn: two MFMAs in a row do not depend on each other
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      const v4i kf = *reinterpret_cast<const v4i*>(sk + b * 32 * ROWB + krow + (kxor ^ (kk << 5)));
+      s[b] = ap_mma<DT>::run(kf, qf[kk], s[b]);
+    }
+  const float mx = score.template finish<BIAS>(s, kt);
+  if (__any(mx > m + AP_TAU)) {       // a row that does not exceed its reference keeps it: its bits do not depend on its neighbours
+    const float mn = mx > m + AP_TAU ? mx : m;
+    mref = mn == -INFINITY ? 0.f : mn;
+    const float alpha = __builtin_amdgcn_exp2f(m - mref);
+    m = mn;
+    l *= alpha;
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[d][r] *= alpha;
+  }
+  uint32_t pk[NB][8];
+#pragma unroll
+  for (int b = 0; b < NB; ++b)
+#pragma unroll
+    for (int r = 0; r < 16; r += 2) {
+      const float e0 = __builtin_amdgcn_exp2f(BIAS ? s[b][r] - mref : fmaf(s[b][r], p.c, -mref));
+      const float e1 = __builtin_amdgcn_exp2f(BIAS ? s[b][r + 1] - mref : fmaf(s[b][r + 1], p.c, -mref));
+      l += e0 + e1;
+      pk[b][r >> 1] = pack2<DT>(e0, e1);
+    }
+#pragma unroll
+  for (int t = 0; t < 2 * NB; ++t) {
+    const uint32_t* w = &pk[t >> 1][4 * (t & 1)];
+    const v4i pf = {(int)w[0], (int)w[1], (int)w[2], (int)w[3]};
+#pragma unroll
+    for (int d = 0; d < DB; ++d) {
+      const char* a = sv + t * 16 * ROWB + vrow + ((d << 6) ^ vxor);
+      const v8s vf = __builtin_shufflevector(__builtin_amdgcn_ds_read_tr16_b64_v4i16((ap_trptr_t)a),
+                                             __builtin_amdgcn_ds_read_tr16_b64_v4i16((ap_trptr_t)(a + 4 * ROWB)), 0, 1, 2, 3, 4, 5, 6, 7);
+      acc[d] = ap_mma<DT>::run(__builtin_bit_cast(v4i, vf), pf, acc[d]);
+    }
+  }
+}
+
+// ---- 128 rows, 32 per wave; key tiles of 64 shared by the waves, two LDS stages, one barrier a tile ----
+// What bounds it: for long ranges the matrix pipe (32 MFMAs of 32 cycles a wave and tile for D = 128) and the vector unit (32
+// exponentials of 16 cycles, some 125 other instructions) together, at the clock that the power limit leaves; for short ranges the
+// vector instructions around the loop, hence pointers that step instead of addresses computed row by row.
+template <int DT, int D, bool BIAS>
+__global__ __launch_bounds__(256, 2) void attn_packed_tile_kernel(const ApParams p) {
+  constexpr int ROWB = 2 * D, TILE = 64 * ROWB, STAGE = 2 * TILE, PIECES = TILE / 4096, RPP = 1024 / ROWB, KK = D / 16, DB = D / 32;
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int kvh = blockIdx.x % p.Hkv;
-  const ApItem it = p.items[blockIdx.x / p.Hkv];
-  float* const lbias = reinterpret_cast<float*>(smem + (FEW ? 8 : 2) * STAGE);
-
-  // ---- this lane's row ----
-  const int nrows = it.q_len * p.G;
-  const int wrow0 = it.row0 + (FEW ? 0 : 32 * wave);
-  const int q_first = it.row0 / p.G, g_first = it.row0 - q_first * p.G;
-  // query and head of row it.row0 + x: x is less than a tile, so the division is one multiplication
-  auto split_row = [&](int x, int& q, int& h) {
-    const int y = g_first + min(x, nrows - 1 - it.row0);
-    const int d = p.G > 1 ? (int)__umulhi((uint32_t)y, p.gmagic) : y;
-    q = q_first + d;
-    h = y - d * p.G;
-  };
-  const int row = wrow0 + (lane & 31);
-  const bool valid = row < nrows;
-  int qi, g;
-  split_row(row - it.row0, qi, g);
-  const int shift = it.k_len - it.q_len;
-  const int pos = qi + shift;
-  const int kmax = p.causal ? min(it.key1, pos + 1) : it.key1;         // keys [key0, kmax) of this row
-  // the tile's last row sees most keys, the wave's first row fewest
-  const int last = min(it.row0 + (FEW ? AP_FEW : AP_ROWS), nrows) - 1;
-  const int key_end = p.causal ? min(it.key1, last / p.G + shift + 1) : it.key1;
-  const int wfirst = min(wrow0, nrows - 1) / p.G + shift, wlast = min(wrow0 + 31, nrows - 1) / p.G + shift;   // positions
-  const int wmin = p.causal ? min(it.key1, wfirst + 1) : it.key1;
-  const int wmax = wrow0 >= nrows ? 0 : (p.causal ? min(it.key1, wlast + 1) : it.key1);
-
-  const uint16_t* const qhead = p.q + (int64_t)it.q_begin * p.q_ts + (int64_t)kvh * p.G * p.q_hs;
-  char* const qstage = smem + STAGE + wave * 32 * ROWB;                // tile kernel: the wave's 32 rows, in stage 1 until tile 1 comes
-  v4i qf[KK];                                                          // Q^T fragments: B operand, lane = row, 8 consecutive d each
-  if constexpr (FEW) {
-    const uint16_t* qp = qhead + qi * p.q_ts + g * p.q_hs + 8 * half;
-#pragma unroll
-    for (int kk = 0; kk < KK; ++kk) qf[kk] = *reinterpret_cast<const v4i*>(qp + 16 * kk);
-  } else {                                                             // whole rows at a time: memory likes full lines
-    constexpr int RP = 1024 / ROWB;
-#pragma unroll
-    for (int t = 0; t < 32 / RP; ++t) {
-      const int x = RP * t + lane / (ROWB / 16);
-      int q2, g2;
-      split_row(wrow0 - it.row0 + x, q2, g2);
-      ap_dma_ptr(qhead + q2 * p.q_ts + g2 * p.q_hs + 8 * ((lane & (ROWB / 16 - 1)) ^ ap_kx<D>(x)), qstage + t * 1024);
-    }
-  }
-  const int bn = 2 * p.R + 1 + 2 * AP_PAD;
-  if constexpr (BIAS) {   // exp2 domain; the type's lowest values as a finite low (a row of nothing else stays a uniform row)
-    const float* b = p.bias + (int64_t)kvh * p.G * (2 * p.R + 1);
-    for (int i = tid; i < p.G * bn; i += 256) {
-      const int h = i / bn, d = max(0, min(2 * p.R, i - h * bn - AP_PAD));
-      const float x = b[h * (2 * p.R + 1) + d];
-      lbias[i] = fabsf(x) > 1e37f && fabsf(x) < INFINITY ? copysignf(1e37f, x) : x * 1.4426950408889634f;
-    }
-    __syncthreads();
-  }
-  const float* const lb = lbias + (BIAS ? g * bn + p.R + AP_PAD : 0);   // lb[key - position]
-  const float b_far_past = BIAS ? lb[-p.R] : 0.f, b_far_next = BIAS ? lb[p.R] : 0.f;
-
-  // ---- LDS-DMA: piece t of this wave; rows past the range re-read the last one (finite, masked) ----
+  const int item = blockIdx.z * AP_GRID_Y + blockIdx.y, kvh = blockIdx.x;
+  if (item >= p.n_items) return;
+  const ApItem it = p.items[item];
+  const int lane = threadIdx.x & 63, half = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int x0 = 32 * wave, bn = 2 * p.R + 1 + 2 * AP_PAD;
+  float* const lbias = reinterpret_cast<float*>(smem + 2 * STAGE);
   const int drow = lane / (ROWB / 16), dchunk = lane & (ROWB / 16 - 1);
-  uint32_t koff[PIECES], voff[PIECES];
-  auto piece_row = [&](int t) { return RPP * (FEW ? t : wave + 4 * t) + drow; };
+
+  // ---- Q: whole rows (memory likes full lines) into the wave's part of stage 1, until tile 1 comes ----
+  char* const qstage = smem + STAGE + x0 * ROWB;
+  {
+    const uint16_t* const qhead = p.q + (int64_t)it.token * p.q_ts + (int64_t)kvh * p.G * p.q_hs;
+    ApRowWalk<D> w(p, it, x0 + drow, p.q_ts, p.q_hs);
 #pragma unroll
-  for (int t = 0; t < PIECES; ++t) {
-    const uint32_t r = piece_row(t);
-    koff[t] = r * (uint32_t)(2 * p.k_ts) + ((dchunk ^ ap_kx<D>(r)) << 4);
-    voff[t] = r * (uint32_t)(2 * p.v_ts) + ((dchunk ^ ap_vx<D>(r)) << 4);
+    for (int t = 0; t < 32 / RPP; ++t, w.next()) {
+      const int x = RPP * t + drow;
+      if (x0 + x < it.rows)                                            // rows past the end: whatever LDS holds, never stored
+        ap_dma_ptr(qhead + w.at + 8 * (dchunk ^ ap_kx<D>(x)), qstage + t * 1024);
+    }
   }
+  // ---- K, V: piece i of this wave is rows RPP (wave + 4 i) ..; rows past the range re-read the last one (finite, masked) ----
+  const uint32_t r0 = RPP * wave + drow;
+  const uint32_t koff = r0 * (uint32_t)(2 * p.k_ts) + ((dchunk ^ ap_kx<D>(r0)) << 4);      // the same permutation in every piece
+  const uint32_t voff = r0 * (uint32_t)(2 * p.v_ts) + ((dchunk ^ ap_vx<D>(r0)) << 4);
   const uint16_t* const kbase = p.k + (int64_t)it.k_begin * p.k_ts + (int64_t)kvh * p.k_hs;
   const uint16_t* const vbase = p.v + (int64_t)it.k_begin * p.v_ts + (int64_t)kvh * p.v_hs;
-  char* const mystage = smem + (FEW ? wave * 2 * STAGE : 0);
   auto fetch = [&](int kt, int buf) {
-    const int nv = min(it.key1 - kt, BK);
+    const int nv = min(it.key1 - kt, 64);
     const uint16_t* kp = kbase + (int64_t)kt * p.k_ts;
     const uint16_t* vp = vbase + (int64_t)kt * p.v_ts;
     const uint32_t kbytes = (uint32_t)((nv - 1) * 2 * p.k_ts + ROWB), vbytes = (uint32_t)((nv - 1) * 2 * p.v_ts + ROWB);
-    char* st = mystage + buf * STAGE + (FEW ? 0 : wave * 1024);
-    constexpr int STEP = FEW ? 1024 : 4096;
-    if (nv == BK) {
+    char* st = smem + buf * STAGE + wave * 1024;
+    if (nv == 64) {
 #pragma unroll
-      for (int t = 0; t < PIECES; ++t)
-        ap_dma(kp, kbytes, st + t * STEP, koff[t]);
-#pragma unroll
-      for (int t = 0; t < PIECES; ++t)
-        ap_dma(vp, vbytes, st + TILE + t * STEP, voff[t]);
+      for (int i = 0; i < PIECES; ++i) {
+        ap_dma(kp, kbytes, st + i * 4096, koff + i * (uint32_t)(8 * RPP * p.k_ts));
+        ap_dma(vp, vbytes, st + TILE + i * 4096, voff + i * (uint32_t)(8 * RPP * p.v_ts));
+      }
     } else {
 #pragma unroll
-      for (int t = 0; t < PIECES; ++t) {
-        const uint32_t r = piece_row(t), rcl = min((int)r, nv - 1);
-        const uint32_t ko = rcl * (uint32_t)(2 * p.k_ts) + ((dchunk ^ ap_kx<D>(r)) << 4);
-        const uint32_t vo = rcl * (uint32_t)(2 * p.v_ts) + ((dchunk ^ ap_vx<D>(r)) << 4);
-        ap_dma(kp, kbytes, st + t * STEP, ko);
-        ap_dma(vp, vbytes, st + TILE + t * STEP, vo);
+      for (int i = 0; i < PIECES; ++i) {
+        const uint32_t r = min((int)r0 + 4 * RPP * i, nv - 1);
+        ap_dma(kp, kbytes, st + i * 4096, r * (uint32_t)(2 * p.k_ts) + ((dchunk ^ ap_kx<D>(r0)) << 4));
+        ap_dma(vp, vbytes, st + TILE + i * 4096, r * (uint32_t)(2 * p.v_ts) + ((dchunk ^ ap_vx<D>(r0)) << 4));
       }
     }
   };
+  // the item's last row sees most keys
+  int q_last, h_last;
+  ap_split(p, it, it.rows - 1, q_last, h_last);
+  const int kend = p.causal ? min(it.key1, it.pos + q_last + 1) : it.key1;
+  int kt = it.key0;
+  if (kt < kend) fetch(kt, 0);
+  if constexpr (BIAS) ap_load_bias(p, kvh, bn, lbias);
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  v4i qf[KK];                                                          // Q^T fragments: B operand, lane = row, 8 consecutive d each
+  {
+    const uint32_t r = lane & 31;
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk) qf[kk] = *reinterpret_cast<const v4i*>(qstage + r * ROWB + (((half ^ ap_kx<D>(r)) << 4) ^ (kk << 5)));
+  }
+  __syncthreads();
+  const ApScore score = ap_score<BIAS>(p, it, x0, lane, lbias, bn);
+  const int wend = x0 < it.rows ? score.wmax : 0;
 
   // ---- fragment addresses ----
   const uint32_t kr = (lane & 19) | ((lane & 4) << 1) | ((lane & 8) >> 1);      // bits 2 and 3 of the row swapped
@@ -208,194 +327,173 @@ __global__ __launch_bounds__(256, FEW ? 1 : 2) void attn_packed_kernel(const ApP
 #pragma unroll
     for (int r = 0; r < 16; ++r) acc[d][r] = 0.f;
   float m = -INFINITY, mref = 0.f, l = 0.f;
-
-  const int step = FEW ? 4 * BK : BK;
-  int kt = it.key0 + (FEW ? wave * BK : 0);
-  const int kend = key_end;
-  if (kt < kend) fetch(kt, 0);
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-  if constexpr (!FEW) {
-    const uint32_t r = lane & 31;
-#pragma unroll
-    for (int kk = 0; kk < KK; ++kk) qf[kk] = *reinterpret_cast<const v4i*>(qstage + r * ROWB + (((half ^ ap_kx<D>(r)) << 4) ^ (kk << 5)));
-    __syncthreads();
-  }
-  for (int buf = 0; kt < kend; kt += step, buf ^= 1) {
-    if (kt + step < kend) fetch(kt + step, buf ^ 1);
-    if (FEW || kt < wmax) {
-      const char* sk = mystage + buf * STAGE;
-      const char* sv = sk + TILE;
-      v16f s[NB];
-#pragma unroll
-      for (int b = 0; b < NB; ++b)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) s[b][r] = 0.f;
-#pragma unroll
-      for (int kk = 0; kk < KK; ++kk)     // the blocks in turn: two MFMAs in a row do not depend on each other
-#pragma unroll
-        for (int b = 0; b < NB; ++b) {
-          const v4i kf = *reinterpret_cast<const v4i*>(sk + b * 32 * ROWB + krow + (kxor ^ (kk << 5)));
-          s[b] = ap_mma<DT>::run(kf, qf[kk], s[b]);
-        }
-      // register r of block b is key kt + 32 b + 16 (r >> 3) + 8 half + (r & 7)
-      if constexpr (BIAS) {
-        const bool next = kt - wlast >= p.R, past = kt + BK - 1 - wfirst <= -p.R;
-        if (next || past) {                                     // the whole tile lies beyond the range: one value a row
-          const float far = next ? b_far_next : b_far_past;
-#pragma unroll
-          for (int b = 0; b < NB; ++b)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) s[b][r] = fmaf(s[b][r], p.c, far);
-        } else {                                                // |key - position| < R + 96 everywhere in the tile
-          const float* d = lb + (kt + 8 * half - pos);
-#pragma unroll
-          for (int b = 0; b < NB; ++b)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) s[b][r] = fmaf(s[b][r], p.c, d[32 * b + 16 * (r >> 3) + (r & 7)]);
-        }
-      }
-      if (kt + BK > wmin) {
-        asm volatile("");                 // a branch: as selects the mask would cost every tile 96 instructions
-        const int lim = kmax - kt - 8 * half;
-#pragma unroll
-        for (int b = 0; b < NB; ++b)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) s[b][r] = 32 * b + 16 * (r >> 3) + (r & 7) < lim ? s[b][r] : -INFINITY;
-      }
-      float mx = s[0][0];
-#pragma unroll
-      for (int b = 0; b < NB; ++b)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[b][r]);
-      mx = ap_other_half(mx, true);
-      if constexpr (!BIAS) mx *= p.c;
-      if (__any(mx > m + AP_TAU)) {
-        const float mn = fmaxf(m, mx);
-        mref = mn == -INFINITY ? 0.f : mn;
-        const float alpha = __builtin_amdgcn_exp2f(m - mref);
-        m = mn;
-        l *= alpha;
-#pragma unroll
-        for (int d = 0; d < DB; ++d)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) acc[d][r] *= alpha;
-      }
-      uint32_t pk[NB][8];
-#pragma unroll
-      for (int b = 0; b < NB; ++b)
-#pragma unroll
-        for (int r = 0; r < 16; r += 2) {
-          const float e0 = __builtin_amdgcn_exp2f(BIAS ? s[b][r] - mref : fmaf(s[b][r], p.c, -mref));
-          const float e1 = __builtin_amdgcn_exp2f(BIAS ? s[b][r + 1] - mref : fmaf(s[b][r + 1], p.c, -mref));
-          l += e0 + e1;
-          pk[b][r >> 1] = pack2<DT>(e0, e1);
-        }
-#pragma unroll
-      for (int t = 0; t < 2 * NB; ++t) {
-        const uint32_t* w = &pk[t >> 1][4 * (t & 1)];
-        const v4i pf = {(int)w[0], (int)w[1], (int)w[2], (int)w[3]};
-#pragma unroll
-        for (int d = 0; d < DB; ++d) {
-          const char* a = sv + t * 16 * ROWB + vrow + ((d << 6) ^ vxor);
-          const ap_v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ap_trptr_t)a);
-          const ap_v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ap_trptr_t)(a + 4 * ROWB));
-          const v8s vf = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-          acc[d] = ap_mma<DT>::run(__builtin_bit_cast(v4i, vf), pf, acc[d]);
-        }
-      }
-    }
-    // this tile's reads have returned and the next tile has landed (FEW: the stages are this wave's own)
+  for (int buf = 0; kt < kend; kt += 64, buf ^= 1) {
+    if (kt + 64 < kend) fetch(kt + 64, buf ^ 1);
+    if (kt < wend) ap_tile<DT, D, 2, BIAS>(p, score, smem + buf * STAGE, smem + buf * STAGE + TILE, krow, kxor, vrow, vxor, kt, qf, acc, m, mref, l);
+    // this tile's reads have returned and the next tile has landed
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-    if constexpr (!FEW) __syncthreads();
+    __syncthreads();
   }
   l = ap_other_half(l, false);
 
   // ---- results.  acc[d][r] is d = 32 d + 8 (r >> 2) + 4 half + (r & 3) of this lane's row ----
-  if constexpr (FEW) {   // join the four waves through LDS
-    constexpr int LD = D + 4;
-    float* jo = reinterpret_cast<float*>(smem);                 // [4][32][LD]
-    float* jm = jo + 4 * 32 * LD;                               // [4][32][2]
-    __syncthreads();
-    float* mo = jo + (wave * 32 + (lane & 31)) * LD;
+  const int x = x0 + (lane & 31);
+  if (it.slot >= 0) {
+    if (x >= it.rows) return;
+    const int64_t pr = (int64_t)kvh * p.ws_rows + it.slot + x;
 #pragma unroll
     for (int d = 0; d < DB; ++d)
 #pragma unroll
       for (int r = 0; r < 16; r += 4)
-        *reinterpret_cast<float4*>(mo + 32 * d + 2 * r + 4 * half) = make_float4(acc[d][r], acc[d][r + 1], acc[d][r + 2], acc[d][r + 3]);
-    if (half == 0) { jm[(wave * 32 + lane) * 2] = m; jm[(wave * 32 + lane) * 2 + 1] = l; }
+        *reinterpret_cast<float4*>(p.po + pr * D + 32 * d + 2 * r + 4 * half) = make_float4(acc[d][r], acc[d][r + 1], acc[d][r + 2], acc[d][r + 3]);
+    if (half == 0) { p.pml[pr * 2] = m; p.pml[pr * 2 + 1] = l; }
+    return;
+  }
+  // through the wave's own 32 rows of LDS (every wave is done with the stages): whole rows go out
+  const float inv = l == 0.f ? 0.f : 1.0f / l;
+  char* const ost = smem + x0 * ROWB;
+  const uint32_t r32 = lane & 31;
+#pragma unroll
+  for (int d = 0; d < DB; ++d)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int r = 8 * j;
+      const uint32_t a0 = pack2<DT>(acc[d][r] * inv, acc[d][r + 1] * inv), a1 = pack2<DT>(acc[d][r + 2] * inv, acc[d][r + 3] * inv);
+      const uint32_t b0 = pack2<DT>(acc[d][r + 4] * inv, acc[d][r + 5] * inv), b1 = pack2<DT>(acc[d][r + 6] * inv, acc[d][r + 7] * inv);
+      const auto s0 = __builtin_amdgcn_permlane32_swap(a0, b0, false, false);
+      const auto s1 = __builtin_amdgcn_permlane32_swap(a1, b1, false, false);
+      *reinterpret_cast<uint4*>(ost + r32 * ROWB + (((4 * d + 2 * j + half) ^ ap_kx<D>(r32)) << 4)) = make_uint4(s0[0], s1[0], s0[1], s1[1]);
+    }
+  __builtin_amdgcn_wave_barrier();
+  uint16_t* const ohead = p.o + (int64_t)it.token * p.o_ts + (int64_t)kvh * p.G * p.o_hs + 8 * dchunk;
+  ApRowWalk<D> w(p, it, x0 + drow, p.o_ts, p.o_hs);
+#pragma unroll
+  for (int t = 0; t < 32 / RPP; ++t, w.next()) {
+    const uint32_t y = RPP * t + drow;
+    const uint4 v = *reinterpret_cast<const uint4*>(ost + y * ROWB + ((dchunk ^ ap_kx<D>(y)) << 4));
+    if (x0 + (int)y < it.rows) *reinterpret_cast<uint4*>(ohead + w.at) = v;
+  }
+}
+
+// ---- up to 32 rows; the waves take different keys, each with two LDS stages of its own, and join at the end ----
+// What bounds it: memory, K and V once.  256 workgroups of 64 KB in flight.
+template <int DT, int D, bool BIAS>
+__global__ __launch_bounds__(256, 1) void attn_packed_few_kernel(const ApParams p) {
+  constexpr int NB = D == 128 ? 1 : 2, BK = 32 * NB;        // keys per tile
+  constexpr int ROWB = 2 * D, TILE = BK * ROWB, STAGE = 2 * TILE, PIECES = TILE / 1024, RPP = 1024 / ROWB, KK = D / 16, DB = D / 32;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const int item = blockIdx.z * AP_GRID_Y + blockIdx.y, kvh = blockIdx.x;
+  if (item >= p.n_items) return;
+  const ApItem it = p.items[item];
+  const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int bn = 2 * p.R + 1 + 2 * AP_PAD;
+  float* const lbias = reinterpret_cast<float*>(smem + 8 * STAGE);
+  v4i qf[KK];
+  {
+    int q, h;
+    ap_split(p, it, min(lane & 31, it.rows - 1), q, h);
+    const uint16_t* qp = p.q + (int64_t)(it.token + q) * p.q_ts + (int64_t)(kvh * p.G + h) * p.q_hs + 8 * half;
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk) qf[kk] = *reinterpret_cast<const v4i*>(qp + 16 * kk);
+  }
+  if constexpr (BIAS) {
+    ap_load_bias(p, kvh, bn, lbias);
     __syncthreads();
-    constexpr int W = D / 8;                                    // d per thread
-    const int jr = tid >> 3, d0 = (tid & 7) * W;
-    const int r2 = it.row0 + jr;
-    if (r2 < nrows) {
-      float mm = -INFINITY, ll = 0.f, oo[W];
+  }
+  const ApScore score = ap_score<BIAS>(p, it, 0, lane, lbias, bn);
+  const int kend = score.wmax;
+
+  const int drow = lane / (ROWB / 16), dchunk = lane & (ROWB / 16 - 1);
+  const uint16_t* const kbase = p.k + (int64_t)it.k_begin * p.k_ts + (int64_t)kvh * p.k_hs;
+  const uint16_t* const vbase = p.v + (int64_t)it.k_begin * p.v_ts + (int64_t)kvh * p.v_hs;
+  char* const mystage = smem + wave * 2 * STAGE;
+  auto fetch = [&](int kt, int buf) {                       // rows past the range re-read the last one (finite, masked)
+    const int nv = min(it.key1 - kt, BK);
+    const uint16_t* kp = kbase + (int64_t)kt * p.k_ts;
+    const uint16_t* vp = vbase + (int64_t)kt * p.v_ts;
+    const uint32_t kbytes = (uint32_t)((nv - 1) * 2 * p.k_ts + ROWB), vbytes = (uint32_t)((nv - 1) * 2 * p.v_ts + ROWB);
+    char* st = mystage + buf * STAGE;
 #pragma unroll
-      for (int w = 0; w < 4; ++w) mm = fmaxf(mm, jm[(w * 32 + jr) * 2]);
-      const float mr = mm == -INFINITY ? 0.f : mm;
+    for (int t = 0; t < PIECES; ++t) {
+      const uint32_t r = RPP * t + drow, rc = min((int)r, nv - 1);
+      ap_dma(kp, kbytes, st + t * 1024, rc * (uint32_t)(2 * p.k_ts) + ((dchunk ^ ap_kx<D>(r)) << 4));
+      ap_dma(vp, vbytes, st + TILE + t * 1024, rc * (uint32_t)(2 * p.v_ts) + ((dchunk ^ ap_vx<D>(r)) << 4));
+    }
+  };
+  const uint32_t kr = (lane & 19) | ((lane & 4) << 1) | ((lane & 8) >> 1);      // bits 2 and 3 of the row swapped
+  const uint32_t krow = kr * ROWB, kxor = (half ^ ap_kx<D>(kr)) << 4;
+  const uint32_t i16 = lane & 15;
+  const uint32_t vkey = 8 * half + (i16 >> 2);
+  const uint32_t vrow = vkey * ROWB + ((((lane >> 4) & 1) * 2 + ((i16 & 3) >> 1)) << 4) + (i16 & 1) * 8;
+  const uint32_t vxor = ap_vx<D>(vkey) << 4;
+
+  v16f acc[DB];
 #pragma unroll
-      for (int e = 0; e < W; ++e) oo[e] = 0.f;
+  for (int d = 0; d < DB; ++d)
 #pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        const float a = __builtin_amdgcn_exp2f(jm[(w * 32 + jr) * 2] - mr);
-        ll += a * jm[(w * 32 + jr) * 2 + 1];
+    for (int r = 0; r < 16; ++r) acc[d][r] = 0.f;
+  float m = -INFINITY, mref = 0.f, l = 0.f;
+  int kt = it.key0 + wave * BK;
+  if (kt < kend) fetch(kt, 0);
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  for (int buf = 0; kt < kend; kt += 4 * BK, buf ^= 1) {
+    if (kt + 4 * BK < kend) fetch(kt + 4 * BK, buf ^ 1);
+    const char* sk = mystage + buf * STAGE;
+    ap_tile<DT, D, NB, BIAS>(p, score, sk, sk + TILE, krow, kxor, vrow, vxor, kt, qf, acc, m, mref, l);
+    // this tile's reads have returned and the next tile has landed (the stages are this wave's own)
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+  }
+  l = ap_other_half(l, false);
+
+  // acc[d][r] is d = 32 d + 8 (r >> 2) + 4 half + (r & 3) of this lane's row
+  // ---- join the four waves through LDS ----
+  constexpr int LD = D + 4;
+  float* jo = reinterpret_cast<float*>(smem);                 // [4][32][LD]
+  float* jm = jo + 4 * 32 * LD;                               // [4][32][2]
+  __syncthreads();
+  float* mo = jo + (wave * 32 + (lane & 31)) * LD;
 #pragma unroll
-        for (int e = 0; e < W; e += 4) {
-          const float4 x = *reinterpret_cast<const float4*>(jo + (w * 32 + jr) * LD + d0 + e);
-          oo[e] += a * x.x; oo[e + 1] += a * x.y; oo[e + 2] += a * x.z; oo[e + 3] += a * x.w;
-        }
-      }
-      if (it.slot >= 0) {
-        const int64_t pr = (int64_t)kvh * p.ws_rows + it.slot + jr;
+  for (int d = 0; d < DB; ++d)
 #pragma unroll
-        for (int e = 0; e < W; e += 4)
-          *reinterpret_cast<float4*>(p.po + pr * D + d0 + e) = make_float4(oo[e], oo[e + 1], oo[e + 2], oo[e + 3]);
-        if (d0 == 0) { p.pml[pr * 2] = mm; p.pml[pr * 2 + 1] = ll; }
-      } else {
-        const float inv = ll == 0.f ? 0.f : 1.0f / ll;
-        const int q2 = r2 / p.G, g2 = r2 - q2 * p.G;
-        uint16_t* op = p.o + (int64_t)(it.q_begin + q2) * p.o_ts + (int64_t)(kvh * p.G + g2) * p.o_hs + d0;
+    for (int r = 0; r < 16; r += 4)
+      *reinterpret_cast<float4*>(mo + 32 * d + 2 * r + 4 * half) = make_float4(acc[d][r], acc[d][r + 1], acc[d][r + 2], acc[d][r + 3]);
+  if (half == 0) { jm[(wave * 32 + lane) * 2] = m; jm[(wave * 32 + lane) * 2 + 1] = l; }
+  __syncthreads();
+  constexpr int W = D / 8;                                    // d per thread
+  const int jr = tid >> 3, d0 = (tid & 7) * W;
+  if (jr < it.rows) {
+    float mm = -INFINITY, ll = 0.f, oo[W];
 #pragma unroll
-        for (int e = 0; e < W; ++e) oo[e] *= inv;
+    for (int w = 0; w < 4; ++w) mm = fmaxf(mm, jm[(w * 32 + jr) * 2]);
+    const float mr = mm == -INFINITY ? 0.f : mm;
 #pragma unroll
-        for (int e = 0; e < W; e += 8) *reinterpret_cast<uint4*>(op + e) = pack8<DT>(oo + e);
+    for (int e = 0; e < W; ++e) oo[e] = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float a = __builtin_amdgcn_exp2f(jm[(w * 32 + jr) * 2] - mr);
+      ll += a * jm[(w * 32 + jr) * 2 + 1];
+#pragma unroll
+      for (int e = 0; e < W; e += 4) {
+        const float4 x = *reinterpret_cast<const float4*>(jo + (w * 32 + jr) * LD + d0 + e);
+        oo[e] += a * x.x; oo[e + 1] += a * x.y; oo[e + 2] += a * x.z; oo[e + 3] += a * x.w;
       }
     }
-  } else {
     if (it.slot >= 0) {
-      if (!valid) return;
-      const int64_t pr = (int64_t)kvh * p.ws_rows + it.slot + 32 * wave + (lane & 31);
+      const int64_t pr = (int64_t)kvh * p.ws_rows + it.slot + jr;
 #pragma unroll
-      for (int d = 0; d < DB; ++d)
+      for (int e = 0; e < W; e += 4)
+        *reinterpret_cast<float4*>(p.po + pr * D + d0 + e) = make_float4(oo[e], oo[e + 1], oo[e + 2], oo[e + 3]);
+      if (d0 == 0) { p.pml[pr * 2] = mm; p.pml[pr * 2 + 1] = ll; }
+    } else {
+      const float inv = ll == 0.f ? 0.f : 1.0f / ll;
+      int q2, g2;
+      ap_split(p, it, jr, q2, g2);
+      uint16_t* op = p.o + (int64_t)(it.token + q2) * p.o_ts + (int64_t)(kvh * p.G + g2) * p.o_hs + d0;
 #pragma unroll
-        for (int r = 0; r < 16; r += 4)
-          *reinterpret_cast<float4*>(p.po + pr * D + 32 * d + 2 * r + 4 * half) = make_float4(acc[d][r], acc[d][r + 1], acc[d][r + 2], acc[d][r + 3]);
-      if (half == 0) { p.pml[pr * 2] = m; p.pml[pr * 2 + 1] = l; }
-    } else {   // through the wave's own 32 rows of LDS (every wave is done with the stages): whole rows go out
-      const float inv = l == 0.f ? 0.f : 1.0f / l;
-      char* const ost = smem + wave * 32 * ROWB;
-      const uint32_t r32 = lane & 31;
+      for (int e = 0; e < W; ++e) oo[e] *= inv;
 #pragma unroll
-      for (int d = 0; d < DB; ++d)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const int r = 8 * j;
-          const uint32_t a0 = pack2<DT>(acc[d][r] * inv, acc[d][r + 1] * inv), a1 = pack2<DT>(acc[d][r + 2] * inv, acc[d][r + 3] * inv);
-          const uint32_t b0 = pack2<DT>(acc[d][r + 4] * inv, acc[d][r + 5] * inv), b1 = pack2<DT>(acc[d][r + 6] * inv, acc[d][r + 7] * inv);
-          const auto s0 = __builtin_amdgcn_permlane32_swap(a0, b0, false, false);
-          const auto s1 = __builtin_amdgcn_permlane32_swap(a1, b1, false, false);
-          *reinterpret_cast<uint4*>(ost + r32 * ROWB + (((4 * d + 2 * j + half) ^ ap_kx<D>(r32)) << 4)) = make_uint4(s0[0], s1[0], s0[1], s1[1]);
-        }
-      __builtin_amdgcn_wave_barrier();
-      uint16_t* const ohead = p.o + (int64_t)it.q_begin * p.o_ts + (int64_t)kvh * p.G * p.o_hs;
-      constexpr int RP = 1024 / ROWB;
-#pragma unroll
-      for (int t = 0; t < 32 / RP; ++t) {
-        const uint32_t x = RP * t + lane / (ROWB / 16), c = lane & (ROWB / 16 - 1);
-        int q2, g2;
-        split_row(wrow0 - it.row0 + x, q2, g2);
-        const uint4 v = *reinterpret_cast<const uint4*>(ost + x * ROWB + ((c ^ ap_kx<D>(x)) << 4));
-        if (wrow0 + (int)x < nrows) *reinterpret_cast<uint4*>(ohead + q2 * p.o_ts + g2 * p.o_hs + 8 * c) = v;
-      }
+      for (int e = 0; e < W; e += 8) *reinterpret_cast<uint4*>(op + e) = pack8<DT>(oo + e);
     }
   }
 }
@@ -422,8 +520,8 @@ __global__ __launch_bounds__(256) void attn_packed_join_kernel(const ApParams p,
     for (int e = 0; e < E; ++e) o[e] += a * p.po[pr * D + lane * E + e];
   }
   const float inv = ll == 0.f ? 0.f : 1.0f / ll;
-  const int row = j.row0 + r, qi = row / p.G, g = row - qi * p.G;
-  uint16_t* op = p.o + (int64_t)(j.q_begin + qi) * p.o_ts + (int64_t)(kvh * p.G + g) * p.o_hs + lane * E;
+  const int y = j.head0 + r, qi = p.G > 1 ? (int)__umulhi((uint32_t)y, p.gmagic) : y, g = y - qi * p.G;
+  uint16_t* op = p.o + (int64_t)(j.token + qi) * p.o_ts + (int64_t)(kvh * p.G + g) * p.o_hs + lane * E;
   if constexpr (E == 2) *reinterpret_cast<uint32_t*>(op) = pack2<DT>(o[0] * inv, o[1] * inv);
   else *op = (uint16_t)pack2<DT>(o[0] * inv, 0.f);
 }
@@ -471,10 +569,11 @@ extern "C" int td_attn_packed_plan(const int64_t* lens_q, const int64_t* lens_k,
           const int64_t quantum = few ? 128 : 64;
           const int64_t per = td_cdiv(td_cdiv(std::max<int64_t>(end, 1), parts), quantum) * quantum;
           const int64_t n = std::max<int64_t>(1, td_cdiv(end, per));
-          if (n > 1) joins.push_back({(int32_t)q0, (int32_t)ql, (int32_t)r0, (int32_t)(last - r0 + 1), (int32_t)ws_rows, (int32_t)n, (int32_t)tr, 0});
+          const int32_t token = (int32_t)(q0 + r0 / G), head0 = (int32_t)(r0 % G), nr = (int32_t)(last - r0 + 1), pos = (int32_t)(r0 / G + kl - ql);
+          if (n > 1) joins.push_back({token, head0, nr, (int32_t)ws_rows, (int32_t)n, (int32_t)tr, 0, 0});
           for (int64_t i = 0; i < n; ++i) {
             const int64_t a = i * per, b = std::min(end, a + per);
-            work[few].push_back({{(int32_t)q0, (int32_t)k0, (int32_t)ql, (int32_t)kl, (int32_t)r0, (int32_t)a, (int32_t)b,
+            work[few].push_back({{token, head0, nr, pos, (int32_t)k0, (int32_t)a, (int32_t)b,
                                   n > 1 ? (int32_t)(ws_rows + i * tr) : -1}, b - a});
           }
           if (n > 1) ws_rows += n * tr;
@@ -483,9 +582,10 @@ extern "C" int td_attn_packed_plan(const int64_t* lens_q, const int64_t* lens_k,
         q0 += ql; k0 += kl;
       }
       if (pass == 0) {
-        // 256 CUs.  A key range is split when the whole work is less than two full rounds of workgroups of the longest
-        // range; a part is at least 512 keys (few: 256), below which writing and joining partials costs more than it saves.
-        chunk[0] = std::max<int64_t>(512, td_cdiv(keys_total[0] * kv_heads, 1024));
+        // 256 CUs, two tile workgroups each (few: one).  A key range is split when it is longer than the share of one of these
+        // slots (few: half of it, to even the load out); a part is at least 512 keys (few: 256), below which writing and joining
+        // partials costs more than it saves.
+        chunk[0] = std::max<int64_t>(512, td_cdiv(keys_total[0] * kv_heads, 512));
         chunk[1] = std::max<int64_t>(256, td_cdiv(keys_total[1] * kv_heads, 512));
       }
     }
@@ -510,10 +610,11 @@ extern "C" int td_attn_packed_plan(const int64_t* lens_q, const int64_t* lens_k,
 template <int DT, int D, bool FEW, bool BIAS>
 static void ap_launch(const ApParams& p, int64_t n, int bias_bytes, hipStream_t st) {
   static std::atomic<uint64_t> mask{0};
-  constexpr int NB = FEW && D == 128 ? 1 : 2;
-  const int tiles = (FEW ? 8 : 2) * 2 * 32 * NB * 2 * D;
-  td_ensure_dyn_lds((const void*)attn_packed_kernel<DT, D, FEW, BIAS>, tiles + 32768, mask);
-  attn_packed_kernel<DT, D, FEW, BIAS><<<(unsigned)(n * p.Hkv), 256, tiles + bias_bytes, st>>>(p);
+  constexpr int tiles = FEW ? 131072 : 4 * 64 * 2 * D;       // two stages of K + V; few: of 8 KB each for every wave
+  const auto kernel = FEW ? attn_packed_few_kernel<DT, D, BIAS> : attn_packed_tile_kernel<DT, D, BIAS>;
+  td_ensure_dyn_lds((const void*)kernel, tiles + 32768, mask);
+  const dim3 grid((unsigned)p.Hkv, (unsigned)std::min<int64_t>(n, AP_GRID_Y), (unsigned)td_cdiv(n, AP_GRID_Y));
+  kernel<<<grid, 256, tiles + bias_bytes, st>>>(p);
 }
 
 extern "C" int td_attn_packed(const void* q, const void* k, const void* v, void* o, const int64_t* strides, int dtype, int heads, int kv_heads,
@@ -532,8 +633,8 @@ extern "C" int td_attn_packed(const void* q, const void* k, const void* v, void*
   const int64_t nt = counts[0], nf = counts[1], nj = counts[2], wr = counts[3];
   TD_REQUIRE(nt >= 0 && nf >= 0 && nj >= 0 && wr >= 0 && (nj == 0 || ws), TD_ERR_INVALID, "td_attn_packed: counts / workspace");
   TD_REQUIRE(counts[5] == 0 || (k && v), TD_ERR_INVALID, "td_attn_packed: null keys or values");
-  TD_REQUIRE(nt * kv_heads < (1ll << 31) && nf * kv_heads < (1ll << 31) && nj < (1ll << 31) && kv_heads <= 65535, TD_ERR_UNSUPPORTED,
-             "td_attn_packed: more than 2^31 workgroups");
+  TD_REQUIRE(nt < (1ll << 31) && nf < (1ll << 31) && nj < (1ll << 31) && kv_heads <= 65535, TD_ERR_UNSUPPORTED,
+             "td_attn_packed: too many workgroups");
   const int G = heads / kv_heads;
   TD_REQUIRE(G <= 16384, TD_ERR_UNSUPPORTED, "td_attn_packed: %d heads share a key head", G);
   int bias_bytes = 0;
@@ -546,7 +647,7 @@ extern "C" int td_attn_packed(const void* q, const void* k, const void* v, void*
   p.q = (const uint16_t*)q; p.k = (const uint16_t*)k; p.v = (const uint16_t*)v; p.o = (uint16_t*)o;
   p.q_ts = strides[0]; p.q_hs = strides[1]; p.k_ts = strides[2]; p.k_hs = strides[3];
   p.v_ts = strides[4]; p.v_hs = strides[5]; p.o_ts = strides[6]; p.o_hs = strides[7];
-  p.bias = bias; p.R = bias_range; p.items = reinterpret_cast<const ApItem*>(table);
+  p.bias = bias; p.R = bias_range;
   p.po = ws; p.pml = ws ? ws + (int64_t)kv_heads * wr * head_dim : nullptr; p.ws_rows = wr;
   p.Hkv = kv_heads; p.G = G; p.causal = causal ? 1 : 0;
   p.gmagic = G > 1 ? (uint32_t)(((1ull << 32) + G - 1) / G) : 0;
@@ -555,6 +656,7 @@ extern "C" int td_attn_packed(const void* q, const void* k, const void* v, void*
   for (int few = 0; few < 2; ++few) {
     const int64_t n = few ? nf : nt;
     p.items = reinterpret_cast<const ApItem*>(table) + (few ? nt : 0);
+    p.n_items = (int)n;
     if (n == 0) continue;
 #define AP_GO2(DT_, D_, F_) { if (bias) ap_launch<DT_, D_, F_, true>(p, n, bias_bytes, st); else ap_launch<DT_, D_, F_, false>(p, n, 0, st); }
 #define AP_GO1(DT_, D_) { if (few) AP_GO2(DT_, D_, true) else AP_GO2(DT_, D_, false) }
