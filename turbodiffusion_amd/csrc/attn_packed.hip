@@ -22,10 +22,12 @@
 #include "td_common.h"
 #include <algorithm>
 #include <math.h>
+#include <type_traits>
 #include <vector>
 
 typedef __attribute__((address_space(3))) void* ap_lptr_t;
 typedef short ap_v4s __attribute__((ext_vector_type(4)));
+typedef unsigned ap_u4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) ap_v4s* ap_trptr_t;
 
 #define AP_ROWS 128        // rows of a tile item
@@ -80,6 +82,10 @@ __device__ __forceinline__ void ap_dma(const void* base, uint32_t bytes, char* l
   __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (ap_lptr_t)lds, 16, off, 0, 0, 0);
 }
 
+__device__ __forceinline__ void ap_store(void* base, uint32_t bytes, v4i v, uint32_t off) {   // an offset of `bytes` or more is not stored
+  const auto r = __builtin_amdgcn_make_buffer_rsrc(base, 0, (int)bytes, 0x00020000);
+  __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(ap_u4, v), r, off, 0, 0);
+}
 __device__ __forceinline__ void ap_dma_ptr(const void* src, char* lds) {   // the same from an address per lane
   __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src, (ap_lptr_t)lds, 16, 0, 0);
 }
@@ -185,8 +191,9 @@ __device__ __forceinline__ ApScore ap_score(const ApParams& p, const ApItem& it,
   return sc;
 }
 
-// One key tile of 32 NB keys from kt for a wave's 32 rows: scores, running maximum and sum, P V
-template <int DT, int D, int NB, bool BIAS>
+// One key tile of 32 NB keys from kt for a wave's 32 rows: scores, running maximum and sum, P V.  FIRST: nothing to add to or to
+// rescale, acc, m and l come in undefined.
+template <int DT, int D, int NB, bool BIAS, bool FIRST>
 __device__ __forceinline__ void ap_tile(const ApParams& p, const ApScore& score, const char* sk, const char* sv, uint32_t krow, uint32_t kxor,
                                         uint32_t vrow, uint32_t vxor, int kt, const v4i (&qf)[D / 16], v16f (&acc)[D / 32], float& m, float& mref,
                                         float& l) {
@@ -204,7 +211,11 @@ __device__ __forceinline__ void ap_tile(const ApParams& p, const ApScore& score,
       s[b] = ap_mma<DT>::run(kf, qf[kk], s[b]);
     }
   const float mx = score.template finish<BIAS>(s, kt);
-  if (__any(mx > m + AP_TAU)) {       // a row that does not exceed its reference keeps it: its bits do not depend on its neighbours
+  if constexpr (FIRST) {
+    m = mx;
+    mref = mx == -INFINITY ? 0.f : mx;
+    l = 0.f;
+  } else if (__any(mx > m + AP_TAU)) {   // a row that does not exceed its reference keeps it: its bits do not depend on its neighbours
     const float mn = mx > m + AP_TAU ? mx : m;
     mref = mn == -INFINITY ? 0.f : mn;
     const float alpha = __builtin_amdgcn_exp2f(m - mref);
@@ -234,7 +245,12 @@ __device__ __forceinline__ void ap_tile(const ApParams& p, const ApScore& score,
       const char* a = sv + t * 16 * ROWB + vrow + ((d << 6) ^ vxor);
       const v8s vf = __builtin_shufflevector(__builtin_amdgcn_ds_read_tr16_b64_v4i16((ap_trptr_t)a),
                                              __builtin_amdgcn_ds_read_tr16_b64_v4i16((ap_trptr_t)(a + 4 * ROWB)), 0, 1, 2, 3, 4, 5, 6, 7);
-      acc[d] = ap_mma<DT>::run(__builtin_bit_cast(v4i, vf), pf, acc[d]);
+      if (FIRST && t == 0) {
+        v16f zero;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) zero[r] = 0.f;
+        acc[d] = ap_mma<DT>::run(__builtin_bit_cast(v4i, vf), pf, zero);
+      } else acc[d] = ap_mma<DT>::run(__builtin_bit_cast(v4i, vf), pf, acc[d]);
     }
   }
 }
@@ -256,16 +272,25 @@ __global__ __launch_bounds__(256, 2) void attn_packed_tile_kernel(const ApParams
   float* const lbias = reinterpret_cast<float*>(smem + 2 * STAGE);
   const int drow = lane / (ROWB / 16), dchunk = lane & (ROWB / 16 - 1);
 
-  // ---- Q: whole rows (memory likes full lines) into the wave's part of stage 1, until tile 1 comes ----
+  // ---- Q: whole rows (memory likes full lines) into the wave's part of stage 1, until tile 1 comes; rows past the end are not
+  //      read (whatever LDS holds, never stored).  One head per key head: the rows are evenly spaced, a bounds-checked buffer needs
+  //      no comparison, and the permutation of a row's chunks has a period of PER groups ----
   char* const qstage = smem + STAGE + x0 * ROWB;
-  {
+  constexpr int PER = D == 128 ? 4 : 2;
+  static_assert(D == 128 || D == 64, "ap_kx of row RPP t + r is ap_kx of row RPP (t mod PER) + r");
+  if (p.G == 1) {
+    const uint16_t* const qhead = p.q + (int64_t)it.token * p.q_ts + (int64_t)kvh * p.q_hs;
+    const uint32_t bytes = (uint32_t)((it.rows - 1) * 2 * p.q_ts + ROWB), row = (uint32_t)(2 * p.q_ts);
+#pragma unroll
+    for (int t = 0; t < 32 / RPP; ++t)
+      ap_dma(qhead, bytes, qstage + t * 1024, (x0 + drow) * row + ((dchunk ^ ap_kx<D>(RPP * (t % PER) + drow)) << 4) + t * RPP * row);
+  } else {
     const uint16_t* const qhead = p.q + (int64_t)it.token * p.q_ts + (int64_t)kvh * p.G * p.q_hs;
     ApRowWalk<D> w(p, it, x0 + drow, p.q_ts, p.q_hs);
 #pragma unroll
     for (int t = 0; t < 32 / RPP; ++t, w.next()) {
       const int x = RPP * t + drow;
-      if (x0 + x < it.rows)                                            // rows past the end: whatever LDS holds, never stored
-        ap_dma_ptr(qhead + w.at + 8 * (dchunk ^ ap_kx<D>(x)), qstage + t * 1024);
+      if (x0 + x < it.rows) ap_dma_ptr(qhead + w.at + 8 * (dchunk ^ ap_kx<D>(x)), qstage + t * 1024);
     }
   }
   // ---- K, V: piece i of this wave is rows RPP (wave + 4 i) ..; rows past the range re-read the last one (finite, masked) ----
@@ -322,18 +347,25 @@ __global__ __launch_bounds__(256, 2) void attn_packed_tile_kernel(const ApParams
   const uint32_t vxor = ap_vx<D>(vkey) << 4;                                    // a multiple of 64: moves whole 32-d blocks
 
   v16f acc[DB];
-#pragma unroll
-  for (int d = 0; d < DB; ++d)
-#pragma unroll
-    for (int r = 0; r < 16; ++r) acc[d][r] = 0.f;
-  float m = -INFINITY, mref = 0.f, l = 0.f;
-  for (int buf = 0; kt < kend; kt += 64, buf ^= 1) {
+  float m, mref, l;
+  auto tile = [&](auto first, int buf) {
     if (kt + 64 < kend) fetch(kt + 64, buf ^ 1);
-    if (kt < wend) ap_tile<DT, D, 2, BIAS>(p, score, smem + buf * STAGE, smem + buf * STAGE + TILE, krow, kxor, vrow, vxor, kt, qf, acc, m, mref, l);
+    if (kt < wend)
+      ap_tile<DT, D, 2, BIAS, decltype(first)::value>(p, score, smem + buf * STAGE, smem + buf * STAGE + TILE, krow, kxor, vrow, vxor, kt, qf, acc, m, mref, l);
     // this tile's reads have returned and the next tile has landed
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
     __syncthreads();
+    kt += 64;
+  };
+  if (kt >= wend) {                 // rows that see nothing
+    m = -INFINITY; l = 0.f;
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[d][r] = 0.f;
   }
+  if (kt < kend) tile(std::true_type{}, 0);
+  for (int buf = 1; kt < kend; buf ^= 1) tile(std::false_type{}, buf);
   l = ap_other_half(l, false);
 
   // ---- results.  acc[d][r] is d = 32 d + 8 (r >> 2) + 4 half + (r & 3) of this lane's row ----
@@ -365,13 +397,24 @@ __global__ __launch_bounds__(256, 2) void attn_packed_tile_kernel(const ApParams
       *reinterpret_cast<uint4*>(ost + r32 * ROWB + (((4 * d + 2 * j + half) ^ ap_kx<D>(r32)) << 4)) = make_uint4(s0[0], s1[0], s0[1], s1[1]);
     }
   __builtin_amdgcn_wave_barrier();
-  uint16_t* const ohead = p.o + (int64_t)it.token * p.o_ts + (int64_t)kvh * p.G * p.o_hs + 8 * dchunk;
-  ApRowWalk<D> w(p, it, x0 + drow, p.o_ts, p.o_hs);
+  if (p.G == 1) {
+    uint16_t* const ohead = p.o + (int64_t)it.token * p.o_ts + (int64_t)kvh * p.o_hs;
+    const uint32_t bytes = (uint32_t)((it.rows - 1) * 2 * p.o_ts + ROWB), row = (uint32_t)(2 * p.o_ts);
 #pragma unroll
-  for (int t = 0; t < 32 / RPP; ++t, w.next()) {
-    const uint32_t y = RPP * t + drow;
-    const uint4 v = *reinterpret_cast<const uint4*>(ost + y * ROWB + ((dchunk ^ ap_kx<D>(y)) << 4));
-    if (x0 + (int)y < it.rows) *reinterpret_cast<uint4*>(ohead + w.at) = v;
+    for (int t = 0; t < 32 / RPP; ++t) {
+      const uint32_t y = RPP * (t % PER) + drow;
+      const v4i v = *reinterpret_cast<const v4i*>(ost + (y + RPP * (t - t % PER)) * ROWB + ((dchunk ^ ap_kx<D>(y)) << 4));
+      ap_store(ohead, bytes, v, (x0 + drow) * row + 16 * dchunk + t * RPP * row);
+    }
+  } else {
+    uint16_t* const ohead = p.o + (int64_t)it.token * p.o_ts + (int64_t)kvh * p.G * p.o_hs + 8 * dchunk;
+    ApRowWalk<D> w(p, it, x0 + drow, p.o_ts, p.o_hs);
+#pragma unroll
+    for (int t = 0; t < 32 / RPP; ++t, w.next()) {
+      const uint32_t y = RPP * t + drow;
+      const uint4 v = *reinterpret_cast<const uint4*>(ost + y * ROWB + ((dchunk ^ ap_kx<D>(y)) << 4));
+      if (x0 + (int)y < it.rows) *reinterpret_cast<uint4*>(ohead + w.at) = v;
+    }
   }
 }
 
@@ -440,7 +483,7 @@ __global__ __launch_bounds__(256, 1) void attn_packed_few_kernel(const ApParams 
   for (int buf = 0; kt < kend; kt += 4 * BK, buf ^= 1) {
     if (kt + 4 * BK < kend) fetch(kt + 4 * BK, buf ^ 1);
     const char* sk = mystage + buf * STAGE;
-    ap_tile<DT, D, NB, BIAS>(p, score, sk, sk + TILE, krow, kxor, vrow, vxor, kt, qf, acc, m, mref, l);
+    ap_tile<DT, D, NB, BIAS, false>(p, score, sk, sk + TILE, krow, kxor, vrow, vxor, kt, qf, acc, m, mref, l);
     // this tile's reads have returned and the next tile has landed (the stages are this wave's own)
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
   }
@@ -626,7 +669,8 @@ extern "C" int td_attn_packed(const void* q, const void* k, const void* v, void*
   TD_REQUIRE(kv_heads > 0 && heads > 0 && heads % kv_heads == 0, TD_ERR_INVALID, "td_attn_packed: %d heads over %d key heads", heads, kv_heads);
   for (int i = 0; i < 8; ++i)
     TD_REQUIRE(strides[i] >= 0 && strides[i] % 8 == 0, TD_ERR_UNSUPPORTED, "td_attn_packed: stride %lld (a multiple of 8 elements)", (long long)strides[i]);
-  TD_REQUIRE(strides[2] < (1 << 24) && strides[4] < (1 << 24), TD_ERR_UNSUPPORTED, "td_attn_packed: key / value token stride of 2^24 elements or more");
+  for (int i = 0; i < 8; i += 2)
+    TD_REQUIRE(strides[i] < (1 << 24), TD_ERR_UNSUPPORTED, "td_attn_packed: token stride %lld (less than 2^24 elements)", (long long)strides[i]);
   TD_REQUIRE((((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)o | (uintptr_t)ws) & 15) == 0, TD_ERR_UNSUPPORTED,
              "td_attn_packed: pointers must be 16-byte aligned");
   TD_REQUIRE(scale > 0.f && scale <= 3.0e38f, TD_ERR_INVALID, "td_attn_packed: scale must be positive and finite");
