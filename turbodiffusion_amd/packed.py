@@ -62,11 +62,11 @@ class _Plan:
 
 def _check_tensors(what, dev, *tensors):
     """GPU tensors on ``dev`` that want no gradient (None: an argument left out)"""
-    grad = torch.is_grad_enabled()
+    index, grad = dev.index, torch.is_grad_enabled()
     for t in tensors:
         if t is None:
             continue
-        if t.device != dev:
+        if t.get_device() != index:
             require_gpu(t)
             raise ValueError(f"{what}: the plan and every tensor must be on one device ({dev}, got {t.device})")
         if grad and t.requires_grad:
