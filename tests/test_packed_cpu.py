@@ -148,3 +148,24 @@ def test_adapter_workspace_of_every_plan():
                 assert out.value == 0 if rows == 0 else out.value >= rows * rank // 2
     with pytest.raises(L.TurboDiffusionAMDError):
         L.call("td_lora_workspace", c, 64, 257, ctypes.byref(out))
+
+
+@pytest.mark.parametrize("bidirectional", [True, False])
+def test_relative_bias_is_the_table_by_bucket(bidirectional):
+    from turbodiffusion_amd.text_encoder import relative_buckets
+    table = torch.arange(32 * 3, dtype=torch.float32).view(32, 3)
+    v = ops.relative_bias(table, max_dist=128, bidirectional=bidirectional)
+    assert v.shape == (3, 257) and v.dtype == torch.float32 and v.is_contiguous()
+    if bidirectional:
+        b = relative_buckets(300, 32, 128, "cpu")
+        rel = (torch.arange(300)[None, :] - torch.arange(300)[:, None]).clamp(-128, 128)
+        for h in range(3):
+            assert torch.equal(v[h][rel + 128], table[b][:, :, h])
+    else:
+        near = [int(v[0, 128 - d]) // 3 for d in range(16)]
+        assert near == list(range(16)) and (v[:, 128:] == table[0][:, None]).all() and (v[:, 0] == table[31]).all()
+        assert (v[0, :129].diff() <= 0).all()                       # further back: never a smaller bucket
+    with pytest.raises(ValueError):
+        ops.relative_bias(table[0])
+    with pytest.raises(ValueError):
+        ops.relative_bias(table, max_dist=4)

@@ -11,10 +11,10 @@ import torch
 import torch.nn as nn
 
 from . import kernels as K
-from .packed import AdapterBank, AdapterPlan, AttentionPlan, lora_add, packed_attention
+from .packed import AdapterBank, AdapterPlan, AttentionPlan, lora_add, packed_attention, relative_bias
 
 __all__ = ["int8_quant", "int8_linear", "rmsnorm", "layernorm", "Int8Linear", "FastRMSNorm", "FastLayerNorm",
-           "AttentionPlan", "packed_attention", "AdapterBank", "AdapterPlan", "lora_add"]
+           "AttentionPlan", "packed_attention", "relative_bias", "AdapterBank", "AdapterPlan", "lora_add"]
 
 
 def int8_quant(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:

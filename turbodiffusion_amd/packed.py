@@ -172,6 +172,35 @@ def packed_attention(q, k, v, plan, scale=None, bias=None, out=None):
     return out
 
 
+def distance_buckets(rel, num_buckets, max_dist, bidirectional=True):
+    """Bucket ids of distances ``rel`` = key - query (T5RelativeEmbedding._relative_position_bucket, umt5.py:289-305): half of a
+    direction's buckets hold one distance each, the others widen logarithmically up to ``max_dist``.  Not bidirectional: later
+    keys share bucket 0 and earlier ones have all buckets."""
+    nb = num_buckets // 2 if bidirectional else num_buckets
+    exact = nb // 2
+    if exact < 1 or max_dist <= exact:
+        raise ValueError(f"{num_buckets} buckets up to distance {max_dist} leave none to widen")
+    if bidirectional:
+        out = (rel > 0).long() * nb
+        rel = rel.abs()
+    else:
+        out = torch.zeros_like(rel)
+        rel = (-rel).clamp(min=0)
+    large = exact + (torch.log(rel.float() / exact) / math.log(max_dist / exact) * (nb - exact)).long()
+    large = torch.min(large, torch.full_like(large, nb - 1))
+    return out + torch.where(rel < exact, rel, large)
+
+
+def relative_bias(table, max_dist=128, bidirectional=True):
+    """The learned relative position bias as ``packed_attention`` reads it: ``table`` [buckets, heads] -> f32 [heads, 2 max_dist + 1],
+    entry max_dist + d for key - query = d; every distance beyond max_dist is in its direction's last bucket.  Laid out once
+    per layer."""
+    if table.dim() != 2:
+        raise ValueError(f"relative_bias: table is {tuple(table.shape)}, wanted [buckets, heads]")
+    rel = torch.arange(-max_dist, max_dist + 1, device=table.device)
+    return table.detach().float()[distance_buckets(rel, table.shape[0], max_dist, bidirectional)].t().contiguous()
+
+
 class AdapterBank:
     """Low-rank pairs for ONE projection, laid out once: ``pairs[i]`` = (A [rank, k], B [n, rank]), all bf16 or all f16, ranks of
     1 to 256 that may differ; ``scales[i]`` (default 1) multiplies the update (the usual alpha / rank)."""

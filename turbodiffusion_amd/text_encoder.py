@@ -28,10 +28,10 @@ is ``oracle/f4_ref.py``.  Tokenisation (umt5.py:58-98) is ``tokenizer.Huggingfac
 (umt5.py:479-545) on top of both."""
 from __future__ import annotations
 
-import math
-
 import torch
 import torch.nn.functional as F
+
+from .packed import AdapterBank, AdapterPlan, AttentionPlan, distance_buckets, lora_add, packed_attention, relative_bias
 
 
 def _fp16_clamp(x):
@@ -44,13 +44,7 @@ def _fp16_clamp(x):
 def relative_buckets(L: int, num_buckets: int, max_dist: int, device) -> torch.Tensor:
     """[L, L] bucket ids of (key - query), bidirectional (T5RelativeEmbedding._relative_position_bucket, umt5.py:289-305)."""
     rel = torch.arange(L, device=device).unsqueeze(0) - torch.arange(L, device=device).unsqueeze(1)
-    nb = num_buckets // 2
-    out = (rel > 0).long() * nb
-    rel = rel.abs()
-    exact = nb // 2
-    large = exact + (torch.log(rel.float() / exact) / math.log(max_dist / exact) * (nb - exact)).long()
-    large = torch.min(large, torch.full_like(large, nb - 1))
-    return out + torch.where(rel < exact, rel, large)
+    return distance_buckets(rel, num_buckets, max_dist)
 
 
 def synthetic_state_dict(layers=24, dim=4096, dim_ffn=10240, heads=64, vocab=256384, num_buckets=32, seed=0,
@@ -77,10 +71,14 @@ def synthetic_state_dict(layers=24, dim=4096, dim_ffn=10240, heads=64, vocab=256
 class Umt5Encoder:
     """``encoder(ids, mask)`` -> [B, L_pad, dim]: ``ids`` / ``mask`` [B, L_pad] as the reference's tokenizer returns them
     (padding on the right).  ``state_dict``: the reference encoder's (``models_t5_umt5-xxl-enc-bf16.pth`` layout); the
-    configuration is read off the tensors.  16-bit on a GPU (the reference loads the bf16 checkpoint, umt5.py:478-488)."""
+    configuration is read off the tensors.  16-bit on a GPU (the reference loads the bf16 checkpoint, umt5.py:478-488).
 
-    def __init__(self, state_dict, dtype=torch.bfloat16, device="cuda", max_dist=128, eps=1e-6):
-        self.dtype, self.device, self.max_dist, self.eps = dtype, torch.device(device), max_dist, eps
+    ``packed=True``: all prompts of a call go through the layers together, their valid tokens behind one another
+    (``encode_packed``).  The rounding points differ from the default path's (scores and their bias stay fp32), so results agree
+    within 16-bit rounding, not bit for bit."""
+
+    def __init__(self, state_dict, dtype=torch.bfloat16, device="cuda", max_dist=128, eps=1e-6, packed=False):
+        self.dtype, self.device, self.max_dist, self.eps, self.packed = dtype, torch.device(device), max_dist, eps, packed
         if dtype not in (torch.bfloat16, torch.float16) or self.device.type != "cuda":
             raise ValueError("Umt5Encoder runs on the HIP kernels only: bf16 / fp16 on a GPU; the library-operator restatement "
                              "for CPU checks is oracle/f4_ref.py")
@@ -119,6 +117,7 @@ class Umt5Encoder:
         self.num_buckets, self.num_heads = pos0.shape
         self.dim_attn = self.layers[0]["o"].shape[1]
         assert self.dim_attn % self.num_heads == 0
+        self._distance_bias = None      # per layer, laid out at the first packed call
 
     @classmethod
     def from_reference(cls, module_or_state_dict, **kw):
@@ -154,6 +153,45 @@ class Umt5Encoder:
         return K.t5_norm(x, self.final_norm, self.eps)
 
     @torch.no_grad()
+    def encode_packed(self, prompts, adapters=None, adapter_ids=None):
+        """Many prompts in one pass: ``prompts`` = the token ids of each (1-D tensors or lists, any lengths, no padding) -> one
+        [n, dim] tensor for each.  Every linear runs once over the rows of all prompts, attention stays within each.
+        ``adapters``: ``Umt5Adapters``; prompt i is encoded with adapter ``adapter_ids[i]`` (-1: with the plain weights)."""
+        K, H = self.K, self.num_heads
+        c = self.dim_attn // H
+        ids = [torch.as_tensor(p, dtype=torch.long).reshape(-1) for p in prompts]
+        lens = [p.numel() for p in ids]
+        if (adapters is None) != (adapter_ids is None):
+            raise ValueError("encode_packed: adapters and adapter_ids go together")
+        if adapters is not None and len(adapter_ids) != len(lens):
+            raise ValueError(f"encode_packed: {len(lens)} prompts, {len(adapter_ids)} adapter ids")
+        plan = AttentionPlan(lens, heads=H, head_dim=c, device=self.device)
+        if plan.tokens == 0:
+            return [torch.empty(0, self.dim, dtype=self.dtype, device=self.device) for _ in lens]
+        rows = None
+        if adapters is not None:
+            adapters.check(self, adapter_ids)
+            rows = AdapterPlan(lens, adapter_ids, device=self.device)
+        if self._distance_bias is None:
+            tables = [self.pos] if self.shared_pos else [lay["pos"] for lay in self.layers]
+            self._distance_bias = [relative_bias(t, self.max_dist) for t in tables]
+
+        def adapt(y, x, layer, target):     # in place
+            bank = None if rows is None else adapters.banks[layer].get(target)
+            return y if bank is None else lora_add(y, x, bank, rows, out=y)
+
+        x = F.embedding(torch.cat([p.to(self.device) for p in ids]), self.emb)                   # gather (plumbing)
+        for i, lay in enumerate(self.layers):
+            h = K.t5_norm(x, lay["n1"], self.eps)
+            qkv = adapt(K.gemm_bf16(h, lay["qkv"]), h, i, "qkv").view(-1, 3, H, c)
+            o = packed_attention(qkv[:, 0], qkv[:, 1], qkv[:, 2], plan, scale=1.0,               # no 1/sqrt(d) (umt5.py:183)
+                                 bias=self._distance_bias[0 if self.shared_pos else i]).view(-1, H * c)
+            x = _fp16_clamp(adapt(K.gemm_bf16(o, lay["o"], res=x), o, i, "o"))
+            h = K.gemm_bf16(K.t5_norm(x, lay["n2"], self.eps), lay["gf"], epilogue="geglu")
+            x = _fp16_clamp(adapt(K.gemm_bf16(h, lay["fc2"], res=x), h, i, "fc2"))
+        return list(K.t5_norm(x, self.final_norm, self.eps).split(lens))
+
+    @torch.no_grad()
     def __call__(self, ids, mask=None):
         ids = ids.to(self.device)
         B, Lp = ids.shape
@@ -162,19 +200,76 @@ class Umt5Encoder:
         for b, n in enumerate(lens):
             if mask is not None and n > 0 and not bool(mask[b, :n].to(self.device).gt(0).all()):
                 raise ValueError("mask must be right-padded (valid tokens first), as the reference's tokenizer produces it")
-            if n > 0:
+            if n > 0 and not self.packed:
                 out[b, :n] = self._rows(ids[b, :n])
+        if self.packed:
+            for b, rows in enumerate(self.encode_packed([ids[b, :n] for b, n in enumerate(lens)])):
+                out[b, :lens[b]] = rows
         return out
+
+
+class Umt5Adapters:
+    """Low-rank adapters of many requests for one ``Umt5Encoder``: ``adapters[j]`` = {"blocks.0.attn.q": (A [rank, in], B [out, rank]),
+    ...} over attn.q / attn.k / attn.v / attn.o / ffn.fc2 of any blocks, ``scales[j]`` (default 1) multiplies its updates.  The q, k
+    and v pairs of a block become one pair of the fused projection (ranks side by side, B block by block).  ffn.gate / ffn.fc1 have
+    none: their activation rides in the projection's epilogue, in front of which an update would have to land."""
+
+    TARGETS = ("attn.q", "attn.k", "attn.v", "attn.o", "ffn.fc2")
+
+    def __init__(self, encoder, adapters, scales=None):
+        self.encoder, self.n = encoder, len(adapters)
+        if not adapters:
+            raise ValueError("Umt5Adapters: no adapters")
+        dim, da, df, dt, dev = encoder.dim, encoder.dim_attn, encoder.dim_ffn, encoder.dtype, encoder.device
+        shape = {"attn.q": (da, dim), "attn.k": (da, dim), "attn.v": (da, dim), "attn.o": (dim, da), "ffn.fc2": (dim, df)}
+        known = {f"blocks.{i}.{t}" for i in range(len(encoder.layers)) for t in self.TARGETS}
+        for j, ad in enumerate(adapters):
+            for name, (a, b) in ad.items():
+                if name not in known:
+                    raise ValueError(f"Umt5Adapters: adapter {j} names {name!r}; supported: blocks.0 .. {len(encoder.layers) - 1}, {', '.join(self.TARGETS)}")
+                out, inp = shape[name.split(".", 2)[2]]
+                if a.dim() != 2 or b.dim() != 2 or a.shape[1] != inp or b.shape != (out, a.shape[0]):
+                    raise ValueError(f"Umt5Adapters: adapter {j}, {name}: {tuple(a.shape)} / {tuple(b.shape)}, wanted [rank, {inp}] / [{out}, rank]")
+
+        def pair(j, i, targets, width):
+            a, b, row = [], [], 0
+            for t in targets:
+                ab = adapters[j].get(f"blocks.{i}.{t}")
+                out, inp = shape[t]
+                if ab is not None:
+                    a.append(ab[0].to(dev, dt))
+                    wide = torch.zeros(width, ab[0].shape[0], dtype=dt, device=dev)
+                    wide[row:row + out] = ab[1].to(dev, dt)
+                    b.append(wide)
+                row += out
+            if not a:      # this adapter leaves the projection alone: an update of zero
+                return torch.zeros(1, shape[targets[0]][1], dtype=dt, device=dev), torch.zeros(width, 1, dtype=dt, device=dev)
+            return torch.cat(a), torch.cat(b, 1)
+
+        self.banks = []
+        for i in range(len(encoder.layers)):
+            banks = {}
+            for key, targets, width in (("qkv", ("attn.q", "attn.k", "attn.v"), 3 * da), ("o", ("attn.o",), dim), ("fc2", ("ffn.fc2",), dim)):
+                if any(f"blocks.{i}.{t}" in ad for ad in adapters for t in targets):
+                    banks[key] = AdapterBank([pair(j, i, targets, width) for j in range(self.n)], scales, device=dev)
+            self.banks.append(banks)
+
+    def check(self, encoder, adapter_ids):
+        if encoder is not self.encoder:
+            raise ValueError("Umt5Adapters: made for another encoder")
+        if any(not -1 <= i < self.n for i in adapter_ids):
+            raise ValueError(f"adapter ids {list(adapter_ids)}: -1 (none) to {self.n - 1}")
 
 
 class UMT5EncoderModel:
     """The reference's ``UMT5EncoderModel`` (umt5.py:479-521): checkpoint + tokenizer -> ``model(texts)`` = [B, text_len, 4096]
     with the rows past each prompt's length zero.  ``checkpoint_path``: the reference's ``models_t5_umt5-xxl-enc-bf16.pth`` (a
     plain state dict) or a state dict already in memory; ``tokenizer_path``: a local ``tokenizer.json`` / directory
-    (``tokenizer.HuggingfaceTokenizer``; the reference's default is the hub id, there is no network here)."""
+    (``tokenizer.HuggingfaceTokenizer``; the reference's default is the hub id, there is no network here).  ``packed``: all texts of
+    a call in one pass (``Umt5Encoder``)."""
 
     def __init__(self, text_len=512, dtype=torch.bfloat16, device="cuda", checkpoint_path="models_t5_umt5-xxl-enc-bf16.pth",
-                 tokenizer_path="google/umt5-xxl"):
+                 tokenizer_path="google/umt5-xxl", packed=False):
         from .tokenizer import HuggingfaceTokenizer
         self.text_len, self.dtype, self.device = text_len, dtype, device
         if isinstance(checkpoint_path, dict):
@@ -182,7 +277,7 @@ class UMT5EncoderModel:
         else:
             assert str(checkpoint_path).endswith(".pth")                       # umt5.py:496
             sd = torch.load(checkpoint_path, map_location="cpu", weights_only=True)
-        self.model = Umt5Encoder(sd, dtype=dtype, device=device)
+        self.model = Umt5Encoder(sd, dtype=dtype, device=device, packed=packed)
         self.tokenizer = HuggingfaceTokenizer(name=tokenizer_path, seq_len=text_len, clean="whitespace")
 
     def __call__(self, texts, device=None):
