@@ -255,13 +255,16 @@ __device__ __forceinline__ void ap_tile(const ApParams& p, const ApScore& score,
   }
 }
 
-// ---- 128 rows, 32 per wave; key tiles of 64 shared by the waves, two LDS stages, one barrier a tile ----
-// What bounds it: for long ranges the matrix pipe (32 MFMAs of 32 cycles a wave and tile for D = 128) and the vector unit (32
-// exponentials of 16 cycles, some 125 other instructions) together, at the clock that the power limit leaves; for short ranges the
-// vector instructions around the loop, hence pointers that step instead of addresses computed row by row.
+// ---- 128 rows, 32 per wave; key tiles of 32 shared by the waves, two LDS stages, one barrier a tile ----
+// What bounds it.  Long ranges: the matrix pipe at the clock that the power limit leaves (causal, 32 760 tokens, 12 heads of 128: 2.97
+// ms, 1.11 PFLOP/s, 0.80 of a large library product on the same card; with the softmax arithmetic taken out 2.72 ms).  Short
+// ranges: the latency of a workgroup's first loads and the vector instructions around the loop.  Hence tiles of 32 keys - three
+// (D = 64: four) workgroups a CU instead of two: 226 keys under 50 960 rows of 12 heads 94 against 100 us, prompts of 1 to 512
+// tokens, 64 heads of 64, 35.3 against 36.7, the long range 1 % slower - and pointers that step instead of addresses
+// computed row by row (1250 -> 950 vector instructions a wave at 226 keys, 107 -> 100 us).
 template <int DT, int D, bool BIAS>
-__global__ __launch_bounds__(256, 2) void attn_packed_tile_kernel(const ApParams p) {
-  constexpr int ROWB = 2 * D, TILE = 64 * ROWB, STAGE = 2 * TILE, PIECES = TILE / 4096, RPP = 1024 / ROWB, KK = D / 16, DB = D / 32;
+__global__ __launch_bounds__(256, D == 128 ? 3 : 4) void attn_packed_tile_kernel(const ApParams p) {
+  constexpr int BK = 32, ROWB = 2 * D, TILE = BK * ROWB, STAGE = 2 * TILE, PIECES = TILE / 4096, RPP = 1024 / ROWB, KK = D / 16, DB = D / 32;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int item = blockIdx.z * AP_GRID_Y + blockIdx.y, kvh = blockIdx.x;
   if (item >= p.n_items) return;
@@ -269,10 +272,10 @@ __global__ __launch_bounds__(256, 2) void attn_packed_tile_kernel(const ApParams
   const int lane = threadIdx.x & 63, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int x0 = 32 * wave, bn = 2 * p.R + 1 + 2 * AP_PAD;
-  float* const lbias = reinterpret_cast<float*>(smem + 2 * STAGE);
+  float* const lbias = reinterpret_cast<float*>(smem + STAGE + AP_ROWS * ROWB);       // stage 1 and behind: Q, at the end O
   const int drow = lane / (ROWB / 16), dchunk = lane & (ROWB / 16 - 1);
 
-  // ---- Q: whole rows (memory likes full lines) into the wave's part of stage 1, until tile 1 comes; rows past the end are not
+  // ---- Q: whole rows (memory likes full lines) into LDS from stage 1 on, until tile 1 comes; rows past the end are not
   //      read (whatever LDS holds, never stored).  One head per key head: the rows are evenly spaced, a bounds-checked buffer needs
   //      no comparison, and the permutation of a row's chunks has a period of PER groups ----
   char* const qstage = smem + STAGE + x0 * ROWB;
@@ -300,12 +303,12 @@ __global__ __launch_bounds__(256, 2) void attn_packed_tile_kernel(const ApParams
   const uint16_t* const kbase = p.k + (int64_t)it.k_begin * p.k_ts + (int64_t)kvh * p.k_hs;
   const uint16_t* const vbase = p.v + (int64_t)it.k_begin * p.v_ts + (int64_t)kvh * p.v_hs;
   auto fetch = [&](int kt, int buf) {
-    const int nv = min(it.key1 - kt, 64);
+    const int nv = min(it.key1 - kt, BK);
     const uint16_t* kp = kbase + (int64_t)kt * p.k_ts;
     const uint16_t* vp = vbase + (int64_t)kt * p.v_ts;
     const uint32_t kbytes = (uint32_t)((nv - 1) * 2 * p.k_ts + ROWB), vbytes = (uint32_t)((nv - 1) * 2 * p.v_ts + ROWB);
     char* st = smem + buf * STAGE + wave * 1024;
-    if (nv == 64) {
+    if (nv == BK) {
 #pragma unroll
       for (int i = 0; i < PIECES; ++i) {
         ap_dma(kp, kbytes, st + i * 4096, koff + i * (uint32_t)(8 * RPP * p.k_ts));
@@ -349,13 +352,13 @@ __global__ __launch_bounds__(256, 2) void attn_packed_tile_kernel(const ApParams
   v16f acc[DB];
   float m, mref, l;
   auto tile = [&](auto first, int buf) {
-    if (kt + 64 < kend) fetch(kt + 64, buf ^ 1);
+    if (kt + BK < kend) fetch(kt + BK, buf ^ 1);
     if (kt < wend)
-      ap_tile<DT, D, 2, BIAS, decltype(first)::value>(p, score, smem + buf * STAGE, smem + buf * STAGE + TILE, krow, kxor, vrow, vxor, kt, qf, acc, m, mref, l);
+      ap_tile<DT, D, 1, BIAS, decltype(first)::value>(p, score, smem + buf * STAGE, smem + buf * STAGE + TILE, krow, kxor, vrow, vxor, kt, qf, acc, m, mref, l);
     // this tile's reads have returned and the next tile has landed
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
     __syncthreads();
-    kt += 64;
+    kt += BK;
   };
   if (kt >= wend) {                 // rows that see nothing
     m = -INFINITY; l = 0.f;
@@ -383,7 +386,7 @@ __global__ __launch_bounds__(256, 2) void attn_packed_tile_kernel(const ApParams
   }
   // through the wave's own 32 rows of LDS (every wave is done with the stages): whole rows go out
   const float inv = l == 0.f ? 0.f : 1.0f / l;
-  char* const ost = smem + x0 * ROWB;
+  char* const ost = smem + STAGE + x0 * ROWB;
   const uint32_t r32 = lane & 31;
 #pragma unroll
   for (int d = 0; d < DB; ++d)
@@ -678,7 +681,7 @@ extern "C" int td_attn_packed_plan(const int64_t* lens_q, const int64_t* lens_k,
 template <int DT, int D, bool FEW, bool BIAS>
 static void ap_launch(const ApParams& p, int64_t n, int bias_bytes, hipStream_t st) {
   static std::atomic<uint64_t> mask{0};
-  constexpr int tiles = FEW ? 131072 : 4 * 64 * 2 * D;       // two stages of K + V; few: of 8 KB each for every wave
+  constexpr int tiles = FEW ? 131072 : (64 + AP_ROWS) * 2 * D;       // a stage of K + V and the rows; few: 2 stages of 16 KB for each wave
   const auto kernel = FEW ? attn_packed_few_kernel<DT, D, BIAS> : attn_packed_tile_kernel<DT, D, BIAS>;
   td_ensure_dyn_lds((const void*)kernel, tiles + 32768, mask);
   const dim3 grid((unsigned)p.Hkv, (unsigned)std::min<int64_t>(n, AP_GRID_Y), (unsigned)td_cdiv(n, AP_GRID_Y));
