@@ -152,6 +152,19 @@ def test_several_tokens_over_a_long_past_split(D):
     check(ops.packed_attention(q, k, v, plan), ref, tol)
 
 
+@pytest.mark.parametrize("D,heads", [(128, (40, 1)), (64, (64, 1)), (64, (300, 2)), (128, (7, 7))])
+def test_many_heads_on_one_key_head(D, heads):
+    """one token's heads fill a tile and spill into the next; rows walk over heads and tokens in every combination"""
+    H, Hkv = heads
+    lens, lens_k = [3, 1, 70, 17], [3, 900, 100, 17]
+    for layout in ("plain", "padded", "heads"):
+        q, k, v = make(lens, lens_k, H, Hkv, D, torch.float16, layout, seed=6)
+        for causal in (True, False):
+            plan = ops.AttentionPlan(lens, lens_k, heads=H, kv_heads=Hkv, head_dim=D, causal=causal)
+            ref, tol = formula(q, k, v, lens, lens_k, causal)
+            check(ops.packed_attention(q, k, v, plan), ref, tol)
+
+
 def test_large_scores_and_growing_maxima():
     """scores of +-200 whose running maximum rises tile after tile; equal scores; a positive scale far from the default"""
     lens = [400, 64]
@@ -278,6 +291,8 @@ def test_refusals():
     for scale in (0.0, -1.0, math.inf, math.nan):
         with pytest.raises(ValueError):
             call(q, k, v, plan, scale=scale)
+    with pytest.raises(TurboDiffusionAMDError):
+        call(q, k, v, plan, scale=2e38)
     with pytest.raises(ValueError):
         call(q, k, v, plan, bias=torch.zeros(4, 6, device="cuda"))
     with pytest.raises(TypeError):

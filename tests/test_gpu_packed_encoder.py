@@ -150,5 +150,8 @@ def test_encoder_refusals():
         TE.Umt5Adapters(enc, [{"blocks.0.ffn.fc2": ads[0]["blocks.0.attn.q"]}])
     with pytest.raises(ValueError):
         TE.Umt5Adapters(enc, [])
+    for bad in (97, -1):
+        with pytest.raises(ValueError):
+            enc.encode_packed([[1, bad]])
     with pytest.raises(ValueError):                      # heads of 32
         TE.Umt5Encoder(encoder_weights(heads=8)).encode_packed(p)

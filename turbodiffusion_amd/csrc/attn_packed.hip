@@ -369,6 +369,7 @@ __global__ __launch_bounds__(256, D == 128 ? 3 : 4) void attn_packed_tile_kernel
   }
   if (kt < kend) tile(std::true_type{}, 0);
   for (int buf = 1; kt < kend; buf ^= 1) tile(std::false_type{}, buf);
+  if (x0 >= it.rows) return;        // no barrier behind this
   l = ap_other_half(l, false);
 
   // ---- results.  acc[d][r] is d = 32 d + 8 (r >> 2) + 4 half + (r & 3) of this lane's row ----
@@ -701,7 +702,7 @@ extern "C" int td_attn_packed(const void* q, const void* k, const void* v, void*
     TD_REQUIRE(strides[i] < (1 << 24), TD_ERR_UNSUPPORTED, "td_attn_packed: token stride %lld (less than 2^24 elements)", (long long)strides[i]);
   TD_REQUIRE((((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)o | (uintptr_t)ws) & 15) == 0, TD_ERR_UNSUPPORTED,
              "td_attn_packed: pointers must be 16-byte aligned");
-  TD_REQUIRE(scale > 0.f && scale <= 3.0e38f, TD_ERR_INVALID, "td_attn_packed: scale must be positive and finite");
+  TD_REQUIRE(scale > 0.f && scale <= 1e38f, TD_ERR_INVALID, "td_attn_packed: scale must be positive, at most 1e38");
   const int64_t nt = counts[0], nf = counts[1], nj = counts[2], wr = counts[3];
   TD_REQUIRE(nt >= 0 && nf >= 0 && nj >= 0 && wr >= 0 && (nj == 0 || ws), TD_ERR_INVALID, "td_attn_packed: counts / workspace");
   TD_REQUIRE(counts[5] == 0 || (k && v), TD_ERR_INVALID, "td_attn_packed: null keys or values");

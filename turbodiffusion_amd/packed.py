@@ -49,14 +49,16 @@ class _Plan:
             self._stream = torch.cuda.current_stream().cuda_stream
             self.table = host.to(self.device)          # synchronous: complete for every stream
 
-    def _launch(self, fn):
-        """``fn(stream)`` with the plan's device current; the table stays allocated while that stream needs it"""
+    def _launch(self, fn, *held):
+        """``fn(stream)`` with the plan's device current; the table and ``held`` (what else the framework keeps for the caller) stay
+        allocated while that stream needs them"""
         if _current_device() != self.device.index:
             with torch.cuda.device(self.device):
-                return self._launch(fn)
+                return self._launch(fn, *held)
         stream = _raw_stream(self.device.index)
-        if stream != self._stream:
-            self.table.record_stream(torch.cuda.current_stream())
+        if stream != self._stream or held:
+            for t in (self.table, *held):
+                t.record_stream(torch.cuda.current_stream())
         fn(stream)
 
 
@@ -240,6 +242,7 @@ class AdapterBank:
         self.max_rank = max(r8)
         k32, n32 = -(-self.k // 32) * 32, -(-self.n // 32) * 32
         with torch.cuda.device(self.device):
+            self._stream = torch.cuda.current_stream().cuda_stream
             self.data = torch.empty(sum(r * (k32 + n32) for r in r8) + self.SPARE, dtype=self.dtype, device=self.device)
             meta = torch.zeros(len(pairs), 3, dtype=torch.int64)
             off, st = 0, stream_ptr()
@@ -325,5 +328,6 @@ def lora_add(y, x, bank, plan, out=None):
     ws = torch.empty(n, dtype=torch.float32, device=dev) if n else None
     plan._launch(lambda stream: call(
         "td_lora_add", x.data_ptr(), ldx, y.data_ptr(), ldy, out.data_ptr(), ldo, dt_code(y.dtype), bank.k, bank.n, bank.data.data_ptr(),
-        bank.meta.data_ptr(), len(bank), bank.max_rank, plan.table.data_ptr(), plan._counts, None if ws is None else ws.data_ptr(), stream))
+        bank.meta.data_ptr(), len(bank), bank.max_rank, plan.table.data_ptr(), plan._counts, None if ws is None else ws.data_ptr(), stream),
+        *(() if _raw_stream(dev.index) == bank._stream else (bank.data, bank.meta)))
     return out

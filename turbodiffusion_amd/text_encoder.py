@@ -175,12 +175,16 @@ class Umt5Encoder:
         if self._distance_bias is None:
             tables = [self.pos] if self.shared_pos else [lay["pos"] for lay in self.layers]
             self._distance_bias = [relative_bias(t, self.max_dist) for t in tables]
+            torch.cuda.current_stream(self.device).synchronize()                                 # complete for every later stream
 
         def adapt(y, x, layer, target):     # in place
             bank = None if rows is None else adapters.banks[layer].get(target)
             return y if bank is None else lora_add(y, x, bank, rows, out=y)
 
-        x = F.embedding(torch.cat([p.to(self.device) for p in ids]), self.emb)                   # gather (plumbing)
+        flat = torch.cat([p.to(self.device) for p in ids])
+        if int(flat.min()) < 0 or int(flat.max()) >= self.emb.shape[0]:
+            raise ValueError(f"encode_packed: token ids must lie in [0, {self.emb.shape[0]})")
+        x = F.embedding(flat, self.emb)                                                          # gather (plumbing)
         for i, lay in enumerate(self.layers):
             h = K.t5_norm(x, lay["n1"], self.eps)
             qkv = adapt(K.gemm_bf16(h, lay["qkv"]), h, i, "qkv").view(-1, 3, H, c)
