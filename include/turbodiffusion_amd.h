@@ -529,11 +529,11 @@ int td_attn_packed(const void* q, const void* k, const void* v, void* o, const i
  * are read and not used.  max_rank: the largest rank8 (at most 256).
  * td_lora_plan (host only): lengths and adapter ids of the requests -> counts = {tiles with an adapter, tiles without, rows, rows
  * with an adapter, largest id + 1, rows per tile} and, with table != NULL, 4 (tiles with + without) + rows int32 words, which go to
- * the device unchanged.  td_lora_workspace: f32 elements of ws. */
+ * the device unchanged.  td_lora_workspace: f32 elements of ws (NULL when 0). */
 int td_lora_pack(const void* a, int64_t lda, const void* b, int64_t ldb, int rank, int64_t k, int64_t n, void* bank_a, void* bank_b,
                  td_stream_t stream);
 int td_lora_plan(const int64_t* lens, const int64_t* ids, int64_t nseq, int32_t* table, int64_t capacity, int64_t* counts);
-int td_lora_workspace(const int64_t* counts, int64_t k, int max_rank, int64_t* floats);
+int td_lora_workspace(const int64_t* counts, int64_t k, int64_t n, int max_rank, int64_t* floats);
 int td_lora_add(const void* x, int64_t ldx, const void* y, int64_t ldy, void* out, int64_t ldo, int dtype, int64_t k, int64_t n,
                 const void* bank, const void* adapters, int num_adapters, int max_rank, const int32_t* table, const int64_t* counts,
                 float* ws, td_stream_t stream);

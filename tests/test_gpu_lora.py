@@ -76,9 +76,21 @@ def test_lora_rows_ranks_and_sizes(dtype, k, n, case):
     assert torch.equal(y, o)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rows,k,n", [(1500, 1000, 1544), (1, 10240, 64), (70, 10248, 256), (300, 4104, 6152)])
+def test_lora_two_launches(dtype, rows, k, n):
+    """between one launch and many rows: K split over workgroups, tiles of 32 rows, small ranks"""
+    lens, ids = [rows // 3, rows - rows // 3], [1, 0]
+    y, x, pairs, scales = make(rows, k, n, [12, 64], dtype, seed=3)
+    bank, plan = ops.AdapterBank(pairs, scales), ops.AdapterPlan(lens, ids)
+    assert plan.workspace(k, n, 64) > 0
+    ref, tol = formula(y, x, pairs, scales, lens, ids)
+    check(ops.lora_add(y, x, bank, plan), ref, tol)
+
+
 @pytest.mark.parametrize("rank", [16, 100])
 def test_lora_many_rows(rank):
-    """enough tiles that every wave walks all of K"""
+    """enough rows for tiles of 256"""
     lens, ids = [20000, 13001], [1, 0]
     y, x, pairs, scales = make(sum(lens), 520, 264, [rank, 24], torch.bfloat16, seed=2)
     bank, plan = ops.AdapterBank(pairs, scales), ops.AdapterPlan(lens, ids)

@@ -138,16 +138,19 @@ def test_adapter_refusals():
 
 
 def test_adapter_workspace_of_every_plan():
-    """no rows with an adapter need no workspace; otherwise at least one fp32 part of every such row"""
-    for tiles, rows, tile in ((0, 0, 32), (1, 1, 32), (5, 150, 32), (32, 8192, 256), (600, 600 * 256, 256)):
+    """no rows with an adapter need no workspace, nor do calls small enough for one launch; otherwise at least one 16-bit part of
+    every such row"""
+    for tiles, rows, tile in ((0, 0, 32), (1, 1, 32), (5, 150, 32), (200, 6400, 32), (32, 8192, 256), (600, 600 * 256, 256)):
         c = (ctypes.c_int64 * 6)(tiles, 0, rows, rows, 1, tile)
         for k in (8, 64, 4096, 10240):
-            for rank in (8, 16, 24, 256):
-                out = ctypes.c_int64(-1)
-                L.call("td_lora_workspace", c, k, rank, ctypes.byref(out))
-                assert out.value == 0 if rows == 0 else out.value >= rows * rank // 2
+            for n in (8, 4096, 12288):
+                for rank in (8, 16, 24, 256):
+                    out = ctypes.c_int64(-1)
+                    L.call("td_lora_workspace", c, k, n, rank, ctypes.byref(out))
+                    few = tile == 32 and rank <= 64 and k <= 8192 and tiles * -(-n // 256) <= 256
+                    assert out.value == 0 if rows == 0 or few else out.value >= rows * rank // 2
     with pytest.raises(L.TurboDiffusionAMDError):
-        L.call("td_lora_workspace", c, 64, 257, ctypes.byref(out))
+        L.call("td_lora_workspace", c, 64, 64, 257, ctypes.byref(out))
 
 
 @pytest.mark.parametrize("bidirectional", [True, False])

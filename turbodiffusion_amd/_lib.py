@@ -97,7 +97,7 @@ SIGNATURES = {
     "td_attn_packed": [_vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _f32, _i32, _vp, _i32, _vp, _vp, _vp, _vp],
     "td_lora_plan": [_vp, _vp, _i64, _vp, _i64, _vp],
     "td_lora_pack": [_vp, _i64, _vp, _i64, _i32, _i64, _i64, _vp, _vp, _vp],
-    "td_lora_workspace": [_vp, _i64, _i32, _vp],
+    "td_lora_workspace": [_vp, _i64, _i64, _i32, _vp],
     "td_lora_add": [_vp, _i64, _vp, _i64, _vp, _i64, _i32, _i64, _i64, _vp, _vp, _i32, _i32, _vp, _vp, _vp, _vp],
     "td_sla_linear_out_fm": [_vp, _i32, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i32, _i64, _i32, _i32, _vp],
 }

@@ -279,14 +279,14 @@ class AdapterPlan(_Plan):
         self._ws = {}
         self._upload(host, device)
 
-    def workspace(self, k, max_rank):
+    def workspace(self, k, n, max_rank):
         """f32 elements a call needs"""
-        n = self._ws.get((k, max_rank))
-        if n is None:
+        floats = self._ws.get((k, n, max_rank))
+        if floats is None:
             out = ctypes.c_int64()
-            L.call("td_lora_workspace", self._counts, k, max_rank, ctypes.byref(out))
-            n = self._ws[(k, max_rank)] = out.value
-        return n
+            L.call("td_lora_workspace", self._counts, k, n, max_rank, ctypes.byref(out))
+            floats = self._ws[(k, n, max_rank)] = out.value
+        return floats
 
 
 def _rows(t, rows, cols, what):
@@ -324,8 +324,8 @@ def lora_add(y, x, bank, plan, out=None):
             raise ValueError("lora_add: out overlaps an input (out=y alone may)")
     if plan.rows == 0:
         return out
-    n = plan.workspace(bank.k, bank.max_rank)
-    ws = torch.empty(n, dtype=torch.float32, device=dev) if n else None
+    floats = plan.workspace(bank.k, bank.n, bank.max_rank)
+    ws = torch.empty(floats, dtype=torch.float32, device=dev) if floats else None
     plan._launch(lambda stream: call(
         "td_lora_add", x.data_ptr(), ldx, y.data_ptr(), ldy, out.data_ptr(), ldo, dt_code(y.dtype), bank.k, bank.n, bank.data.data_ptr(),
         bank.meta.data_ptr(), len(bank), bank.max_rank, plan.table.data_ptr(), plan._counts, None if ws is None else ws.data_ptr(), stream),
