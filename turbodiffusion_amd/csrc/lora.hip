@@ -314,12 +314,13 @@ __global__ __launch_bounds__(256, RJ <= 8 ? 2 : 1) void lora_expand_kernel(const
 #undef LR_EXPAND
 }
 
-// Both steps in one launch, for a few rows: every workgroup of 256 columns forms the tile's S itself, its 16 waves splitting K,
-// and the first four expand.  A_i is read once per workgroup (from L2), which pays while there are few of them: one row, K = N =
-// 4096, rank 16: one launch of 4.9 us instead of 3.5 + 3.4 us and a second launch on the host (3 us).
+// Both steps in one launch, for a few rows: every workgroup of 256 columns forms the tile's S itself, its 8 waves splitting K, and
+// the first four expand.  A_i is read once per workgroup (from L2), which pays while there are few of them.  One row, K = N =
+// 4096, rank 16: 8.8 us a call instead of 12.2 (a second launch costs the host 3 us); replayed from a graph, where launches are
+// cheap, 6.4 instead of 5.9.
 template <int DT, int RJ>
-__global__ __launch_bounds__(1024) void lora_few_kernel(const LoraParams p) {
-  constexpr int RS = 16 * RJ, KK = (RJ + 1) / 2, W = 16;
+__global__ __launch_bounds__(512) void lora_few_kernel(const LoraParams p) {
+  constexpr int RS = 16 * RJ, KK = (RJ + 1) / 2, W = 8;
   const int lane = threadIdx.x & 63, l16 = lane & 15, lq = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const LoraTile t = p.tiles[blockIdx.x];
@@ -331,8 +332,8 @@ __global__ __launch_bounds__(1024) void lora_few_kernel(const LoraParams p) {
   __syncthreads();
   if (t.adapter < 0) {            // rows without an adapter: copy
     const int64_t c = (int64_t)blockIdx.y * 256 + 8 * (lane & 31);
-    const int r = 2 * wave + (lane >> 5);
-    if (c < p.N && r < t.rows) *reinterpret_cast<uint4*>(p.out + prow[r] * p.ldo + c) = *reinterpret_cast<const uint4*>(p.y + prow[r] * p.ldy + c);
+    if (c < p.N)
+      for (int r = 2 * wave + (lane >> 5); r < t.rows; r += 2 * W) *reinterpret_cast<uint4*>(p.out + prow[r] * p.ldo + c) = *reinterpret_cast<const uint4*>(p.y + prow[r] * p.ldy + c);
     return;
   }
   const LoraAdapter ad = p.adapters[t.adapter];
@@ -429,7 +430,7 @@ extern "C" int td_lora_plan(const int64_t* lens, const int64_t* ids, int64_t nse
 
 struct LoraShape { int rj, splits, chunks; bool few; };
 // 256 CUs: K is split over workgroups until there are about 256 of them (at most 8 parts, 512 of K each or more)
-// few: one launch (lora_few_kernel) while its workgroups all run at once and a wave has at most 8 chunks of K to walk
+// few: one launch (lora_few_kernel) while its workgroups all run at once and a wave has at most 8 chunks of K (0.5 us each) to walk
 static LoraShape lora_shape(const int64_t* counts, int64_t k, int64_t n, int max_rank) {
   LoraShape s;
   s.rj = max_rank <= 16 ? 1 : max_rank <= 32 ? 2 : max_rank <= 64 ? 4 : max_rank <= 128 ? 8 : 16;
@@ -437,7 +438,7 @@ static LoraShape lora_shape(const int64_t* counts, int64_t k, int64_t n, int max
   const int64_t want = counts[5] == LR_WIDE ? 1 : std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(8, td_cdiv(256, tiles)), nch / 8));
   s.chunks = (int)td_cdiv(nch, want);
   s.splits = (int)td_cdiv(nch, s.chunks);
-  s.few = counts[5] == LR_NARROW && s.rj <= 4 && k <= 8192 && (counts[0] + counts[1]) * td_cdiv(n, 256) <= 256;
+  s.few = counts[5] == LR_NARROW && s.rj <= 4 && k <= 4096 && (counts[0] + counts[1]) * td_cdiv(n, 256) <= 256;
   return s;
 }
 
@@ -501,9 +502,9 @@ extern "C" int td_lora_add(const void* x, int64_t ldx, const void* y, int64_t ld
   }
   if (sh.few) {
 #define LR_FEW(DT_)                                                       \
-    if (sh.rj == 1) lora_few_kernel<DT_, 1><<<ge, 1024, 0, st>>>(p);        \
-    else if (sh.rj == 2) lora_few_kernel<DT_, 2><<<ge, 1024, 0, st>>>(p);   \
-    else lora_few_kernel<DT_, 4><<<ge, 1024, 0, st>>>(p);
+    if (sh.rj == 1) lora_few_kernel<DT_, 1><<<ge, 512, 0, st>>>(p);        \
+    else if (sh.rj == 2) lora_few_kernel<DT_, 2><<<ge, 512, 0, st>>>(p);   \
+    else lora_few_kernel<DT_, 4><<<ge, 512, 0, st>>>(p);
     if (dtype == TD_BF16) { LR_FEW(TD_BF16) } else { LR_FEW(TD_F16) }
 #undef LR_FEW
     TD_CHECK_LAUNCH();
