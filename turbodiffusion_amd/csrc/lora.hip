@@ -5,13 +5,18 @@
 // x [rows, K], y / out [rows, N], A_i [rank_i, K], B_i [N, rank_i], 16-bit.  The rows are taken adapter by adapter (a permutation
 // made by the plan), in tiles of one adapter, so an adapter is read for all of its rows at once however its requests lie.
 //
-//   shrink   S = A_i x by MFMA 16x16x32, fp32.  x streams from memory straight into fragments.  A workgroup takes 32 rows, its
-//            four waves split K; with few rows K is split over workgroups too and expand adds the fp32 parts in order.
+//   shrink   S = A_i x by MFMA 16x16x32, fp32.  A workgroup takes 32 rows, its four waves split K; with few rows K is split over
+//            workgroups too and expand adds the fp32 parts in order.
 //   expand   out = y + B_i (s_i S): S is scaled in fp32 and rounded once to the operands' type (half a step of the update only:
 //            it stays below the rounding of the output wherever the update is not many times larger than the output itself).
 //            A wave keeps B_i of 64 columns in registers and walks the tile's rows, 16 at a time.
-// The bank holds A and B in fragment order (td_lora_pack): every load of them is a contiguous kilobyte, ranks are padded to 8
-// only.  Memory-bound: y and out dominate, then x; 2 rank flops per byte of them.
+// The bank holds A and B in fragment order (td_lora_pack): every load of them is a contiguous kilobyte, ranks are padded to 8 only.
+//
+// What bounds it: memory; y and out dominate, then x, at 2 rank flops per byte.  MFMA fragments want 64 bytes from each of 16 rows;
+// memory wants whole 128-byte lines, so x, y and out pass through LDS on their way (50 960 rows, 1536 -> 8960, ranks 128 and 64:
+// expand 506 -> 419 us, 4.4 TB/s, shrink 85 -> 65 us; 32 760 rows, 5120 -> 5120, rank 32: 162 -> 122 us, 5.5 TB/s, and 103 -> 98, where
+// shrink also waits for the previous pass's writes).  A large copy moves 4.9 TB/s.  With B_i read again for every 64 rows expand
+// took 639 us; non-temporal loads and stores cost 2 to 15 %.
 #include "td_common.h"
 #include <algorithm>
 #include <new>
