@@ -6,7 +6,7 @@ fp32 sum over the ranks, the scale and y by (rank + 4) 2^-24 of the sum of what 
 import pytest
 import torch
 
-from turbodiffusion_amd import ops
+from turbodiffusion_amd import ops, packed
 from turbodiffusion_amd._lib import TurboDiffusionAMDError
 
 pytestmark = pytest.mark.gpu
@@ -83,7 +83,7 @@ def test_lora_two_launches(dtype, rows, k, n):
     lens, ids = [rows // 3, rows - rows // 3], [1, 0]
     y, x, pairs, scales = make(rows, k, n, [12, 64], dtype, seed=3)
     bank, plan = ops.AdapterBank(pairs, scales), ops.AdapterPlan(lens, ids)
-    assert plan.workspace(k, n, 64) > 0
+    assert packed._lora_layout(y, x, bank, plan, None)[3] > 0
     ref, tol = formula(y, x, pairs, scales, lens, ids)
     check(ops.lora_add(y, x, bank, plan), ref, tol)
 

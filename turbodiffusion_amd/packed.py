@@ -40,6 +40,7 @@ class _Plan:
     """A host-made table of int32 records on ``device``."""
 
     def _upload(self, host, device):
+        self._admitted = {}        # layouts (shapes, strides, types) that passed the checks -> what the C entry takes for them
         self.device = torch.device(device)
         if self.device.type != "cuda":
             raise ValueError(f"{type(self).__name__}: the operators run on a GPU, got device {device!r}")
@@ -48,6 +49,12 @@ class _Plan:
         with torch.cuda.device(self.device):
             self._stream = torch.cuda.current_stream().cuda_stream
             self.table = host.to(self.device)          # synchronous: complete for every stream
+
+    def _admit(self, key, value):
+        if len(self._admitted) >= 256:
+            self._admitted.clear()
+        self._admitted[key] = value
+        return value
 
     def _launch(self, fn, *held):
         """``fn(stream)`` with the plan's device current; the table and ``held`` (what else the framework keeps for the caller) stay
@@ -108,9 +115,12 @@ class AttentionPlan(_Plan):
         host = torch.zeros(max(1, n), 8, dtype=torch.int32)
         L.call("td_attn_packed_plan", *args, ptr(host), n, self._counts)
         self.tokens, self.tokens_k = self._counts[4], self._counts[5]
-        self._strides = {}                             # stride tuples seen, as C arrays
         self.ws_floats = self._counts[3] * self.kv_heads * (self.head_dim + 2)
         self._upload(host, device)
+
+
+def _layout(t):
+    return None if t is None else (t.shape, t.stride(), t.dtype)
 
 
 def _packed_strides(t, tokens, heads, head_dim, what):
@@ -120,6 +130,35 @@ def _packed_strides(t, tokens, heads, head_dim, what):
     if ds != 1:
         raise ValueError(f"packed_attention: the last dimension of {what} must be contiguous")
     return (ts if tokens > 1 else 0), (hs if heads > 1 else 0)   # a stride that no second element uses is arbitrary
+
+
+def _attention_layout(plan, q, k, v, scale, bias, out):
+    """The checks that depend on shapes, strides, types and scale alone -> (strides as a C array, dtype code, scale, bias range)"""
+    H, Hkv, D, dt = plan.heads, plan.kv_heads, plan.head_dim, q.dtype
+    if k.dtype != dt or v.dtype != dt or (dt != torch.bfloat16 and dt != torch.float16):
+        raise TypeError(f"packed_attention: q, k, v must all be bf16 or all f16 (got {q.dtype}, {k.dtype}, {v.dtype})")
+    strides = (*_packed_strides(q, plan.tokens, H, D, "q"), *_packed_strides(k, plan.tokens_k, Hkv, D, "k"),
+               *_packed_strides(v, plan.tokens_k, Hkv, D, "v"))
+    R = 0
+    if bias is not None:
+        _f32c(bias, "bias")
+        if bias.dim() != 2 or bias.shape[0] != H or bias.shape[1] % 2 == 0:
+            raise ValueError(f"packed_attention: bias is {tuple(bias.shape)}, wanted [{H}, 2 R + 1]")
+        R = bias.shape[1] // 2
+    scale = 1.0 / math.sqrt(D) if scale is None else scale
+    if not 0.0 < scale < math.inf:
+        raise ValueError(f"packed_attention: scale must be positive and finite, got {scale}")
+    if out is None:
+        strides += (H * D, D)
+    else:
+        if out.dtype != dt:
+            raise TypeError(f"packed_attention: out is {out.dtype}, the inputs {dt}")
+        ts, hs = _packed_strides(out, plan.tokens, H, D, "out")
+        if not ((H == 1 or hs >= D) and (plan.tokens <= 1 or ts >= (H - 1) * hs + D)
+                or (plan.tokens <= 1 or ts >= D) and (H == 1 or hs >= (plan.tokens - 1) * ts + D)):
+            raise ValueError("packed_attention: out overlaps itself")
+        strides += (ts, hs)
+    return _i64_array(strides), dt_code(dt), scale, R
 
 
 def packed_attention(q, k, v, plan, scale=None, bias=None, out=None):
@@ -133,44 +172,22 @@ def packed_attention(q, k, v, plan, scale=None, bias=None, out=None):
     the inputs' type for the second product.  A masked key weighs exactly 0, so its VALUE must be finite like any other.
     ``out``: written instead of a new tensor; it may not overlap the inputs.  Any stream, capturable; the plan must outlive a
     captured graph."""
-    H, Hkv, D = plan.heads, plan.kv_heads, plan.head_dim
-    dev, dt = plan.device, q.dtype
-    _check_tensors("packed_attention", dev, q, k, v, bias, out)
-    if k.dtype != dt or v.dtype != dt or (dt != torch.bfloat16 and dt != torch.float16):
-        raise TypeError(f"packed_attention: q, k, v must all be bf16 or all f16 (got {q.dtype}, {k.dtype}, {v.dtype})")
-    strides = (*_packed_strides(q, plan.tokens, H, D, "q"), *_packed_strides(k, plan.tokens_k, Hkv, D, "k"),
-               *_packed_strides(v, plan.tokens_k, Hkv, D, "v"))
-    R = 0
-    if bias is not None:
-        _f32c(bias, "bias")
-        if bias.dim() != 2 or bias.shape[0] != H or bias.shape[1] % 2 == 0:
-            raise ValueError(f"packed_attention: bias is {tuple(bias.shape)}, wanted [{H}, 2 R + 1]")
-        R = bias.shape[1] // 2
-    scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
-    if not 0.0 < scale < math.inf:
-        raise ValueError(f"packed_attention: scale must be positive and finite, got {scale}")
+    _check_tensors("packed_attention", plan.device, q, k, v, bias, out)
+    if scale is not None and type(scale) is not float:
+        scale = float(scale)
+    key = (_layout(q), _layout(k), _layout(v), scale, _layout(bias), _layout(out))
+    strides, dt, scale_, R = plan._admitted.get(key) or plan._admit(key, _attention_layout(plan, q, k, v, scale, bias, out))
     if out is None:
-        out = torch.empty((plan.tokens, H, D), dtype=dt, device=dev)
-        strides += (H * D, D)
-    else:
-        if out.dtype != dt:
-            raise TypeError(f"packed_attention: out is {out.dtype}, the inputs {dt}")
-        ts, hs = _packed_strides(out, plan.tokens, H, D, "out")
-        if not ((H == 1 or hs >= D) and (plan.tokens <= 1 or ts >= (H - 1) * hs + D)
-                or (plan.tokens <= 1 or ts >= D) and (H == 1 or hs >= (plan.tokens - 1) * ts + D)):
-            raise ValueError("packed_attention: out overlaps itself")
-        if any(_overlap(out, t) for t in (q, k, v)):
-            raise ValueError("packed_attention: out overlaps an input")
-        strides += (ts, hs)
+        out = q.new_empty((plan.tokens, plan.heads, plan.head_dim))
+    elif any(_overlap(out, t) for t in (q, k, v, bias) if t is not None):
+        raise ValueError("packed_attention: out overlaps an input")
     if plan.tokens == 0:
         return out
-    packed_strides = plan._strides.get(strides)
-    if packed_strides is None:
-        packed_strides = plan._strides[strides] = _i64_array(strides)
-    ws = torch.empty(plan.ws_floats, dtype=torch.float32, device=dev) if plan.ws_floats else None
+    ws = q.new_empty(plan.ws_floats, dtype=torch.float32) if plan.ws_floats else None
     plan._launch(lambda stream: call(
-        "td_attn_packed", q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), packed_strides, dt_code(dt), H, Hkv, D, scale, plan.causal,
-        None if bias is None else bias.data_ptr(), R, plan.table.data_ptr(), plan._counts, None if ws is None else ws.data_ptr(), stream))
+        "td_attn_packed", q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), strides, dt, plan.heads, plan.kv_heads, plan.head_dim, scale_,
+        plan.causal, None if bias is None else bias.data_ptr(), R, plan.table.data_ptr(), plan._counts, None if ws is None else ws.data_ptr(),
+        stream))
     return out
 
 
@@ -240,6 +257,7 @@ class AdapterBank:
         self.ranks = [a.shape[0] for a, _ in pairs]
         r8 = [-(-r // 8) * 8 for r in self.ranks]
         self.max_rank = max(r8)
+        self.layout = (self.dtype, self.k, self.n, len(pairs), self.max_rank)
         k32, n32 = -(-self.k // 32) * 32, -(-self.n // 32) * 32
         with torch.cuda.device(self.device):
             self._stream = torch.cuda.current_stream().cuda_stream
@@ -276,17 +294,7 @@ class AdapterPlan(_Plan):
         host = torch.zeros(max(1, n), dtype=torch.int32)
         L.call("td_lora_plan", *args, ptr(host), n, self._counts)
         self.rows = self._counts[2]
-        self._ws = {}
         self._upload(host, device)
-
-    def workspace(self, k, n, max_rank):
-        """f32 elements a call needs"""
-        floats = self._ws.get((k, n, max_rank))
-        if floats is None:
-            out = ctypes.c_int64()
-            L.call("td_lora_workspace", self._counts, k, n, max_rank, ctypes.byref(out))
-            floats = self._ws[(k, n, max_rank)] = out.value
-        return floats
 
 
 def _rows(t, rows, cols, what):
@@ -298,6 +306,24 @@ def _rows(t, rows, cols, what):
     return ld if rows > 1 else 0
 
 
+def _lora_layout(y, x, bank, plan, out):
+    """The checks that depend on shapes, strides, types and the bank's sizes alone -> (row strides of y, x, out; workspace; dtype code)"""
+    if x.dtype != bank.dtype or y.dtype != bank.dtype:
+        raise TypeError(f"lora_add: x is {x.dtype}, y {y.dtype}, the adapters {bank.dtype}")
+    if plan._counts[4] > len(bank):
+        raise ValueError(f"lora_add: the plan names adapter {plan._counts[4] - 1}, the bank holds {len(bank)}")
+    ldx, ldy, ldo = _rows(x, plan.rows, bank.k, "x"), _rows(y, plan.rows, bank.n, "y"), bank.n
+    if out is not None:
+        if out.dtype != y.dtype:
+            raise TypeError(f"lora_add: out is {out.dtype}, y {y.dtype}")
+        ldo = _rows(out, plan.rows, bank.n, "out")
+        if plan.rows > 1 and ldo < bank.n:
+            raise ValueError("lora_add: out overlaps itself")
+    floats = ctypes.c_int64()
+    L.call("td_lora_workspace", plan._counts, bank.k, bank.n, bank.max_rank, ctypes.byref(floats))
+    return ldy, ldx, ldo, floats.value, dt_code(y.dtype)
+
+
 def lora_add(y, x, bank, plan, out=None):
     """y [rows, n] + the adapters' updates of x [rows, k] (row stride: any multiple of 8 elements) -> [rows, n]: row r of a request
     with adapter i becomes y[r] + scale_i * (x[r] A_i^T) B_i^T, one without stays y[r].  ``y`` is the output of the projection that
@@ -306,28 +332,17 @@ def lora_add(y, x, bank, plan, out=None):
     is added in fp32 and rounded with the result.  Any stream, capturable; bank and plan must outlive a captured graph."""
     dev = plan.device
     _check_tensors("lora_add", dev, y, x, out, bank.data)
-    if x.dtype != bank.dtype or y.dtype != bank.dtype:
-        raise TypeError(f"lora_add: x is {x.dtype}, y {y.dtype}, the adapters {bank.dtype}")
-    if plan._counts[4] > len(bank):
-        raise ValueError(f"lora_add: the plan names adapter {plan._counts[4] - 1}, the bank holds {len(bank)}")
-    ldx, ldy = _rows(x, plan.rows, bank.k, "x"), _rows(y, plan.rows, bank.n, "y")
+    key = (_layout(y), _layout(x), _layout(out), bank.layout)
+    ldy, ldx, ldo, floats, dt = plan._admitted.get(key) or plan._admit(key, _lora_layout(y, x, bank, plan, out))
     if out is None:
-        out = torch.empty((plan.rows, bank.n), dtype=y.dtype, device=dev)
-        ldo = bank.n
-    else:
-        if out.dtype != y.dtype:
-            raise TypeError(f"lora_add: out is {out.dtype}, y {y.dtype}")
-        ldo = _rows(out, plan.rows, bank.n, "out")
-        if plan.rows > 1 and ldo < bank.n:
-            raise ValueError("lora_add: out overlaps itself")
-        if _overlap(out, x) or (_overlap(out, y) and (out.data_ptr() != y.data_ptr() or ldo != ldy)):
-            raise ValueError("lora_add: out overlaps an input (out=y alone may)")
+        out = y.new_empty((plan.rows, bank.n))
+    elif _overlap(out, x) or (_overlap(out, y) and (out.data_ptr() != y.data_ptr() or ldo != ldy)):
+        raise ValueError("lora_add: out overlaps an input (out=y alone may)")
     if plan.rows == 0:
         return out
-    floats = plan.workspace(bank.k, bank.n, bank.max_rank)
-    ws = torch.empty(floats, dtype=torch.float32, device=dev) if floats else None
+    ws = y.new_empty(floats, dtype=torch.float32) if floats else None
     plan._launch(lambda stream: call(
-        "td_lora_add", x.data_ptr(), ldx, y.data_ptr(), ldy, out.data_ptr(), ldo, dt_code(y.dtype), bank.k, bank.n, bank.data.data_ptr(),
+        "td_lora_add", x.data_ptr(), ldx, y.data_ptr(), ldy, out.data_ptr(), ldo, dt, bank.k, bank.n, bank.data.data_ptr(),
         bank.meta.data_ptr(), len(bank), bank.max_rank, plan.table.data_ptr(), plan._counts, None if ws is None else ws.data_ptr(), stream),
         *(() if _raw_stream(dev.index) == bank._stream else (bank.data, bank.meta)))
     return out
