@@ -34,7 +34,8 @@ typedef __attribute__((address_space(3))) ap_v4s* ap_trptr_t;
 #define AP_FEW 32          // rows of a few item
 #define AP_FEW_KEYS 128    // ... of sequences with more keys than this; with fewer the four waves would not all have a tile
 #define AP_PAD 96          // the bias table repeats its ends: distances within a key tile of the range need no clamp
-#define AP_TAU 8.0f        // the reference maximum moves only when exceeded by 2^8: P <= 256 fits f16 / bf16 and the fp32 sum
+#define AP_TAU 8.0f        // a row's reference moves when a score exceeds it by 8 (a weight of 2^8),
+#define AP_LOOK 4096.0f    // looked for when the 16 (32) weights of a lane in a tile add up to more than this
 
 // One workgroup's work per key head: `rows` rows from head `head0` of query token `token`, which stands at position `pos` of its
 // sequence, over keys [key0, key1) of the sequence whose first key token is k_begin.  slot: row in the partial buffer, -1 = writes o
@@ -129,27 +130,27 @@ __device__ __forceinline__ void ap_load_bias(const ApParams& p, int kvh, int bn,
     }
 }
 
-// scores of 32 N keys from kb, registers s[b][r] = key kb + 32 b + 16 (r >> 3) + 8 half + (r & 7) of this lane's row: bias, mask, maximum
+// Scores of 32 N keys from kb, registers s[b][r] = key kb + 32 b + 16 (r >> 3) + 8 half + (r & 7) of this lane's row: bias and mask.
+// Afterwards the score in the exp2 domain is mul * s + base.
 struct ApScore {
   float c; int R; const float* lb;          // lb[key - position]
   float far_past, far_next;
   int pos, kmax, half;                      // this row's position and end
   int wfirst, wlast, wmin, wmax;            // the wave's first and last position, smallest and largest end
-  template <bool BIAS, int N> __device__ __forceinline__ float finish(v16f (&s)[N], int kb) const {
+  template <bool BIAS, int N> __device__ __forceinline__ void finish(v16f (&s)[N], int kb, float& mul, float& base) const {
+    mul = c;
+    base = 0.f;
     if constexpr (BIAS) {
       const bool next = kb - wlast >= R, past = kb + 32 * N - 1 - wfirst <= -R;
       if (next || past) {                                     // all of it lies beyond the range: one value a row
-        const float far = next ? far_next : far_past;
-#pragma unroll
-        for (int b = 0; b < N; ++b)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) s[b][r] = fmaf(s[b][r], c, far);
+        base = next ? far_next : far_past;
       } else {                                                // |key - position| < R + 96 everywhere
         const float* d = lb + (kb + 8 * half - pos);
 #pragma unroll
         for (int b = 0; b < N; ++b)
 #pragma unroll
           for (int r = 0; r < 16; ++r) s[b][r] = fmaf(s[b][r], c, d[32 * b + 16 * (r >> 3) + (r & 7)]);
+        mul = 1.f;
       }
     }
     if (kb + 32 * N > wmin) {
@@ -160,13 +161,14 @@ struct ApScore {
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[b][r] = 32 * b + 16 * (r >> 3) + (r & 7) < lim ? s[b][r] : -INFINITY;
     }
+  }
+  template <int N> __device__ __forceinline__ float maximum(const v16f (&s)[N], float mul, float base) const {   // of the row
     float mx = s[0][0];
 #pragma unroll
     for (int b = 0; b < N; ++b)
 #pragma unroll
       for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[b][r]);
-    mx = ap_other_half(mx, true);
-    return BIAS ? mx : mx * c;
+    return fmaf(ap_other_half(mx, true), mul, base);
   }
 };
 
@@ -191,12 +193,19 @@ __device__ __forceinline__ ApScore ap_score(const ApParams& p, const ApItem& it,
   return sc;
 }
 
-// One key tile of 32 NB keys from kt for a wave's 32 rows: scores, running maximum and sum, P V.  FIRST: nothing to add to or to
-// rescale, acc, m and l come in undefined.
+// Running state of a wave's rows: weights are exp2(score - ref).  ref is a row's maximum when it was last looked at, not its
+// running maximum: the maximum of a tile is taken only when a lane's weights of it add up to more than 2^12, which one weight of
+// more than 2^8 must have caused (of 60 vector instructions a block 24 less).  Weights up to 2^12 fit f16, bf16 and the fp32 sums.
+struct ApState {
+  float m, ref, l;          // m: ref, or -infinity while the row has seen nothing
+  bool unseen;              // a row of the wave has
+};
+
+// One key tile of 32 NB keys from kt for a wave's 32 rows: scores, weights and their sum, P V.  FIRST: nothing to add to or to
+// rescale, acc and st come in undefined.
 template <int DT, int D, int NB, bool BIAS, bool FIRST>
 __device__ __forceinline__ void ap_tile(const ApParams& p, const ApScore& score, const char* sk, const char* sv, uint32_t krow, uint32_t kxor,
-                                        uint32_t vrow, uint32_t vxor, int kt, const v4i (&qf)[D / 16], v16f (&acc)[D / 32], float& m, float& mref,
-                                        float& l) {
+                                        uint32_t vrow, uint32_t vxor, int kt, const v4i (&qf)[D / 16], v16f (&acc)[D / 32], ApState& st) {
   constexpr int ROWB = 2 * D, KK = D / 16, DB = D / 32;
   v16f s[NB];
 #pragma unroll
@@ -210,32 +219,50 @@ __device__ __forceinline__ void ap_tile(const ApParams& p, const ApScore& score,
       const v4i kf = *reinterpret_cast<const v4i*>(sk + b * 32 * ROWB + krow + (kxor ^ (kk << 5)));
       s[b] = ap_mma<DT>::run(kf, qf[kk], s[b]);
     }
-  const float mx = score.template finish<BIAS>(s, kt);
-  if constexpr (FIRST) {
-    m = mx;
-    mref = mx == -INFINITY ? 0.f : mx;
-    l = 0.f;
-  } else if (__any(mx > m + AP_TAU)) {   // a row that does not exceed its reference keeps it: its bits do not depend on its neighbours
-    const float mn = mx > m + AP_TAU ? mx : m;
-    mref = mn == -INFINITY ? 0.f : mn;
-    const float alpha = __builtin_amdgcn_exp2f(m - mref);
-    m = mn;
-    l *= alpha;
-#pragma unroll
-    for (int d = 0; d < DB; ++d)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) acc[d][r] *= alpha;
-  }
+  float mul, base;
+  score.template finish<BIAS>(s, kt, mul, base);
   uint32_t pk[NB][8];
+  auto weights = [&]() {
+    const float off = base - st.ref;
+    float sum = 0.f;
 #pragma unroll
-  for (int b = 0; b < NB; ++b)
+    for (int b = 0; b < NB; ++b)
 #pragma unroll
-    for (int r = 0; r < 16; r += 2) {
-      const float e0 = __builtin_amdgcn_exp2f(BIAS ? s[b][r] - mref : fmaf(s[b][r], p.c, -mref));
-      const float e1 = __builtin_amdgcn_exp2f(BIAS ? s[b][r + 1] - mref : fmaf(s[b][r + 1], p.c, -mref));
-      l += e0 + e1;
-      pk[b][r >> 1] = pack2<DT>(e0, e1);
+      for (int r = 0; r < 16; r += 2) {
+        const float e0 = __builtin_amdgcn_exp2f(fmaf(s[b][r], mul, off)), e1 = __builtin_amdgcn_exp2f(fmaf(s[b][r + 1], mul, off));
+        sum += e0 + e1;
+        pk[b][r >> 1] = pack2<DT>(e0, e1);
+      }
+    return sum;
+  };
+  if constexpr (FIRST) {
+    st.m = score.maximum(s, mul, base);
+    st.ref = st.m == -INFINITY ? 0.f : st.m;
+    st.l = weights();
+    st.unseen = __any(st.m == -INFINITY);
+  } else {
+    float sum = 0.f;
+    bool look = st.unseen;
+    if (!look) {
+      sum = weights();
+      look = __any(sum > AP_LOOK);
     }
+    if (look) {                       // a row that does not exceed its reference keeps it: its bits do not depend on its neighbours
+      const float mx = score.maximum(s, mul, base);
+      const float mn = mx > st.m + AP_TAU ? mx : st.m;
+      st.ref = mn == -INFINITY ? 0.f : mn;
+      const float alpha = __builtin_amdgcn_exp2f(st.m - st.ref);
+      st.m = mn;
+      st.l *= alpha;
+#pragma unroll
+      for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[d][r] *= alpha;
+      sum = weights();
+      st.unseen = __any(st.m == -INFINITY);
+    }
+    st.l += sum;
+  }
 #pragma unroll
   for (int t = 0; t < 2 * NB; ++t) {
     const uint32_t* w = &pk[t >> 1][4 * (t & 1)];
@@ -350,18 +377,18 @@ __global__ __launch_bounds__(256, D == 128 ? 3 : 4) void attn_packed_tile_kernel
   const uint32_t vxor = ap_vx<D>(vkey) << 4;                                    // a multiple of 64: moves whole 32-d blocks
 
   v16f acc[DB];
-  float m, mref, l;
+  ApState st;
   auto tile = [&](auto first, int buf) {
     if (kt + BK < kend) fetch(kt + BK, buf ^ 1);
     if (kt < wend)
-      ap_tile<DT, D, 1, BIAS, decltype(first)::value>(p, score, smem + buf * STAGE, smem + buf * STAGE + TILE, krow, kxor, vrow, vxor, kt, qf, acc, m, mref, l);
+      ap_tile<DT, D, 1, BIAS, decltype(first)::value>(p, score, smem + buf * STAGE, smem + buf * STAGE + TILE, krow, kxor, vrow, vxor, kt, qf, acc, st);
     // this tile's reads have returned and the next tile has landed
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
     __syncthreads();
     kt += BK;
   };
   if (kt >= wend) {                 // rows that see nothing
-    m = -INFINITY; l = 0.f;
+    st.m = -INFINITY; st.l = 0.f;
 #pragma unroll
     for (int d = 0; d < DB; ++d)
 #pragma unroll
@@ -370,7 +397,7 @@ __global__ __launch_bounds__(256, D == 128 ? 3 : 4) void attn_packed_tile_kernel
   if (kt < kend) tile(std::true_type{}, 0);
   for (int buf = 1; kt < kend; buf ^= 1) tile(std::false_type{}, buf);
   if (x0 >= it.rows) return;        // no barrier behind this
-  l = ap_other_half(l, false);
+  const float l = ap_other_half(st.l, false);
 
   // ---- results.  acc[d][r] is d = 32 d + 8 (r >> 2) + 4 half + (r & 3) of this lane's row ----
   const int x = x0 + (lane & 31);
@@ -382,7 +409,7 @@ __global__ __launch_bounds__(256, D == 128 ? 3 : 4) void attn_packed_tile_kernel
 #pragma unroll
       for (int r = 0; r < 16; r += 4)
         *reinterpret_cast<float4*>(p.po + pr * D + 32 * d + 2 * r + 4 * half) = make_float4(acc[d][r], acc[d][r + 1], acc[d][r + 2], acc[d][r + 3]);
-    if (half == 0) { p.pml[pr * 2] = m; p.pml[pr * 2 + 1] = l; }
+    if (half == 0) { p.pml[pr * 2] = st.m; p.pml[pr * 2 + 1] = l; }
     return;
   }
   // through the wave's own 32 rows of LDS (every wave is done with the stages): whole rows go out
@@ -482,18 +509,18 @@ __global__ __launch_bounds__(256, 1) void attn_packed_few_kernel(const ApParams 
   for (int d = 0; d < DB; ++d)
 #pragma unroll
     for (int r = 0; r < 16; ++r) acc[d][r] = 0.f;
-  float m = -INFINITY, mref = 0.f, l = 0.f;
+  ApState st = {-INFINITY, 0.f, 0.f, true};
   int kt = it.key0 + wave * BK;
   if (kt < kend) fetch(kt, 0);
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   for (int buf = 0; kt < kend; kt += 4 * BK, buf ^= 1) {
     if (kt + 4 * BK < kend) fetch(kt + 4 * BK, buf ^ 1);
     const char* sk = mystage + buf * STAGE;
-    ap_tile<DT, D, NB, BIAS, false>(p, score, sk, sk + TILE, krow, kxor, vrow, vxor, kt, qf, acc, m, mref, l);
+    ap_tile<DT, D, NB, BIAS, false>(p, score, sk, sk + TILE, krow, kxor, vrow, vxor, kt, qf, acc, st);
     // this tile's reads have returned and the next tile has landed (the stages are this wave's own)
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
   }
-  l = ap_other_half(l, false);
+  const float l = ap_other_half(st.l, false), m = st.m;
 
   // acc[d][r] is d = 32 d + 8 (r >> 2) + 4 half + (r & 3) of this lane's row
   // ---- join the four waves through LDS ----
