@@ -55,6 +55,25 @@ def test_attention_plan_covers_every_visible_key_once(seed):
         assert len(set(rows)) == len(rows) and (not rows or max(rows) < ws_rows)
 
 
+@pytest.mark.parametrize("kv", [1, 3, 8, 12, 40, 300])
+def test_attention_plan_splits_long_pasts(kv):
+    """one new token over up to 2^30 keys: ranges of at least 256 keys (but a sequence's last), no shorter part before a longer one,
+    enough workgroups where there are keys for them; no split while no sequence has more than 1024 keys"""
+    for lk in ([1024] * 3, [1, 1024, 129], [1025], [32760], [8000] * 8, [32760, 1, 129, 20011, 777], [8000] * 256, [1 << 30], [1 << 29, 300, 1 << 28]):
+        t, (tiles, few, joins, ws_rows, tq, tk) = attention_table([1] * len(lk), lk, kv, kv, 1)
+        assert tiles == 0 and few >= len(lk)
+        items = sorted(t[:few])
+        for s, n in enumerate(lk):
+            parts = [x for x in items if x[0] == s]
+            assert [x[5] for x in parts] == [0] + [x[6] for x in parts[:-1]] and parts[-1][6] == n
+            assert all(x[6] - x[5] >= 256 and (x[6] - x[5]) % 128 == 0 for x in parts[:-1])
+            assert len(parts) == 1 or max(lk) > 1024
+        sizes = [x[6] - x[5] for x in t[:few]]
+        assert sizes == sorted(sizes, reverse=True)
+        if max(lk) > 1024 and sum(lk) * kv >= 256 * 1024:
+            assert few * kv >= 176
+
+
 def test_attention_plan_refusals():
     with pytest.raises(ValueError):
         ops.AttentionPlan([3, 4], [3], heads=2)

@@ -121,10 +121,11 @@ template <int D> struct ApRowWalk {
 };
 
 // exp2 domain; the type's lowest values as a finite low (a row of nothing else stays a uniform row)
+template <int THREADS>
 __device__ __forceinline__ void ap_load_bias(const ApParams& p, int kvh, int bn, float* lbias) {
   const float* b = p.bias + (int64_t)kvh * p.G * (2 * p.R + 1);
   for (int h = 0; h < p.G; ++h)
-    for (int i = threadIdx.x; i < bn; i += 256) {
+    for (int i = threadIdx.x; i < bn; i += THREADS) {
       const float x = b[h * (2 * p.R + 1) + max(0, min(2 * p.R, i - AP_PAD))];
       lbias[h * bn + i] = fabsf(x) > 1e37f && fabsf(x) < INFINITY ? copysignf(1e37f, x) : x * 1.4426950408889634f;
     }
@@ -201,27 +202,11 @@ struct ApState {
   bool unseen;              // a row of the wave has
 };
 
-// One key tile of 32 NB keys from kt for a wave's 32 rows: scores, weights and their sum, P V.  FIRST: nothing to add to or to
-// rescale, acc and st come in undefined.
+// Scores of 32 NB keys from kt to weights, packed, and their sum into st.  FIRST: nothing to add to or to rescale, acc and st come in undefined.
 template <int DT, int D, int NB, bool BIAS, bool FIRST>
-__device__ __forceinline__ void ap_tile(const ApParams& p, const ApScore& score, const char* sk, const char* sv, uint32_t krow, uint32_t kxor,
-                                        uint32_t vrow, uint32_t vxor, int kt, const v4i (&qf)[D / 16], v16f (&acc)[D / 32], ApState& st) {
-  constexpr int ROWB = 2 * D, KK = D / 16, DB = D / 32;
-  v16f s[NB];
-#pragma unroll
-  for (int b = 0; b < NB; ++b)
-#pragma unroll
-    for (int r = 0; r < 16; ++r) s[b][r] = 0.f;
-#pragma unroll
-  for (int kk = 0; kk < KK; ++kk)     // the blocks in turn: two MFMAs in a row do not depend on each other
-#pragma unroll
-    for (int b = 0; b < NB; ++b) {
-      const v4i kf = *reinterpret_cast<const v4i*>(sk + b * 32 * ROWB + krow + (kxor ^ (kk << 5)));
-      s[b] = ap_mma<DT>::run(kf, qf[kk], s[b]);
-    }
+__device__ __forceinline__ void ap_weights(const ApScore& score, int kt, v16f (&s)[NB], v16f (&acc)[D / 32], ApState& st, uint32_t (&pk)[NB][8]) {
   float mul, base;
   score.template finish<BIAS>(s, kt, mul, base);
-  uint32_t pk[NB][8];
   auto weights = [&]() {
     const float off = base - st.ref;
     float sum = 0.f;
@@ -255,7 +240,7 @@ __device__ __forceinline__ void ap_tile(const ApParams& p, const ApScore& score,
       st.m = mn;
       st.l *= alpha;
 #pragma unroll
-      for (int d = 0; d < DB; ++d)
+      for (int d = 0; d < D / 32; ++d)
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[d][r] *= alpha;
       sum = weights();
@@ -263,12 +248,26 @@ __device__ __forceinline__ void ap_tile(const ApParams& p, const ApScore& score,
     }
     st.l += sum;
   }
+}
+
+// A whole tile of 32 keys: scores, weights, P V.
+template <int DT, int D, bool BIAS, bool FIRST>
+__device__ __forceinline__ void ap_tile(const ApScore& score, const char* sk, const char* sv, uint32_t krow, uint32_t kxor,
+                                        uint32_t vrow, uint32_t vxor, int kt, const v4i (&qf)[D / 16], v16f (&acc)[D / 32], ApState& st) {
+  constexpr int ROWB = 2 * D;
+  v16f s[1];
 #pragma unroll
-  for (int t = 0; t < 2 * NB; ++t) {
-    const uint32_t* w = &pk[t >> 1][4 * (t & 1)];
+  for (int r = 0; r < 16; ++r) s[0][r] = 0.f;
+#pragma unroll
+  for (int kk = 0; kk < D / 16; ++kk) s[0] = ap_mma<DT>::run(*reinterpret_cast<const v4i*>(sk + krow + (kxor ^ (kk << 5))), qf[kk], s[0]);
+  uint32_t pk[1][8];
+  ap_weights<DT, D, 1, BIAS, FIRST>(score, kt, s, acc, st, pk);
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    const uint32_t* w = &pk[0][4 * t];
     const v4i pf = {(int)w[0], (int)w[1], (int)w[2], (int)w[3]};
 #pragma unroll
-    for (int d = 0; d < DB; ++d) {
+    for (int d = 0; d < D / 32; ++d) {
       const char* a = sv + t * 16 * ROWB + vrow + ((d << 6) ^ vxor);
       const v8s vf = __builtin_shufflevector(__builtin_amdgcn_ds_read_tr16_b64_v4i16((ap_trptr_t)a),
                                              __builtin_amdgcn_ds_read_tr16_b64_v4i16((ap_trptr_t)(a + 4 * ROWB)), 0, 1, 2, 3, 4, 5, 6, 7);
@@ -356,7 +355,7 @@ __global__ __launch_bounds__(256, D == 128 ? 3 : 4) void attn_packed_tile_kernel
   const int kend = p.causal ? min(it.key1, it.pos + q_last + 1) : it.key1;
   int kt = it.key0;
   if (kt < kend) fetch(kt, 0);
-  if constexpr (BIAS) ap_load_bias(p, kvh, bn, lbias);
+  if constexpr (BIAS) ap_load_bias<256>(p, kvh, bn, lbias);
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   v4i qf[KK];                                                          // Q^T fragments: B operand, lane = row, 8 consecutive d each
   {
@@ -381,7 +380,7 @@ __global__ __launch_bounds__(256, D == 128 ? 3 : 4) void attn_packed_tile_kernel
   auto tile = [&](auto first, int buf) {
     if (kt + BK < kend) fetch(kt + BK, buf ^ 1);
     if (kt < wend)
-      ap_tile<DT, D, 1, BIAS, decltype(first)::value>(p, score, smem + buf * STAGE, smem + buf * STAGE + TILE, krow, kxor, vrow, vxor, kt, qf, acc, st);
+      ap_tile<DT, D, BIAS, decltype(first)::value>(score, smem + buf * STAGE, smem + buf * STAGE + TILE, krow, kxor, vrow, vxor, kt, qf, acc, st);
     // this tile's reads have returned and the next tile has landed
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
     __syncthreads();
@@ -449,14 +448,36 @@ __global__ __launch_bounds__(256, D == 128 ? 3 : 4) void attn_packed_tile_kernel
   }
 }
 
-// ---- up to 32 rows; the waves take different keys, each with two LDS stages of its own, and join at the end ----
-// What bounds it: memory, K and V once: 16 sequences of up to 32 760 keys, 40 heads of 128 over 8 key heads, 702 MB in 137 us, 5.1
-// TB/s (a large copy moves 4.9).  One workgroup a CU with 64 KB in flight; 32 rows of the MFMA for G = 5 valid ones cost nothing
-// beside that.  A range of 777 keys of 12 heads takes 10 us in one launch, 6.6 + 4 split over four workgroups and joined.
+// The 16 transposing reads of a wave's V tile (8 KB), all in flight: vf[4 u + i] is the fragment at a[i] + 16 u rows.
+template <int ROWB>
+__device__ __forceinline__ void ap_read_v(const uint32_t (&a)[4], v4i (&vf)[8]) {
+  v2i x[16];
+  asm volatile(
+      "ds_read_b64_tr_b16 %0, %16\n ds_read_b64_tr_b16 %1, %16 offset:%20\n ds_read_b64_tr_b16 %2, %17\n ds_read_b64_tr_b16 %3, %17 offset:%20\n"
+      "ds_read_b64_tr_b16 %4, %18\n ds_read_b64_tr_b16 %5, %18 offset:%20\n ds_read_b64_tr_b16 %6, %19\n ds_read_b64_tr_b16 %7, %19 offset:%20\n"
+      "ds_read_b64_tr_b16 %8, %16 offset:%21\n ds_read_b64_tr_b16 %9, %16 offset:%22\n ds_read_b64_tr_b16 %10, %17 offset:%21\n"
+      "ds_read_b64_tr_b16 %11, %17 offset:%22\n ds_read_b64_tr_b16 %12, %18 offset:%21\n ds_read_b64_tr_b16 %13, %18 offset:%22\n"
+      "ds_read_b64_tr_b16 %14, %19 offset:%21\n ds_read_b64_tr_b16 %15, %19 offset:%22\n s_waitcnt lgkmcnt(0)"
+      : "=&v"(x[0]), "=&v"(x[1]), "=&v"(x[2]), "=&v"(x[3]), "=&v"(x[4]), "=&v"(x[5]), "=&v"(x[6]), "=&v"(x[7]), "=&v"(x[8]), "=&v"(x[9]),
+        "=&v"(x[10]), "=&v"(x[11]), "=&v"(x[12]), "=&v"(x[13]), "=&v"(x[14]), "=&v"(x[15])
+      : "v"(a[0]), "v"(a[1]), "v"(a[2]), "v"(a[3]), "n"(4 * ROWB), "n"(16 * ROWB), "n"(20 * ROWB)
+      : "memory");
+#pragma unroll
+  for (int i = 0; i < 8; ++i) vf[i] = v4i{x[2 * i][0], x[2 * i][1], x[2 * i + 1][0], x[2 * i + 1][1]};
+}
+
+// ---- up to 32 rows; the waves take different keys, each with a K and a V stage of its own, and join at the end ----
+// What bounds it: memory, K and V once: 16 sequences of up to 32 760 keys, 40 heads of 128 over 8 key heads, 702 MB in 134 us, 5.2
+// TB/s (a large copy moves 4.9).  One workgroup a CU with up to 128 KB in flight; 32 rows of the MFMA for G = 5 valid ones cost nothing
+// beside that.  A wave fetches its next K tile once this one is in registers and its next V tile likewise, so that 16 KB hold what
+// two stages did and eight waves fit where four did: a range of 777 keys of 12 heads 8.7 against 11.4 us.
+#define AP_FEW_WAVES 8
 template <int DT, int D, bool BIAS>
-__global__ __launch_bounds__(256, 1) void attn_packed_few_kernel(const ApParams p) {
+__global__ __launch_bounds__(64 * AP_FEW_WAVES, 1) void attn_packed_few_kernel(const ApParams p) {
   constexpr int NB = D == 128 ? 1 : 2, BK = 32 * NB;        // keys per tile
   constexpr int ROWB = 2 * D, TILE = BK * ROWB, STAGE = 2 * TILE, PIECES = TILE / 1024, RPP = 1024 / ROWB, KK = D / 16, DB = D / 32;
+  constexpr int NW = AP_FEW_WAVES;
+  static_assert(TILE == 8192 && PIECES == 8, "the waits below count pieces");
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int item = blockIdx.z * AP_GRID_Y + blockIdx.y, kvh = blockIdx.x;
   if (item >= p.n_items) return;
@@ -464,7 +485,7 @@ __global__ __launch_bounds__(256, 1) void attn_packed_few_kernel(const ApParams 
   const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int bn = 2 * p.R + 1 + 2 * AP_PAD;
-  float* const lbias = reinterpret_cast<float*>(smem + 8 * STAGE);
+  float* const lbias = reinterpret_cast<float*>(smem + NW * STAGE);
   v4i qf[KK];
   {
     int q, h;
@@ -474,28 +495,27 @@ __global__ __launch_bounds__(256, 1) void attn_packed_few_kernel(const ApParams 
     for (int kk = 0; kk < KK; ++kk) qf[kk] = *reinterpret_cast<const v4i*>(qp + 16 * kk);
   }
   if constexpr (BIAS) {
-    ap_load_bias(p, kvh, bn, lbias);
+    ap_load_bias<64 * NW>(p, kvh, bn, lbias);
     __syncthreads();
   }
   const ApScore score = ap_score<BIAS>(p, it, 0, lane, lbias, bn);
   const int kend = score.wmax;
 
   const int drow = lane / (ROWB / 16), dchunk = lane & (ROWB / 16 - 1);
+  char* const stage = smem + wave * STAGE;
+  // a tile of K (V) from key kt; rows past the range re-read the last one (finite, masked)
   const uint16_t* const kbase = p.k + (int64_t)it.k_begin * p.k_ts + (int64_t)kvh * p.k_hs;
   const uint16_t* const vbase = p.v + (int64_t)it.k_begin * p.v_ts + (int64_t)kvh * p.v_hs;
-  char* const mystage = smem + wave * 2 * STAGE;
-  auto fetch = [&](int kt, int buf) {                       // rows past the range re-read the last one (finite, masked)
+  auto fetch = [&](const uint16_t* b0, int64_t ts, char* dst, auto isv, int kt) {
     const int nv = min(it.key1 - kt, BK);
-    const uint16_t* kp = kbase + (int64_t)kt * p.k_ts;
-    const uint16_t* vp = vbase + (int64_t)kt * p.v_ts;
-    const uint32_t kbytes = (uint32_t)((nv - 1) * 2 * p.k_ts + ROWB), vbytes = (uint32_t)((nv - 1) * 2 * p.v_ts + ROWB);
-    char* st = mystage + buf * STAGE;
+    const uint16_t* b = b0 + (int64_t)kt * ts;
+    const uint32_t bytes = (uint32_t)((nv - 1) * 2 * ts + ROWB);
 #pragma unroll
     for (int t = 0; t < PIECES; ++t) {
-      const uint32_t r = RPP * t + drow, rc = min((int)r, nv - 1);
-      ap_dma(kp, kbytes, st + t * 1024, rc * (uint32_t)(2 * p.k_ts) + ((dchunk ^ ap_kx<D>(r)) << 4));
-      ap_dma(vp, vbytes, st + TILE + t * 1024, rc * (uint32_t)(2 * p.v_ts) + ((dchunk ^ ap_vx<D>(r)) << 4));
+      const uint32_t r = RPP * t + drow, rc = min((int)r, nv - 1), x = decltype(isv)::value ? ap_vx<D>(r) : ap_kx<D>(r);
+      ap_dma(b, bytes, dst + t * 1024, rc * (uint32_t)(2 * ts) + ((dchunk ^ x) << 4));
     }
+    asm volatile("" ::: "memory");       // the waits count these in order
   };
   const uint32_t kr = (lane & 19) | ((lane & 4) << 1) | ((lane & 8) >> 1);      // bits 2 and 3 of the row swapped
   const uint32_t krow = kr * ROWB, kxor = (half ^ ap_kx<D>(kr)) << 4;
@@ -503,6 +523,10 @@ __global__ __launch_bounds__(256, 1) void attn_packed_few_kernel(const ApParams 
   const uint32_t vkey = 8 * half + (i16 >> 2);
   const uint32_t vrow = vkey * ROWB + ((((lane >> 4) & 1) * 2 + ((i16 & 3) >> 1)) << 4) + (i16 & 1) * 8;
   const uint32_t vxor = ap_vx<D>(vkey) << 4;
+  uint32_t va[4];                        // fragment i: d block i % DB, 32 keys further for i >= DB
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    va[i] = (uint32_t)(uintptr_t)(ap_trptr_t)(stage + TILE) + vrow + (((i % DB) << 6) ^ vxor) + (i / DB) * 32 * ROWB;
 
   v16f acc[DB];
 #pragma unroll
@@ -511,42 +535,71 @@ __global__ __launch_bounds__(256, 1) void attn_packed_few_kernel(const ApParams 
     for (int r = 0; r < 16; ++r) acc[d][r] = 0.f;
   ApState st = {-INFINITY, 0.f, 0.f, true};
   int kt = it.key0 + wave * BK;
-  if (kt < kend) fetch(kt, 0);
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-  for (int buf = 0; kt < kend; kt += 4 * BK, buf ^= 1) {
-    if (kt + 4 * BK < kend) fetch(kt + 4 * BK, buf ^ 1);
-    const char* sk = mystage + buf * STAGE;
-    ap_tile<DT, D, NB, BIAS, false>(p, score, sk, sk + TILE, krow, kxor, vrow, vxor, kt, qf, acc, st);
-    // this tile's reads have returned and the next tile has landed (the stages are this wave's own)
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+  if (kt < kend) {
+    fetch(kbase, p.k_ts, stage, std::false_type{}, kt);
+    fetch(vbase, p.v_ts, stage + TILE, std::true_type{}, kt);
+  }
+  for (; kt < kend; kt += NW * BK) {
+    const bool more = kt + NW * BK < kend;
+    asm volatile("s_waitcnt vmcnt(8)" ::: "memory");                  // K has landed (V's 8 pieces came after it)
+    v4i kf[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) kf[i] = *reinterpret_cast<const v4i*>(stage + (i / KK) * 32 * ROWB + krow + (kxor ^ ((i % KK) << 5)));
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");                // and has been read: its stage is free (it is this wave's own)
+    if (more) fetch(kbase, p.k_ts, stage, std::false_type{}, kt + NW * BK);
+    v16f s[NB];
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[b][r] = 0.f;
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk)
+#pragma unroll
+      for (int b = 0; b < NB; ++b) s[b] = ap_mma<DT>::run(kf[b * KK + kk], qf[kk], s[b]);
+    uint32_t pk[NB][8];
+    ap_weights<DT, D, NB, BIAS, false>(score, kt, s, acc, st, pk);
+    if (more) asm volatile("s_waitcnt vmcnt(8)" ::: "memory");        // V has landed
+    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    v4i vf[8];
+    ap_read_v<ROWB>(va, vf);
+    if (more) fetch(vbase, p.v_ts, stage + TILE, std::true_type{}, kt + NW * BK);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int t = (i >> 2) + 2 * ((i & 3) / DB);
+      const uint32_t* w = &pk[t >> 1][4 * (t & 1)];
+      acc[i % DB] = ap_mma<DT>::run(vf[i], v4i{(int)w[0], (int)w[1], (int)w[2], (int)w[3]}, acc[i % DB]);
+    }
   }
   const float l = ap_other_half(st.l, false), m = st.m;
 
   // acc[d][r] is d = 32 d + 8 (r >> 2) + 4 half + (r & 3) of this lane's row
-  // ---- join the four waves through LDS ----
+  // ---- join the waves through LDS ----
   constexpr int LD = D + 4;
-  float* jo = reinterpret_cast<float*>(smem);                 // [4][32][LD]
-  float* jm = jo + 4 * 32 * LD;                               // [4][32][2]
+  float* jo = reinterpret_cast<float*>(smem);                 // [NW][32][LD]
+  float* jm = jo + NW * 32 * LD;                              // [NW][32][2]
   __syncthreads();
-  float* mo = jo + (wave * 32 + (lane & 31)) * LD;
+  const int row = lane & 31;
+  if (row < it.rows) {
+    float* mo = jo + (wave * 32 + row) * LD;
 #pragma unroll
-  for (int d = 0; d < DB; ++d)
+    for (int d = 0; d < DB; ++d)
 #pragma unroll
-    for (int r = 0; r < 16; r += 4)
-      *reinterpret_cast<float4*>(mo + 32 * d + 2 * r + 4 * half) = make_float4(acc[d][r], acc[d][r + 1], acc[d][r + 2], acc[d][r + 3]);
-  if (half == 0) { jm[(wave * 32 + lane) * 2] = m; jm[(wave * 32 + lane) * 2 + 1] = l; }
+      for (int r = 0; r < 16; r += 4)
+        *reinterpret_cast<float4*>(mo + 32 * d + 2 * r + 4 * half) = make_float4(acc[d][r], acc[d][r + 1], acc[d][r + 2], acc[d][r + 3]);
+    if (half == 0) { jm[(wave * 32 + row) * 2] = m; jm[(wave * 32 + row) * 2 + 1] = l; }
+  }
   __syncthreads();
-  constexpr int W = D / 8;                                    // d per thread
-  const int jr = tid >> 3, d0 = (tid & 7) * W;
+  constexpr int W = D / (2 * NW);                             // d per thread
+  const int jr = tid / (2 * NW), d0 = (tid % (2 * NW)) * W;
   if (jr < it.rows) {
     float mm = -INFINITY, ll = 0.f, oo[W];
 #pragma unroll
-    for (int w = 0; w < 4; ++w) mm = fmaxf(mm, jm[(w * 32 + jr) * 2]);
+    for (int w = 0; w < NW; ++w) mm = fmaxf(mm, jm[(w * 32 + jr) * 2]);
     const float mr = mm == -INFINITY ? 0.f : mm;
 #pragma unroll
     for (int e = 0; e < W; ++e) oo[e] = 0.f;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
+    for (int w = 0; w < NW; ++w) {
       const float a = __builtin_amdgcn_exp2f(jm[(w * 32 + jr) * 2] - mr);
       ll += a * jm[(w * 32 + jr) * 2 + 1];
 #pragma unroll
@@ -567,9 +620,8 @@ __global__ __launch_bounds__(256, 1) void attn_packed_few_kernel(const ApParams 
       ap_split(p, it, jr, q2, g2);
       uint16_t* op = p.o + (int64_t)(it.token + q2) * p.o_ts + (int64_t)(kvh * p.G + g2) * p.o_hs + d0;
 #pragma unroll
-      for (int e = 0; e < W; ++e) oo[e] *= inv;
-#pragma unroll
-      for (int e = 0; e < W; e += 8) *reinterpret_cast<uint4*>(op + e) = pack8<DT>(oo + e);
+      for (int e = 0; e < W; e += 4)
+        *reinterpret_cast<uint2*>(op + e) = make_uint2(pack2<DT>(oo[e] * inv, oo[e + 1] * inv), pack2<DT>(oo[e + 2] * inv, oo[e + 3] * inv));
     }
   }
 }
@@ -625,6 +677,26 @@ __global__ __launch_bounds__(256) void attn_packed_join_kernel(const ApParams p,
 // ---- the plan: which workgroup does what (host) --------------------------------------------------------------------
 // Table of 8-word records: tile items, few items, joins (in this order).  counts = {tile items, few items, joins, partial rows,
 // query tokens, key tokens}.
+
+// Keys a few workgroup takes.  One has a CU to itself and needs 2.5 us beside its keys; all 256 read 39 keys a us each (D = 128), one
+// alone 150.  W keys in parts of L take W / (39 * 256) + 2.5 W / (256 L) and, while the last ones run without the others, L / 150:
+// least at L = sqrt(1.5 W) (D = 64: sqrt(3 W)).  Or all run at once, if as many as there are CUs share W evenly.
+static int64_t ap_few_chunk(const std::vector<int64_t>& keys, int64_t total, int64_t kv_heads) {
+  const int64_t w = total * kv_heads;
+  const auto up = [](int64_t x) { return td_cdiv(std::max<int64_t>(x, 256), 128) * 128; };
+  const int64_t many = up((int64_t)std::sqrt(2.0 * (double)w));
+  // Not split: up to 1024 keys, where a workgroup is done before a second launch and the join would be (5 us), or little more than a part.
+  const int64_t longest = keys.empty() ? 0 : *std::max_element(keys.begin(), keys.end());
+  if (longest <= std::max<int64_t>(1024, many + many / 2)) return up(longest);
+  for (int64_t one = up(w / 256);; one += up(one / 32) - 128) {
+    one = std::min(one, up(longest));
+    int64_t n = 0;
+    for (int64_t x : keys) n += kv_heads * std::max<int64_t>(1, td_cdiv(x, one));
+    if (n <= 256 && (one <= many / 4 * 7 || (n >= 224 && w >= n * one / 8 * 7))) return one;
+    if (n <= 256 || one >= longest) return many;
+  }
+}
+
 extern "C" int td_attn_packed_plan(const int64_t* lens_q, const int64_t* lens_k, int64_t nseq, int heads, int kv_heads, int causal,
                                    int32_t* table, int64_t capacity, int64_t* counts) {
   TD_REQUIRE(lens_q && lens_k && counts && nseq >= 0, TD_ERR_INVALID, "td_attn_packed_plan: null pointer or %lld sequences", (long long)nseq);
@@ -641,7 +713,8 @@ extern "C" int td_attn_packed_plan(const int64_t* lens_q, const int64_t* lens_k,
     struct Work { ApItem it; int64_t keys; };
     std::vector<Work> work[2];
     std::vector<ApJoin> joins;
-    int64_t keys_total[2] = {0, 0}, few_longest = 0;
+    int64_t keys_total[2] = {0, 0};
+    std::vector<int64_t> few_keys;
     // few rows over few keys go with whatever kernel the others need
     bool few_short = false, any_tile = false;
     for (int64_t s = 0; s < nseq; ++s) {
@@ -662,12 +735,11 @@ extern "C" int td_attn_packed_plan(const int64_t* lens_q, const int64_t* lens_k,
           const int64_t end = causal ? std::max<int64_t>(0, std::min(kl, last / G + kl - ql + 1)) : kl;
           if (pass == 0) {
             keys_total[few] += end;
-            if (few) few_longest = std::max(few_longest, end);
+            if (few) few_keys.push_back(end);
             continue;
           }
-          const int64_t parts = std::max<int64_t>(1, td_cdiv(end, chunk[few]));
-          const int64_t quantum = few ? 128 : 64;
-          const int64_t per = td_cdiv(td_cdiv(std::max<int64_t>(end, 1), parts), quantum) * quantum;
+          int64_t per = chunk[few];          // few: the rest of a range makes a short part, which runs last
+          if (!few) per = td_cdiv(td_cdiv(std::max<int64_t>(end, 1), std::max<int64_t>(1, td_cdiv(end, per))), 64) * 64;
           const int64_t n = std::max<int64_t>(1, td_cdiv(end, per));
           const int32_t token = (int32_t)(q0 + r0 / G), head0 = (int32_t)(r0 % G), nr = (int32_t)(last - r0 + 1), pos = (int32_t)(r0 / G + kl - ql);
           if (n > 1) joins.push_back({token, head0, nr, (int32_t)ws_rows, (int32_t)n, (int32_t)tr, 0, 0});
@@ -682,12 +754,10 @@ extern "C" int td_attn_packed_plan(const int64_t* lens_q, const int64_t* lens_k,
         q0 += ql; k0 += kl;
       }
       if (pass == 0) {
-        // 256 CUs, two tile workgroups each (few: one).  A key range is split when it is longer than the share of one of these
-        // slots (few: half of it, to even the load out); a part is at least 512 keys (few: 256), below which writing and joining
-        // partials costs more than it saves.
+        // 256 CUs, two tile workgroups each.  A key range is split when it is longer than the share of one of these slots; a part is
+        // at least 512 keys, below which writing and joining partials costs more than it saves.
         chunk[0] = std::max<int64_t>(512, td_cdiv(keys_total[0] * kv_heads, 512));
-        // Up to 1024 keys a workgroup is done (under a microsecond per 128) before a second launch and the join would be (5 us).
-        chunk[1] = few_longest <= 1024 ? 1024 : std::max<int64_t>(256, td_cdiv(keys_total[1] * kv_heads, 512));
+        chunk[1] = ap_few_chunk(few_keys, keys_total[1], kv_heads);
       }
     }
     for (auto& w : work)   // longest first: the short ones fill the tail
@@ -711,11 +781,12 @@ extern "C" int td_attn_packed_plan(const int64_t* lens_q, const int64_t* lens_k,
 template <int DT, int D, bool FEW, bool BIAS>
 static void ap_launch(const ApParams& p, int64_t n, int bias_bytes, hipStream_t st) {
   static std::atomic<uint64_t> mask{0};
-  constexpr int tiles = FEW ? 131072 : (64 + AP_ROWS) * 2 * D;       // a stage of K + V and the rows; few: 2 stages of 16 KB for each wave
+  // a stage of K + V and the rows; few: 16 KB for each wave, at the end the waves' sums, maxima and rows over them
+  constexpr int tiles = FEW ? AP_FEW_WAVES * 16384 : (64 + AP_ROWS) * 2 * D, join = FEW ? AP_FEW_WAVES * 32 * (D + 4 + 2) * 4 : 0;
   const auto kernel = FEW ? attn_packed_few_kernel<DT, D, BIAS> : attn_packed_tile_kernel<DT, D, BIAS>;
-  td_ensure_dyn_lds((const void*)kernel, tiles + 32768, mask);
+  td_ensure_dyn_lds((const void*)kernel, std::max(tiles + 32768, join), mask);
   const dim3 grid((unsigned)p.Hkv, (unsigned)std::min<int64_t>(n, AP_GRID_Y), (unsigned)td_cdiv(n, AP_GRID_Y));
-  kernel<<<grid, 256, tiles + bias_bytes, st>>>(p);
+  kernel<<<grid, FEW ? 64 * AP_FEW_WAVES : 256, std::max(tiles + bias_bytes, join), st>>>(p);
 }
 
 extern "C" int td_attn_packed(const void* q, const void* k, const void* v, void* o, const int64_t* strides, int dtype, int heads, int kv_heads,
