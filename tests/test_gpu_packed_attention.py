@@ -141,6 +141,19 @@ def test_single_tokens_over_long_pasts(dtype, D, heads):
         check(ops.packed_attention(q, k, v, plan, bias=bias), ref, tol)
 
 
+@pytest.mark.parametrize("longest", [383, 385])
+@pytest.mark.parametrize("D", [64, 128])
+def test_many_single_tokens(D, longest):
+    """more workgroups than the chip holds at a time: short pasts take the tile kernel, one longer past brings all to the other"""
+    lens_k = [129 + (37 * i) % 200 for i in range(299)] + [longest]
+    lens = [1] * len(lens_k)
+    q, k, v = make(lens, lens_k, 4, 1, D, torch.bfloat16, seed=18)
+    plan = ops.AttentionPlan(lens, lens_k, heads=4, kv_heads=1, head_dim=D, causal=True)
+    assert (plan._counts[1] == 0) == (longest == 383)
+    ref, tol = formula(q, k, v, lens, lens_k, True)
+    check(ops.packed_attention(q, k, v, plan), ref, tol)
+
+
 @pytest.mark.parametrize("D", [64, 128])
 def test_several_tokens_over_a_long_past_split(D):
     """few workgroups of 128 rows over long keys: their ranges are split too; beside them rows that take the other kernel"""

@@ -14,8 +14,8 @@
 //
 // Two kernels, by rows of a sequence:
 //   tile  128 rows per workgroup, 32 per wave, key tiles of 32 shared by the four waves (LDS-DMA, two stages);
-//   few   <= 32 rows over more than 128 keys (new tokens): the four waves take different keys, each with its own two LDS stages and
-//         no barrier in the loop, and join at the end through LDS.
+//   few   <= 32 rows over more than 128 keys (new tokens): eight waves take different keys, each with its own LDS stage and no
+//         barrier in the loop, and join at the end through LDS.
 // Where there are too few workgroups for the chip the key range is split over several and joined by a third kernel.
 // P is rounded to the operands' 16-bit type for the second product (half a step, relative, of every weight: the errors of
 // independent weights average out below the output's own rounding); sums and statistics stay fp32.
@@ -32,7 +32,9 @@ typedef __attribute__((address_space(3))) ap_v4s* ap_trptr_t;
 
 #define AP_ROWS 128        // rows of a tile item
 #define AP_FEW 32          // rows of a few item
-#define AP_FEW_KEYS 128    // ... of sequences with more keys than this; with fewer the four waves would not all have a tile
+#define AP_FEW_KEYS 128    // ... of sequences with more keys than this, where all workgroups run at once (one token over 200 keys, 12 heads
+                           // of 128: 5.5 against 7.5 us).  Where they do not, the tile kernel has three a CU, which pays up to
+#define AP_MANY_KEYS 384   // ... this many (128 tokens over 150 keys each 39.9 against 26.1 us, 400: 68.7 against 60.0, 777: 116 against 127)
 #define AP_PAD 96          // the bias table repeats its ends: distances within a key tile of the range need no clamp
 #define AP_TAU 8.0f        // a row's reference moves when a score exceeds it by 8 (a weight of 2^8),
 #define AP_LOOK 4096.0f    // looked for when the 16 (32) weights of a lane in a tile add up to more than this
@@ -196,7 +198,8 @@ __device__ __forceinline__ ApScore ap_score(const ApParams& p, const ApItem& it,
 
 // Running state of a wave's rows: weights are exp2(score - ref).  ref is a row's maximum when it was last looked at, not its
 // running maximum: the maximum of a tile is taken only when a lane's weights of it add up to more than 2^12, which one weight of
-// more than 2^8 must have caused (of 60 vector instructions a block 24 less).  Weights up to 2^12 fit f16, bf16 and the fp32 sums.
+// more than 2^8 must have caused (of 60 vector instructions a block 24 less: 32 760 causal tokens 3.06 -> 2.85 ms).  Weights up to 2^12
+// fit f16, bf16 and the fp32 sums.
 struct ApState {
   float m, ref, l;          // m: ref, or -infinity while the row has seen nothing
   bool unseen;              // a row of the wave has
@@ -282,12 +285,12 @@ __device__ __forceinline__ void ap_tile(const ApScore& score, const char* sk, co
 }
 
 // ---- 128 rows, 32 per wave; key tiles of 32 shared by the waves, two LDS stages, one barrier a tile ----
-// What bounds it.  Long ranges: the matrix pipe at the clock that the power limit leaves (causal, 32 760 tokens, 12 heads of 128: 2.97
-// ms, 1.11 PFLOP/s, 0.80 of a large library product on the same card; with the softmax arithmetic taken out 2.72 ms).  Short
+// What bounds it.  Long ranges: the matrix pipe at the clock that the power limit leaves (causal, 32 760 tokens, 12 heads of 128: 2.85
+// ms, 1.16 PFLOP/s, 0.84 of a large library product on the same card; with the softmax arithmetic taken out 2.72 ms).  Short
 // ranges: the latency of a workgroup's first loads and the vector instructions around the loop.  Hence tiles of 32 keys - three
-// (D = 64: four) workgroups a CU instead of two: 226 keys under 50 960 rows of 12 heads 94 against 100 us, prompts of 1 to 512
-// tokens, 64 heads of 64, 35.3 against 36.7, the long range 1 % slower - and pointers that step instead of addresses
-// computed row by row (1250 -> 950 vector instructions a wave at 226 keys, 107 -> 100 us).
+// (D = 64: four) workgroups a CU instead of two: 226 keys under 50 960 rows of 12 heads 91 us (94 against 100 when tried), prompts
+// of 1 to 512 tokens, 64 heads of 64, 34.8 (35.3 against 36.7), the long range 1 % slower - and pointers that step instead of
+// addresses computed row by row (1250 -> 950 vector instructions a wave at 226 keys, 107 -> 100 us).
 template <int DT, int D, bool BIAS>
 __global__ __launch_bounds__(256, D == 128 ? 3 : 4) void attn_packed_tile_kernel(const ApParams p) {
   constexpr int BK = 32, ROWB = 2 * D, TILE = BK * ROWB, STAGE = 2 * TILE, PIECES = TILE / 4096, RPP = 1024 / ROWB, KK = D / 16, DB = D / 32;
@@ -717,9 +720,13 @@ extern "C" int td_attn_packed_plan(const int64_t* lens_q, const int64_t* lens_k,
     std::vector<int64_t> few_keys;
     // few rows over few keys go with whatever kernel the others need
     bool few_short = false, any_tile = false;
+    const auto is_few = [&](int64_t s, int64_t keys) { return lens_q[s] > 0 && lens_q[s] * G <= AP_FEW && lens_k[s] > keys; };
+    int64_t n_few = 0;
+    for (int64_t s = 0; s < nseq; ++s) n_few += is_few(s, AP_FEW_KEYS);
+    const int64_t few_keys_min = n_few * kv_heads > 256 ? AP_MANY_KEYS : AP_FEW_KEYS;
     for (int64_t s = 0; s < nseq; ++s) {
       any_tile |= lens_q[s] * G > AP_FEW;
-      few_short |= lens_q[s] > 0 && lens_q[s] * G <= AP_FEW && lens_k[s] > AP_FEW_KEYS;
+      few_short |= is_few(s, few_keys_min);
     }
     few_short &= !any_tile;
     // pass 0 counts the keys each kernel reads, pass 1 emits items of at most `chunk` keys
@@ -728,7 +735,7 @@ extern "C" int td_attn_packed_plan(const int64_t* lens_q, const int64_t* lens_k,
       int64_t q0 = 0, k0 = 0;
       for (int64_t s = 0; s < nseq; ++s) {
         const int64_t ql = lens_q[s], kl = lens_k[s], rows = ql * G;
-        const int few = rows <= AP_FEW && (kl > AP_FEW_KEYS || few_short);
+        const int few = rows <= AP_FEW && (kl > few_keys_min || few_short);
         const int64_t tr = few ? AP_FEW : AP_ROWS;
         for (int64_t r0 = 0; r0 < rows; r0 += tr) {
           const int64_t last = std::min(r0 + tr, rows) - 1;
