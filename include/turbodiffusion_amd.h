@@ -525,7 +525,7 @@ int td_attn_packed(const void* q, const void* k, const void* v, void* o, const i
  * when out == y).  x [rows, k], y / out [rows, n]: 16-bit, row strides in elements (multiples of 8; k, n too), 16-byte aligned.
  * bank: every adapter in fragment order (td_lora_pack): 32 ceil(k / 32) rank8 elements for A_i [rank, k], 32 ceil(n / 32) rank8 for
  * B_i [n, rank], rank8 = the rank rounded up to 8; adapters: num_adapters records {int64 offset of A_i, int64 offset of B_i
- * (elements), int32 rank8, f32 scale}; both on the device, trusted; the bank ends with 16384 spare elements of any content, which
+ * (elements), int32 rank, f32 scale}; both on the device, trusted; the bank ends with 16384 spare elements of any content, which
  * are read and not used.  max_rank: the largest rank8 (at most 256).
  * td_lora_plan (host only): lengths and adapter ids of the requests -> counts = {tiles with an adapter, tiles without, rows, rows
  * with an adapter, largest id + 1, rows per tile} and, with table != NULL, 4 (tiles with + without) + rows int32 words, which go to

@@ -131,6 +131,24 @@ def test_lora_rows_of_other_requests_do_not_leak():
     assert torch.equal(o[keep], base[keep])
 
 
+@pytest.mark.parametrize("rank", [5, 8, 24, 40, 100, 200])
+@pytest.mark.parametrize("rows,k", [(3, 64), (40, 8192), (8200, 64)])
+def test_lora_infinities_stay_what_the_formula_makes_of_them(rank, rows, k):
+    """a row whose A x overflows f16 in one rank, and one with an infinite x: infinities of B's signs, no NaN from the ranks that
+    the layout adds"""
+    y, x, pairs, _ = make(rows, k, 64, [rank], torch.float16, seed=6)
+    a, b = pairs[0]
+    x[0], x[1] = 0.0, 0.0
+    x[0, 3] = 60000.0
+    x[1, 3] = float("inf")
+    a[:, 3] = 0.5
+    a[0, 3] = 4.0                                     # 60000 * 4 is past f16, 60000 / 2 is not
+    b.copy_(b.abs() * 2.0 ** -6)
+    o = ops.lora_add(y, x, ops.AdapterBank([(a, b)]), ops.AdapterPlan([rows], [0]))
+    assert (o[0] == float("inf")).all() and (o[1] == float("inf")).all()
+    assert torch.isfinite(o[2:]).all()
+
+
 def test_lora_row_offsets_past_32_bits():
     """rows 2 MB apart in x, y and out"""
     lens, ids = [1500, 700], [0, -1]

@@ -28,7 +28,17 @@
 #define LR_MAX_RANK 256
 
 struct LoraTile { int32_t perm0, rows, adapter, pad; };
-struct LoraAdapter { int64_t a_off, b_off; int32_t rank8; float scale; };   // offsets in elements; rank rounded up to 8 (zeros)
+struct LoraAdapter {
+  int64_t a_off, b_off;       // elements
+  int32_t rank; float scale;
+  __device__ int rank8() const { return (rank + 7) & ~7; }      // as laid out: rounded up to 8 (zeros)
+};
+// S past the rank is zero, whatever an infinite row of x or what lies behind A in the bank made of it: B is zero there, and only
+// zero times zero is
+template <int DT> __device__ __forceinline__ uint2 lr_scaled(const float4& v, float scale, int r0, int rank) {
+  return make_uint2(pack2<DT>(r0 < rank ? v.x * scale : 0.f, r0 + 1 < rank ? v.y * scale : 0.f),
+                    pack2<DT>(r0 + 2 < rank ? v.z * scale : 0.f, r0 + 3 < rank ? v.w * scale : 0.f));
+}
 
 struct LoraParams {
   const uint16_t *x, *y; uint16_t* out;
@@ -143,7 +153,7 @@ __global__ __launch_bounds__(256, RJ <= 8 ? 2 : 1) void lora_shrink_kernel(const
   for (int i = 0; i < 4; ++i)                                     // rows past the tile repeat its last one
     xp[i] = p.x + (int64_t)p.perm[t.perm0 + min(row0 + 8 * i + (lane >> 3), t.rows - 1)] * p.ldx;
   const uint16_t* ap = p.bank + ad.a_off + (l16 * 4 + lq) * 8;
-  const int64_t astep = 32 * ad.rank8;
+  const int64_t astep = 32 * ad.rank8();
   const int nchunks = (int)((p.K + 63) / 64);
   const int per = (p.chunks + 3) / 4;
   const int c0 = blockIdx.y * p.chunks + wave * per, c1 = min(min(nchunks, (int)(blockIdx.y + 1) * p.chunks), c0 + per);
@@ -155,13 +165,13 @@ __global__ __launch_bounds__(256, RJ <= 8 ? 2 : 1) void lora_shrink_kernel(const
 #pragma unroll
     for (int j = 0; j < RJ; ++j) acc[g][j] = (v4f){0.f, 0.f, 0.f, 0.f};
 #define LR_SHRINK(NJ_) lr_shrink<DT, NJ_, RJ>(acc, xp, ap, astep, c0, c1, p.K, smem + wave * 4096, lane)
-  if (ad.rank8 <= 16) LR_SHRINK(1);
+  if (ad.rank8() <= 16) LR_SHRINK(1);
   else if constexpr (RJ > 1) {
-    if (ad.rank8 <= 32) LR_SHRINK(2);
+    if (ad.rank8() <= 32) LR_SHRINK(2);
     else if constexpr (RJ > 2) {
-      if (ad.rank8 <= 64) LR_SHRINK(4);
+      if (ad.rank8() <= 64) LR_SHRINK(4);
       else if constexpr (RJ > 4) {
-        if (ad.rank8 <= 128) LR_SHRINK(8);
+        if (ad.rank8() <= 128) LR_SHRINK(8);
         else if constexpr (RJ > 8) LR_SHRINK(16);
       }
     }
@@ -177,7 +187,7 @@ __global__ __launch_bounds__(256, RJ <= 8 ? 2 : 1) void lora_shrink_kernel(const
   __syncthreads();
   for (int i = wave; i < 2 * RJ; i += 4) {
     const int g = i / RJ, j = i % RJ, r = row0 + 16 * g + l16;
-    if (16 * j >= ad.rank8 || r >= t.rows) continue;
+    if (16 * j >= ad.rank8() || r >= t.rows) continue;
     float4 v = red[0][i][lane];
 #pragma unroll
     for (int w = 1; w < 4; ++w) {
@@ -186,8 +196,7 @@ __global__ __launch_bounds__(256, RJ <= 8 ? 2 : 1) void lora_shrink_kernel(const
     }
     const int64_t pr = t.perm0 + r;
     if (p.splits == 1)
-      *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(p.s) + pr * RS + 16 * j + 4 * lq) =
-          make_uint2(pack2<DT>(v.x * ad.scale, v.y * ad.scale), pack2<DT>(v.z * ad.scale, v.w * ad.scale));
+      *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(p.s) + pr * RS + 16 * j + 4 * lq) = lr_scaled<DT>(v, ad.scale, 16 * j + 4 * lq, ad.rank);
     else
       *reinterpret_cast<float4*>(reinterpret_cast<float*>(p.s) + ((int64_t)blockIdx.y * p.rows + pr) * RS + 16 * j + 4 * lq) = v;
   }
@@ -230,8 +239,8 @@ __device__ __forceinline__ void lr_expand(const LoraParams& p, const uint16_t* s
     }
 #pragma unroll
     for (int kk = 0; kk < NK; ++kk) {
-      const int r0 = min(32 * kk + 8 * lq, rank8 - 8);           // past the rank: any value, B is zero there
-      sf[kk] = *reinterpret_cast<const v4i*>(sb + (int64_t)min(g + l16, rows - 1) * srs + r0);
+      const int r0 = 32 * kk + 8 * lq, keep = r0 < rank8 ? -1 : 0;               // zero past the rank, like B
+      sf[kk] = *reinterpret_cast<const v4i*>(sb + (int64_t)min(g + l16, rows - 1) * srs + min(r0, rank8 - 8)) & (v4i){keep, keep, keep, keep};
     }
   };
   load(0);
@@ -263,8 +272,6 @@ __device__ __forceinline__ void lr_expand(const LoraParams& p, const uint16_t* s
   }
 }
 
-// S past the rank must be finite where B is zero: shrink leaves the ranks of a last half block (rank8 % 16 == 8) as whatever
-// lies behind the adapter in the bank, so nothing past rank8 is read
 template <int DT, int RJ>
 __global__ __launch_bounds__(256, RJ <= 8 ? 2 : 1) void lora_expand_kernel(const LoraParams p) {
   constexpr int RS = 16 * RJ, KK = (RJ + 1) / 2;
@@ -289,7 +296,7 @@ __global__ __launch_bounds__(256, RJ <= 8 ? 2 : 1) void lora_expand_kernel(const
   __shared__ __attribute__((aligned(16))) uint16_t ssum[LR_NARROW * (RS + 8)];
   if (p.splits > 1) {             // add the parts of S, scale, round (narrow tiles only)
     const float* sp = reinterpret_cast<const float*>(p.s) + (int64_t)t.perm0 * RS;
-    const int quads = ad.rank8 / 4;
+    const int quads = ad.rank8() / 4;
     for (int i = threadIdx.x; i < t.rows * quads; i += 256) {
       const int r = i / quads, c = 4 * (i - r * quads);
       float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -298,8 +305,7 @@ __global__ __launch_bounds__(256, RJ <= 8 ? 2 : 1) void lora_expand_kernel(const
         const float4 o = *reinterpret_cast<const float4*>(sp + (s * p.rows + r) * RS + c);
         v.x += o.x; v.y += o.y; v.z += o.z; v.w += o.w;
       }
-      *reinterpret_cast<uint2*>(ssum + r * (RS + 8) + c) =
-          make_uint2(pack2<DT>(v.x * ad.scale, v.y * ad.scale), pack2<DT>(v.z * ad.scale, v.w * ad.scale));
+      *reinterpret_cast<uint2*>(ssum + r * (RS + 8) + c) = lr_scaled<DT>(v, ad.scale, c, ad.rank);
     }
     sb = ssum;
     srs = RS + 8;
@@ -307,12 +313,12 @@ __global__ __launch_bounds__(256, RJ <= 8 ? 2 : 1) void lora_expand_kernel(const
   __syncthreads();
   if (n >= p.N) return;
   const uint16_t* bp = p.bank + ad.b_off + lane * 8;
-#define LR_EXPAND(NK_) lr_expand<DT, NK_>(p, sb, srs, prow, t.rows, bp, ad.rank8, n, l16, lq, turn[wave])
-  if (ad.rank8 <= 32) LR_EXPAND(1);
+#define LR_EXPAND(NK_) lr_expand<DT, NK_>(p, sb, srs, prow, t.rows, bp, ad.rank8(), n, l16, lq, turn[wave])
+  if (ad.rank8() <= 32) LR_EXPAND(1);
   else if constexpr (KK > 1) {
-    if (ad.rank8 <= 64) LR_EXPAND(2);
+    if (ad.rank8() <= 64) LR_EXPAND(2);
     else if constexpr (KK > 2) {
-      if (ad.rank8 <= 128) LR_EXPAND(4);
+      if (ad.rank8() <= 128) LR_EXPAND(4);
       else if constexpr (KK > 4) LR_EXPAND(8);
     }
   }
@@ -347,7 +353,7 @@ __global__ __launch_bounds__(512) void lora_few_kernel(const LoraParams p) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) xp[i] = p.x + (int64_t)prow[min(8 * i + (lane >> 3), t.rows - 1)] * p.ldx;
     const uint16_t* ap = p.bank + ad.a_off + (l16 * 4 + lq) * 8;
-    const int64_t astep = 32 * ad.rank8;
+    const int64_t astep = 32 * ad.rank8();
     const int nchunks = (int)((p.K + 63) / 64), per = (nchunks + W - 1) / W;
     v4f acc[2][RJ];
 #pragma unroll
@@ -355,9 +361,9 @@ __global__ __launch_bounds__(512) void lora_few_kernel(const LoraParams p) {
 #pragma unroll
       for (int j = 0; j < RJ; ++j) acc[g][j] = (v4f){0.f, 0.f, 0.f, 0.f};
 #define LR_SHRINK(NJ_) lr_shrink<DT, NJ_, RJ>(acc, xp, ap, astep, wave * per, min(nchunks, (wave + 1) * per), p.K, smem + wave * 4096, lane)
-    if (ad.rank8 <= 16) LR_SHRINK(1);
+    if (ad.rank8() <= 16) LR_SHRINK(1);
     else if constexpr (RJ > 1) {
-      if (ad.rank8 <= 32) LR_SHRINK(2);
+      if (ad.rank8() <= 32) LR_SHRINK(2);
       else if constexpr (RJ > 2) LR_SHRINK(4);
     }
 #undef LR_SHRINK
@@ -376,8 +382,7 @@ __global__ __launch_bounds__(512) void lora_few_kernel(const LoraParams p) {
         const float4 o = red[w][wave][lane];
         v.x += o.x; v.y += o.y; v.z += o.z; v.w += o.w;
       }
-      *reinterpret_cast<uint2*>(ssum + r * (RS + 8) + 16 * j + 4 * lq) =
-          make_uint2(pack2<DT>(v.x * ad.scale, v.y * ad.scale), pack2<DT>(v.z * ad.scale, v.w * ad.scale));
+      *reinterpret_cast<uint2*>(ssum + r * (RS + 8) + 16 * j + 4 * lq) = lr_scaled<DT>(v, ad.scale, 16 * j + 4 * lq, ad.rank);
     }
     __syncthreads();
   }
@@ -385,8 +390,8 @@ __global__ __launch_bounds__(512) void lora_few_kernel(const LoraParams p) {
   if (wave >= 4 || n >= p.N) return;
   const uint16_t* bp = p.bank + ad.b_off + lane * 8;
   float* const turn = reinterpret_cast<float*>(smem) + wave * 16 * LR_TURN;
-#define LR_EXPAND(NK_) lr_expand<DT, NK_>(p, ssum, RS + 8, prow, t.rows, bp, ad.rank8, n, l16, lq, turn)
-  if (ad.rank8 <= 32) LR_EXPAND(1);
+#define LR_EXPAND(NK_) lr_expand<DT, NK_>(p, ssum, RS + 8, prow, t.rows, bp, ad.rank8(), n, l16, lq, turn)
+  if (ad.rank8() <= 32) LR_EXPAND(1);
   else if constexpr (KK > 1) LR_EXPAND(2);
 #undef LR_EXPAND
 }
@@ -484,6 +489,7 @@ extern "C" int td_lora_add(const void* x, int64_t ldx, const void* y, int64_t ld
   TD_REQUIRE(counts[4] <= num_adapters, TD_ERR_INVALID, "td_lora_add: the plan names adapter %lld of %d", (long long)counts[4] - 1, num_adapters);
   TD_REQUIRE(counts[0] >= 0 && counts[1] >= 0 && counts[0] + counts[1] < (1 << 28), TD_ERR_INVALID, "td_lora_add: counts");
   TD_REQUIRE(counts[5] == LR_WIDE || counts[5] == LR_NARROW, TD_ERR_INVALID, "td_lora_add: counts");
+  TD_REQUIRE(out != y || ldo == ldy || counts[2] <= 1, TD_ERR_INVALID, "td_lora_add: out = y with another row stride");
   const LoraShape sh = lora_shape(counts, k, n, max_rank);
   TD_REQUIRE(counts[3] == 0 || sh.few || ws, TD_ERR_INVALID, "td_lora_add: null workspace");
   LoraParams p;

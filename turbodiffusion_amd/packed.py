@@ -271,7 +271,7 @@ class AdapterBank:
                 call("td_lora_pack", ptr(a), self.k, ptr(b), r, r, self.k, self.n, ptr(self.data[oa:]), ptr(self.data[ob:]), st)
                 meta[i, 0], meta[i, 1] = oa, ob
                 words = meta[i, 2:].view(torch.int32)
-                words[0] = r_
+                words[0] = r
                 words.view(torch.float32)[1] = scales[i]
             self.meta = meta.to(self.device)
         torch.cuda.current_stream(self.device).synchronize()      # laid out once, complete for every stream
