@@ -246,6 +246,21 @@ def test_strides_and_out(layout):
     assert (big == 7.0).all()                                  # nothing around it was written
 
 
+@pytest.mark.parametrize("heads", [(4, 4), (4, 2)])
+@pytest.mark.parametrize("n", [1, 40, 700])
+def test_one_token_into_out(heads, n):
+    """a token whose stride in q and out is arbitrary, as nothing follows it"""
+    H, Hkv = heads
+    q, k, v = make([1], [n], H, Hkv, 128, torch.bfloat16, seed=19)
+    plan = ops.AttentionPlan([1], [n], heads=H, kv_heads=Hkv, head_dim=128, causal=True)
+    ref, tol = formula(q, k, v, [1], [n], True)
+    big = torch.full((4, H, 136), 7.0, dtype=torch.bfloat16, device="cuda")
+    for out in (big[1:2, :, :128], torch.as_strided(big, (1, H, 128), (8, 136, 1), H * 136)):
+        check(ops.packed_attention(q, k, v, plan, out=out), ref, tol)
+        out[:] = 7.0
+        assert (big == 7.0).all()
+
+
 def test_key_offsets_past_32_bits():
     """keys and values whose rows lie 128 KB apart: 5 GB between the first and the last"""
     n, H, D = 40000, 2, 64

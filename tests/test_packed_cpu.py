@@ -93,6 +93,10 @@ def test_attention_plan_refusals():
         ops.AttentionPlan([1 << 30, 1 << 30], heads=2)
     with pytest.raises(ValueError):
         ops.AttentionPlan([3], heads=2, device="cpu")
+    with pytest.raises(ValueError):
+        ops.AttentionPlan([(1 << 64) + 3], heads=2)          # would be 3 in 64 bits
+    with pytest.raises(ValueError):
+        ops.AdapterPlan([3], [(1 << 64) - 1])                # would be -1
 
 
 def test_attention_refuses_cpu_tensors():

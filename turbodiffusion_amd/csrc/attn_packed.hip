@@ -691,6 +691,7 @@ static int64_t ap_few_chunk(const std::vector<int64_t>& keys, int64_t total, int
   // Not split: up to 1024 keys, where a workgroup is done before a second launch and the join would be (5 us), or little more than a part.
   const int64_t longest = keys.empty() ? 0 : *std::max_element(keys.begin(), keys.end());
   if (longest <= std::max<int64_t>(1024, many + many / 2)) return up(longest);
+  if ((int64_t)keys.size() * kv_heads > 256) return many;
   for (int64_t one = up(w / 256);; one += up(one / 32) - 128) {
     one = std::min(one, up(longest));
     int64_t n = 0;
@@ -809,6 +810,7 @@ extern "C" int td_attn_packed(const void* q, const void* k, const void* v, void*
     TD_REQUIRE(strides[i] < (1 << 24), TD_ERR_UNSUPPORTED, "td_attn_packed: token stride %lld (less than 2^24 elements)", (long long)strides[i]);
   TD_REQUIRE((((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)o | (uintptr_t)ws) & 15) == 0, TD_ERR_UNSUPPORTED,
              "td_attn_packed: pointers must be 16-byte aligned");
+  TD_REQUIRE(counts[4] <= 1 || strides[6] >= head_dim, TD_ERR_INVALID, "td_attn_packed: the tokens of o overlap");
   TD_REQUIRE(scale > 0.f && scale <= 1e38f, TD_ERR_INVALID, "td_attn_packed: scale must be positive, at most 1e38");
   const int64_t nt = counts[0], nf = counts[1], nj = counts[2], wr = counts[3];
   TD_REQUIRE(nt >= 0 && nf >= 0 && nj >= 0 && wr >= 0 && (nj == 0 || ws), TD_ERR_INVALID, "td_attn_packed: counts / workspace");
@@ -827,6 +829,7 @@ extern "C" int td_attn_packed(const void* q, const void* k, const void* v, void*
   p.q = (const uint16_t*)q; p.k = (const uint16_t*)k; p.v = (const uint16_t*)v; p.o = (uint16_t*)o;
   p.q_ts = strides[0]; p.q_hs = strides[1]; p.k_ts = strides[2]; p.k_hs = strides[3];
   p.v_ts = strides[4]; p.v_hs = strides[5]; p.o_ts = strides[6]; p.o_hs = strides[7];
+  if (counts[4] <= 1) p.o_ts = head_dim;         // the rows past a sequence's end lie behind the end of its last one
   p.bias = bias; p.R = bias_range;
   p.po = ws; p.pml = ws ? ws + (int64_t)kv_heads * wr * head_dim : nullptr; p.ws_rows = wr;
   p.Hkv = kv_heads; p.G = G; p.causal = causal ? 1 : 0;

@@ -29,6 +29,8 @@ def _lengths(lens, what):
     for n in lens:
         if isinstance(n, bool) or int(n) != n:
             raise ValueError(f"{what}: whole numbers, got {n!r}")
+        if not -1 << 63 <= n < 1 << 63:
+            raise ValueError(f"{what}: {n} does not fit 64 bits")
     return [int(n) for n in lens]
 
 
