@@ -301,6 +301,28 @@ def test_same_bits_every_time_on_any_stream_and_in_graphs():
         assert torch.equal(outs[0], base) and torch.equal(outs[1], base)
 
 
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("heads", [(4, 4), (20, 5)])
+def test_a_rows_bits_are_its_own(D, heads):
+    """scores that outgrow a row's first ones by 2^8 to 2^12: neither what earlier calls left in rows past a sequence's end nor a
+    sequence's other rows changes a row's bits"""
+    H, Hkv = heads
+    lens_k = [57, 39, 33, 31, 86, 63, 53, 92, 33, 100, 128, 90]
+    lens = [1, 3, 4, 4, 4, 1, 2, 4, 31, 7, 5, 90]
+    q, k, v = make(lens, lens_k, H, Hkv, D, torch.bfloat16, seed=20, std=3.0)
+    plan = ops.AttentionPlan(lens, lens_k, heads=H, kv_heads=Hkv, head_dim=D, causal=True)
+    first = ops.packed_attention(q, k, v, plan)
+    ref, tol = formula(q, k, v, lens, lens_k, True)
+    check(first, ref, tol)
+    for i in range(10):
+        ops.packed_attention(q * 2 ** i, k.roll(1, 0), v, plan)
+        assert torch.equal(ops.packed_attention(q, k, v, plan), first)
+    end = sum(lens) - 90
+    other = q.clone()
+    other[end + 40:] *= 100.0
+    assert torch.equal(ops.packed_attention(other, k, v, plan)[:end + 40], first[:end + 40])
+
+
 def test_refusals():
     lens = [5, 9]
     q, k, v = make(lens, lens, 4, 2, 64, torch.bfloat16)

@@ -229,15 +229,12 @@ __device__ __forceinline__ void ap_weights(const ApScore& score, int kt, v16f (&
     st.l = weights();
     st.unseen = __any(st.m == -INFINITY);
   } else {
-    float sum = 0.f;
-    bool look = st.unseen;
-    if (!look) {
-      sum = weights();
-      look = __any(sum > AP_LOOK);
-    }
-    if (look) {                       // a row that does not exceed its reference keeps it: its bits do not depend on its neighbours
+    float sum = weights();
+    if (st.unseen || __any(sum > AP_LOOK)) {
+      // a row moves for its own sum only: its bits do not depend on its neighbours (nor on what stands in rows past the end)
+      const bool own = ap_other_half(sum, true) > AP_LOOK || st.m == -INFINITY;
       const float mx = score.maximum(s, mul, base);
-      const float mn = mx > st.m + AP_TAU ? mx : st.m;
+      const float mn = own && mx > st.m + AP_TAU ? mx : st.m;
       st.ref = mn == -INFINITY ? 0.f : mn;
       const float alpha = __builtin_amdgcn_exp2f(st.m - st.ref);
       st.m = mn;
