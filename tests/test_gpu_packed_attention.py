@@ -156,7 +156,7 @@ def test_many_single_tokens(D, longest):
 
 @pytest.mark.parametrize("D", [64, 128])
 def test_several_tokens_over_a_long_past_split(D):
-    """few workgroups of 128 rows over long keys: their ranges are split too; beside them rows that take the other kernel"""
+    """few workgroups of 128 rows over long keys: their ranges are split too; beside them single tokens, on the same kernel"""
     lens, lens_k = [100, 1, 300, 2], [9000, 5000, 7001, 65]
     q, k, v = make(lens, lens_k, 2, 1, D, torch.bfloat16, seed=7)
     plan = ops.AttentionPlan(lens, lens_k, heads=2, kv_heads=1, head_dim=D, causal=True)

@@ -12,9 +12,9 @@
 // in the order (bits 2 and 3 of the row swapped) in which its result registers are the second one's B operand: P never leaves
 // the registers.  V^T fragments come from the row-major V tile by the transposing LDS read.
 //
-// Two kernels, by rows of a sequence:
+// Two kernels, by the rows of a batch's sequences:
 //   tile  128 rows per workgroup, 32 per wave, key tiles of 32 shared by the four waves (LDS-DMA, two stages);
-//   few   <= 32 rows over more than 128 keys (new tokens): eight waves take different keys, each with its own LDS stage and no
+//   few   <= 32 rows each, some over more than 128 keys (new tokens): eight waves take different keys, each with its own LDS stage and no
 //         barrier in the loop, and join at the end through LDS.
 // Where there are too few workgroups for the chip the key range is split over several and joined by a third kernel.
 // P is rounded to the operands' 16-bit type for the second product (half a step, relative, of every weight: the errors of
@@ -32,7 +32,7 @@ typedef __attribute__((address_space(3))) ap_v4s* ap_trptr_t;
 
 #define AP_ROWS 128        // rows of a tile item
 #define AP_FEW 32          // rows of a few item
-#define AP_FEW_KEYS 128    // ... of sequences with more keys than this, where all workgroups run at once (one token over 200 keys, 12 heads
+#define AP_FEW_KEYS 128    // ... of batches with more keys for some than this, where all workgroups run at once (one token over 200 keys, 12 heads
                            // of 128: 5.5 against 7.5 us).  Where they do not, the tile kernel has three a CU, which pays up to
 #define AP_MANY_KEYS 384   // ... this many (128 tokens over 150 keys each 39.9 against 26.1 us, 400: 68.7 against 60.0, 777: 116 against 127)
 #define AP_PAD 96          // the bias table repeats its ends: distances within a key tile of the range need no clamp
@@ -712,46 +712,43 @@ extern "C" int td_attn_packed_plan(const int64_t* lens_q, const int64_t* lens_k,
   }
   try {
     struct Work { ApItem it; int64_t keys; };
-    std::vector<Work> work[2];
+    std::vector<Work> work;
     std::vector<ApJoin> joins;
-    int64_t keys_total[2] = {0, 0};
-    std::vector<int64_t> few_keys;
-    // few rows over few keys go with whatever kernel the others need
-    bool few_short = false, any_tile = false;
-    const auto is_few = [&](int64_t s, int64_t keys) { return lens_q[s] > 0 && lens_q[s] * G <= AP_FEW && lens_k[s] > keys; };
-    int64_t n_few = 0;
-    for (int64_t s = 0; s < nseq; ++s) n_few += is_few(s, AP_FEW_KEYS);
-    const int64_t few_keys_min = n_few * kv_heads > 256 ? AP_MANY_KEYS : AP_FEW_KEYS;
+    // One kernel for the whole batch (a second launch costs more than the better kernel saves: a prompt of 512 tokens and 8 tokens over
+    // 900 keys each, 40 heads of 128 over 8, 21 us by the tile kernel, 28 by both; 8000 keys 58 against 75).
+    bool few = true;
+    int64_t n_few = 0, few_longest = 0;
     for (int64_t s = 0; s < nseq; ++s) {
-      any_tile |= lens_q[s] * G > AP_FEW;
-      few_short |= is_few(s, few_keys_min);
+      few &= lens_q[s] * G <= AP_FEW;
+      if (lens_q[s] == 0) continue;
+      n_few += lens_k[s] > AP_FEW_KEYS;
+      few_longest = std::max(few_longest, lens_k[s]);
     }
-    few_short &= !any_tile;
-    // pass 0 counts the keys each kernel reads, pass 1 emits items of at most `chunk` keys
-    int64_t chunk[2] = {0, 0}, ws_rows = 0;
+    few &= few_longest > (n_few * kv_heads > 256 ? AP_MANY_KEYS : AP_FEW_KEYS);
+    const int64_t tr = few ? AP_FEW : AP_ROWS;
+    // pass 0 counts the keys, pass 1 emits items of at most `chunk` keys
+    std::vector<int64_t> ranges;
+    int64_t chunk = 0, total = 0, ws_rows = 0;
     for (int pass = 0; pass < 2; ++pass) {
       int64_t q0 = 0, k0 = 0;
       for (int64_t s = 0; s < nseq; ++s) {
         const int64_t ql = lens_q[s], kl = lens_k[s], rows = ql * G;
-        const int few = rows <= AP_FEW && (kl > few_keys_min || few_short);
-        const int64_t tr = few ? AP_FEW : AP_ROWS;
         for (int64_t r0 = 0; r0 < rows; r0 += tr) {
           const int64_t last = std::min(r0 + tr, rows) - 1;
           const int64_t end = causal ? std::max<int64_t>(0, std::min(kl, last / G + kl - ql + 1)) : kl;
           if (pass == 0) {
-            keys_total[few] += end;
-            if (few) few_keys.push_back(end);
+            total += end;
+            if (few) ranges.push_back(end);
             continue;
           }
-          int64_t per = chunk[few];          // few: the rest of a range makes a short part, which runs last
+          int64_t per = chunk;               // few: the rest of a range makes a short part, which runs last
           if (!few) per = td_cdiv(td_cdiv(std::max<int64_t>(end, 1), std::max<int64_t>(1, td_cdiv(end, per))), 64) * 64;
           const int64_t n = std::max<int64_t>(1, td_cdiv(end, per));
           const int32_t token = (int32_t)(q0 + r0 / G), head0 = (int32_t)(r0 % G), nr = (int32_t)(last - r0 + 1), pos = (int32_t)(r0 / G + kl - ql);
           if (n > 1) joins.push_back({token, head0, nr, (int32_t)ws_rows, (int32_t)n, (int32_t)tr, 0, 0});
           for (int64_t i = 0; i < n; ++i) {
             const int64_t a = i * per, b = std::min(end, a + per);
-            work[few].push_back({{token, head0, nr, pos, (int32_t)k0, (int32_t)a, (int32_t)b,
-                                  n > 1 ? (int32_t)(ws_rows + i * tr) : -1}, b - a});
+            work.push_back({{token, head0, nr, pos, (int32_t)k0, (int32_t)a, (int32_t)b, n > 1 ? (int32_t)(ws_rows + i * tr) : -1}, b - a});
           }
           if (n > 1) ws_rows += n * tr;
           TD_REQUIRE(ws_rows <= MAXT, TD_ERR_UNSUPPORTED, "td_attn_packed_plan: more than 2^30 partial rows");
@@ -761,19 +758,18 @@ extern "C" int td_attn_packed_plan(const int64_t* lens_q, const int64_t* lens_k,
       if (pass == 0) {
         // 256 CUs, two tile workgroups each.  A key range is split when it is longer than the share of one of these slots; a part is
         // at least 512 keys, below which writing and joining partials costs more than it saves.
-        chunk[0] = std::max<int64_t>(512, td_cdiv(keys_total[0] * kv_heads, 512));
-        chunk[1] = ap_few_chunk(few_keys, keys_total[1], kv_heads);
+        chunk = few ? ap_few_chunk(ranges, total, kv_heads) : std::max<int64_t>(512, td_cdiv(total * kv_heads, 512));
       }
     }
-    for (auto& w : work)   // longest first: the short ones fill the tail
-      std::stable_sort(w.begin(), w.end(), [](const Work& a, const Work& b) { return a.keys > b.keys; });
-    counts[0] = (int64_t)work[0].size(); counts[1] = (int64_t)work[1].size(); counts[2] = (int64_t)joins.size();
+    // longest first: the short ones fill the tail
+    std::stable_sort(work.begin(), work.end(), [](const Work& a, const Work& b) { return a.keys > b.keys; });
+    counts[few] = (int64_t)work.size(); counts[!few] = 0; counts[2] = (int64_t)joins.size();
     counts[3] = ws_rows; counts[4] = tq; counts[5] = tk;
     const int64_t n = counts[0] + counts[1] + counts[2];
     if (table) {
       TD_REQUIRE(capacity >= n, TD_ERR_INVALID, "td_attn_packed_plan: table of %lld records, %lld needed", (long long)capacity, (long long)n);
       ApItem* t = reinterpret_cast<ApItem*>(table);
-      for (auto& w : work) for (auto& x : w) *t++ = x.it;
+      for (auto& x : work) *t++ = x.it;
       for (auto& j : joins) *reinterpret_cast<ApJoin*>(t++) = j;
     }
   } catch (const std::bad_alloc&) {
