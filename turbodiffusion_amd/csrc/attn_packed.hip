@@ -38,6 +38,7 @@ typedef __attribute__((address_space(3))) ap_v4s* ap_trptr_t;
 #define AP_PAD 96          // the bias table repeats its ends: distances within a key tile of the range need no clamp
 #define AP_TAU 8.0f        // a row's reference moves when a score exceeds it by 8 (a weight of 2^8),
 #define AP_LOOK 4096.0f    // looked for when the 16 (32) weights of a lane in a tile add up to more than this
+#define AP_STEP 4194304.0f // from here on a reference's own rounding (2^-24 of it) is a matter of weights: 2^22, where that is 2^0.25
 
 // One workgroup's work per key head: `rows` rows from head `head0` of query token `token`, which stands at position `pos` of its
 // sequence, over keys [key0, key1) of the sequence whose first key token is k_begin.  slot: row in the partial buffer, -1 = writes o
@@ -200,9 +201,13 @@ __device__ __forceinline__ ApScore ap_score(const ApParams& p, const ApItem& it,
 // running maximum: the maximum of a tile is taken only when a lane's weights of it add up to more than 2^12, which one weight of
 // more than 2^8 must have caused (of 60 vector instructions a block 24 less: 32 760 causal tokens 3.06 -> 2.85 ms).  Weights up to 2^12
 // fit f16, bf16 and the fp32 sums.
+//
+// score = mul * s + base is fused into the exponent, so it is never rounded by itself, while ref is.  Where a score is large (a far tile
+// under a bias of -1e9, products of 1e9) that rounding is many powers of two: a weight against ref could be anything.  Rows whose ref
+// reaches AP_STEP take their scores rounded as ref was, so the largest weighs 1; they alone, for a row's bits are its own.
 struct ApState {
   float m, ref, l;          // m: ref, or -infinity while the row has seen nothing
-  bool unseen;              // a row of the wave has
+  bool look;                // a row of the wave has, or its ref is that large: the maximum of every tile is taken
 };
 
 // Scores of 32 NB keys from kt to weights, packed, and their sum into st.  FIRST: nothing to add to or to rescale, acc and st come in undefined.
@@ -210,6 +215,15 @@ template <int DT, int D, int NB, bool BIAS, bool FIRST>
 __device__ __forceinline__ void ap_weights(const ApScore& score, int kt, v16f (&s)[NB], v16f (&acc)[D / 32], ApState& st, uint32_t (&pk)[NB][8]) {
   float mul, base;
   score.template finish<BIAS>(s, kt, mul, base);
+  auto settle = [&]() {
+    const bool own = fabsf(st.ref) >= AP_STEP;
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[b][r] = own ? fmaf(s[b][r], mul, base) : s[b][r];
+    mul = own ? 1.f : mul;
+    base = own ? 0.f : base;
+  };
   auto weights = [&]() {
     const float off = base - st.ref;
     float sum = 0.f;
@@ -226,13 +240,14 @@ __device__ __forceinline__ void ap_weights(const ApScore& score, int kt, v16f (&
   if constexpr (FIRST) {
     st.m = score.maximum(s, mul, base);
     st.ref = st.m == -INFINITY ? 0.f : st.m;
+    st.look = __any(fabsf(st.m) >= AP_STEP);           // -infinity too
+    if (st.look) settle();
     st.l = weights();
-    st.unseen = __any(st.m == -INFINITY);
   } else {
     float sum = weights();
-    if (st.unseen || __any(sum > AP_LOOK)) {
+    if (st.look || __any(sum > AP_LOOK)) {
       // a row moves for its own sum only: its bits do not depend on its neighbours (nor on what stands in rows past the end)
-      const bool own = ap_other_half(sum, true) > AP_LOOK || st.m == -INFINITY;
+      const bool own = ap_other_half(sum, true) > AP_LOOK || fabsf(st.m) >= AP_STEP;
       const float mx = score.maximum(s, mul, base);
       const float mn = own && mx > st.m + AP_TAU ? mx : st.m;
       st.ref = mn == -INFINITY ? 0.f : mn;
@@ -243,8 +258,9 @@ __device__ __forceinline__ void ap_weights(const ApScore& score, int kt, v16f (&
       for (int d = 0; d < D / 32; ++d)
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[d][r] *= alpha;
+      st.look = __any(fabsf(st.m) >= AP_STEP);
+      if (st.look) settle();
       sum = weights();
-      st.unseen = __any(st.m == -INFINITY);
     }
     st.l += sum;
   }
@@ -302,7 +318,7 @@ __global__ __launch_bounds__(256, D == 128 ? 3 : 4) void attn_packed_tile_kernel
   const int drow = lane / (ROWB / 16), dchunk = lane & (ROWB / 16 - 1);
 
   // ---- Q: whole rows (memory likes full lines) into LDS from stage 1 on, until tile 1 comes; rows past the end are not
-  //      read (whatever LDS holds, never stored).  One head per key head: the rows are evenly spaced, a bounds-checked buffer needs
+  //      read (zeros below, never stored).  One head per key head: the rows are evenly spaced, a bounds-checked buffer needs
   //      no comparison, and the permutation of a row's chunks has a period of PER groups ----
   char* const qstage = smem + STAGE + x0 * ROWB;
   constexpr int PER = D == 128 ? 4 : 2;
@@ -362,6 +378,11 @@ __global__ __launch_bounds__(256, D == 128 ? 3 : 4) void attn_packed_tile_kernel
     const uint32_t r = lane & 31;
 #pragma unroll
     for (int kk = 0; kk < KK; ++kk) qf[kk] = *reinterpret_cast<const v4i*>(qstage + r * ROWB + (((half ^ ap_kx<D>(r)) << 4) ^ (kk << 5)));
+    if (x0 + 32 > it.rows) {         // what LDS held would send the whole wave after its maxima
+      const int keep = x0 + (int)r < it.rows ? -1 : 0;
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk) qf[kk] &= (v4i){keep, keep, keep, keep};
+    }
   }
   __syncthreads();
   const ApScore score = ap_score<BIAS>(p, it, x0, lane, lbias, bn);
