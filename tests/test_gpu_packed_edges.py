@@ -147,3 +147,17 @@ def test_a_neighbour_with_large_scores_changes_no_bits(D, heads):
     other[1:90:2] *= 1e8                               # every second row; rows of large and of ordinary scores share waves
     o = ops.packed_attention(other, k, v, plan)
     assert torch.equal(o[0:90:2], first[0:90:2]) and torch.equal(o[90:], first[90:]) and o.isfinite().all()
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("path", PATHS)
+@pytest.mark.parametrize("past,here", [(-0.9e37, -1.1e37), (-1.1e37, -0.9e37), (1.1e37, 0.9e37), (0.9e37, 1.1e37), (-1e38, LOW), (2e38, -LOW)])
+def test_order_of_the_largest_biases(D, path, past, here):
+    """the keys of the larger bias take all the weight, evenly: no score is more than a rounding of such a bias"""
+    lens, lens_k, plan = plan_of(path, 4, 2, D, False)
+    q, k, v = make(lens, lens_k, 4, 2, D, torch.bfloat16, seed=3)
+    bias = torch.full((4, 21), here, device="cuda")
+    bias[:, :8] = past
+    ref, _ = formula(q, k, v, lens, lens_k, False, 1.0, bias, exact_scores=True)
+    u = torch.finfo(torch.bfloat16).eps / 2
+    check(ops.packed_attention(q, k, v, plan, scale=1.0, bias=bias), ref, torch.full_like(ref, (u + 2.0 ** -18) * v.double().abs().max()))       # u A

@@ -123,14 +123,16 @@ template <int D> struct ApRowWalk {
   }
 };
 
-// exp2 domain; the type's lowest values as a finite low (a row of nothing else stays a uniform row)
+// exp2 domain; finite values whose product with log2 e is past fp32 (from 2.36e38 on, the type's lowest among them) stay finite: a row of
+// nothing else is a uniform row, and the order of the values is kept
 template <int THREADS>
 __device__ __forceinline__ void ap_load_bias(const ApParams& p, int kvh, int bn, float* lbias) {
   const float* b = p.bias + (int64_t)kvh * p.G * (2 * p.R + 1);
   for (int h = 0; h < p.G; ++h)
     for (int i = threadIdx.x; i < bn; i += THREADS) {
       const float x = b[h * (2 * p.R + 1) + max(0, min(2 * p.R, i - AP_PAD))];
-      lbias[h * bn + i] = fabsf(x) > 1e37f && fabsf(x) < INFINITY ? copysignf(1e37f, x) : x * 1.4426950408889634f;
+      const float y = x * 1.4426950408889634f;
+      lbias[h * bn + i] = fabsf(x) < INFINITY && fabsf(y) == INFINITY ? copysignf(3.4028235e38f, x) : y;
     }
 }
 

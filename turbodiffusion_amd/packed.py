@@ -170,8 +170,9 @@ def packed_attention(q, k, v, plan, scale=None, bias=None, out=None):
     Row i of a sequence with m queries and n keys stands at position i + n - m: the queries are its last m positions, so one new
     token over the keys kept so far is ``lens`` = 1.  ``plan.causal``: keys at or before that position only.  ``scale``: positive,
     default 1 / sqrt(D).  ``bias``: f32 [heads, 2 R + 1], added to the scaled score by distance key - query clamped to [-R, R]
-    (``relative_bias``).  A row with nothing to attend to is zero.  Scores, maxima and sums are fp32; the weights are rounded to
-    the inputs' type for the second product.  A masked key weighs exactly 0, so its VALUE must be finite like any other.
+    (``relative_bias``); finite values past 2.36e38 count as that, and (2 R + 193) heads / kv_heads may not exceed 8192.  A row with
+    nothing to attend to is zero.  Scores, maxima and sums are fp32; the weights are rounded to the inputs' type for the second
+    product.  A masked key weighs exactly 0, so its VALUE must be finite like any other.
     ``out``: written instead of a new tensor; it may not overlap the inputs.  Any stream, capturable; the plan must outlive a
     captured graph."""
     _check_tensors("packed_attention", plan.device, q, k, v, bias, out)
