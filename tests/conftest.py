@@ -35,8 +35,22 @@ def _gemm_dequant_mode(request):
         K.set_tuning(K.TUNE_GEMM_FAST, 0)
 
 
+# Tests that expect a value which the operator's definition contradicts: they run, and are expected to fail.
+CONTRADICTED = {
+    f"test_gpu_lora.py::test_lora_infinities_stay_what_the_formula_makes_of_them[{size}-{rank}]":
+        "expects infinity for row 0 in f16; y + B (A x) in 64 bits is below 52 000 there (S = 240 000 and 30 000, |B| about 2^-6), finite "
+        "in f16: test_gpu_lora_range.py::test_an_inner_product_past_f16 compares the same row with the formula"
+    for size in ("3-64", "40-8192", "8200-64") for rank in (5, 8, 24, 40, 100)      # at rank 200 the formula itself is past f16
+}
+
+
 def pytest_collection_modifyitems(config, items):
     import torch
+
+    for item in items:
+        reason = CONTRADICTED.get(item.nodeid.rsplit("/", 1)[-1])
+        if reason:
+            item.add_marker(pytest.mark.xfail(reason=reason, strict=True))
 
     if torch.cuda.is_available():
         return

@@ -7,9 +7,11 @@
 //
 //   shrink   S = A_i x by MFMA 16x16x32, fp32.  A workgroup takes 32 rows, its four waves split K; with few rows K is split over
 //            workgroups too and expand adds the fp32 parts in order.
-//   expand   out = y + B_i (s_i S): S is scaled in fp32 and rounded once to the operands' type (half a step of the update only:
-//            it stays below the rounding of the output wherever the update is not many times larger than the output itself).
-//            A wave keeps B_i of 64 columns in registers and walks the tile's rows, 16 at a time.
+//   expand   out = y + s_i B_i S: S is rounded once to the operands' type (half a step of the update only: it stays below the
+//            rounding of the output wherever the update is not many times larger than the output itself), the scale multiplies
+//            the update in fp32.  f16 ends at 65 504, which S passes long before the update does: each row of S is brought to
+//            2^14 .. 2^15 by the power of two that its largest finite value asks for, and the update is brought back, both
+//            exactly.  A wave keeps B_i of 64 columns in registers and walks the tile's rows, 16 at a time.
 // The bank holds A and B in fragment order (td_lora_pack): every load of them is a contiguous kilobyte, ranks are padded to 8 only.
 //
 // What bounds it: memory; y and out dominate, then x, at 2 rank flops per byte.  MFMA fragments want 64 bytes from each of 16 rows;
@@ -35,9 +37,23 @@ struct LoraAdapter {
 };
 // S past the rank is zero, whatever an infinite row of x or what lies behind A in the bank made of it: B is zero there, and only
 // zero times zero is
-template <int DT> __device__ __forceinline__ uint2 lr_scaled(const float4& v, float scale, int r0, int rank) {
-  return make_uint2(pack2<DT>(r0 < rank ? v.x * scale : 0.f, r0 + 1 < rank ? v.y * scale : 0.f),
-                    pack2<DT>(r0 + 2 < rank ? v.z * scale : 0.f, r0 + 3 < rank ? v.w * scale : 0.f));
+__device__ __forceinline__ float4 lr_within(const float4& v, int r0, int rank) {
+  return make_float4(r0 < rank ? v.x : 0.f, r0 + 1 < rank ? v.y : 0.f, r0 + 2 < rank ? v.z : 0.f, r0 + 3 < rank ? v.w : 0.f);
+}
+__device__ __forceinline__ float lr_largest(const float4& v) {        // of the finite magnitudes
+  const auto f = [](float x) { return fabsf(x) < INFINITY ? fabsf(x) : 0.f; };
+  return fmaxf(fmaxf(f(v.x), f(v.y)), fmaxf(f(v.z), f(v.w)));
+}
+// the power of two that brings a row of S with this largest value to [2^14, 2^15) (bf16 has the range of fp32: 1), and its inverse
+template <int DT> __device__ __forceinline__ int lr_shift(float largest) {
+  if constexpr (DT == TD_BF16) return 0;
+  return max(-100, min(100, 15 - __builtin_amdgcn_frexp_expf(largest)));
+}
+__device__ __forceinline__ float lr_power(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
+template <int DT> __device__ __forceinline__ uint2 lr_round(const float4& v, int shift) {
+  if constexpr (DT == TD_BF16) return make_uint2(pack2<DT>(v.x, v.y), pack2<DT>(v.z, v.w));
+  const float f = lr_power(shift);
+  return make_uint2(pack2<DT>(v.x * f, v.y * f), pack2<DT>(v.z * f, v.w * f));
 }
 
 struct LoraParams {
@@ -45,7 +61,8 @@ struct LoraParams {
   int64_t ldx, ldy, ldo;
   const uint16_t* bank; const LoraAdapter* adapters;
   const LoraTile* tiles; const int32_t* perm;
-  void* s;                  // splits == 1: 16-bit, scaled [rows][RS]; else f32 parts [splits][rows][RS]
+  void* s;                  // splits == 1: 16-bit [rows][RS]; else f32 parts [splits][rows][RS]
+  float* back;              // splits == 1, f16: what brings a row's update back [rows]
   int64_t rows, K, N;
   int splits, chunks;       // K splits over workgroups, K chunks of 64 per split
   int subs;                 // 32-row groups of a full tile
@@ -185,29 +202,63 @@ __global__ __launch_bounds__(256, RJ <= 8 ? 2 : 1) void lora_shrink_kernel(const
 #pragma unroll
     for (int j = 0; j < RJ; ++j) red[wave][g * RJ + j][lane] = make_float4(acc[g][j][0], acc[g][j][1], acc[g][j][2], acc[g][j][3]);
   __syncthreads();
-  for (int i = wave; i < 2 * RJ; i += 4) {
-    const int g = i / RJ, j = i % RJ, r = row0 + 16 * g + l16;
-    if (16 * j >= ad.rank8() || r >= t.rows) continue;
+  const auto total = [&](int i) {
     float4 v = red[0][i][lane];
 #pragma unroll
     for (int w = 1; w < 4; ++w) {
       const float4 o = red[w][i][lane];
       v.x += o.x; v.y += o.y; v.z += o.z; v.w += o.w;
     }
-    const int64_t pr = t.perm0 + r;
-    if (p.splits == 1)
-      *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(p.s) + pr * RS + 16 * j + 4 * lq) = lr_scaled<DT>(v, ad.scale, 16 * j + 4 * lq, ad.rank);
-    else
-      *reinterpret_cast<float4*>(reinterpret_cast<float*>(p.s) + ((int64_t)blockIdx.y * p.rows + pr) * RS + 16 * j + 4 * lq) = v;
+    return v;
+  };
+  if (p.splits > 1) {
+    for (int i = wave; i < 2 * RJ; i += 4) {
+      const int g = i / RJ, j = i % RJ, r = row0 + 16 * g + l16;
+      if (16 * j >= ad.rank8() || r >= t.rows) continue;
+      *reinterpret_cast<float4*>(reinterpret_cast<float*>(p.s) + ((int64_t)blockIdx.y * p.rows + t.perm0 + r) * RS + 16 * j + 4 * lq) = total(i);
+    }
+    return;
+  }
+  // f16: the largest value of each row first, block by block
+  __shared__ float largest[2 * RJ][16];
+  constexpr int PER = (2 * RJ + 3) / 4;
+  float4 v[PER];
+#pragma unroll
+  for (int n = 0; n < PER; ++n) {
+    const int i = wave + 4 * n, j = i % RJ;
+    if (i >= 2 * RJ || 16 * j >= ad.rank8()) continue;
+    v[n] = lr_within(total(i), 16 * j + 4 * lq, ad.rank);
+    if constexpr (DT == TD_F16) {
+      float m = lr_largest(v[n]);
+      m = fmaxf(m, __shfl_xor(m, 16, 64));
+      m = fmaxf(m, __shfl_xor(m, 32, 64));
+      if (lq == 0) largest[i][l16] = m;
+    }
+  }
+  if constexpr (DT == TD_F16) __syncthreads();
+#pragma unroll
+  for (int n = 0; n < PER; ++n) {
+    const int i = wave + 4 * n, g = i / RJ, j = i % RJ, r = row0 + 16 * g + l16;
+    if (i >= 2 * RJ || 16 * j >= ad.rank8() || r >= t.rows) continue;
+    int shift = 0;
+    if constexpr (DT == TD_F16) {
+      float m = largest[g * RJ][l16];
+#pragma unroll
+      for (int k = 1; k < RJ; ++k)
+        if (16 * k < ad.rank8()) m = fmaxf(m, largest[g * RJ + k][l16]);
+      shift = lr_shift<DT>(m);
+      if (j == 0 && lq == 0) p.back[t.perm0 + r] = lr_power(-shift);
+    }
+    *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(p.s) + (t.perm0 + r) * (int64_t)RS + 16 * j + 4 * lq) = lr_round<DT>(v[n], shift);
   }
 }
 
 // 64 columns from n of the tile's rows, ranks [0, 32 NK): B stays in registers, y and S of the next 16 rows are on their way
-// while these multiply.  sb / srs: the tile's S (16-bit, scaled) and its row stride; prow: its rows' numbers (LDS); turn: the
-// wave's own 16 x 64 floats of LDS.
+// while these multiply.  sb / srs: the tile's S (16-bit) and its row stride; prow: its rows' numbers, back: f16, what brings their
+// updates back (both LDS); turn: the wave's own 16 x 64 floats of LDS.
 template <int DT, int NK>
-__device__ __forceinline__ void lr_expand(const LoraParams& p, const uint16_t* sb, int srs, const int32_t* prow, int rows, const uint16_t* bp,
-                                          int rank8, int64_t n, int l16, int lq, float* turn) {
+__device__ __forceinline__ void lr_expand(const LoraParams& p, const uint16_t* sb, int srs, const int32_t* prow, const float* back, int rows,
+                                          const uint16_t* bp, int rank8, float scale, int64_t n, int l16, int lq, float* turn) {
   v4i bf[2][2][NK];
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
@@ -231,10 +282,12 @@ __device__ __forceinline__ void lr_expand(const LoraParams& p, const uint16_t* s
   uint4 yv[2];
   v4i sf[NK];
   int64_t row[2];
+  float bk[2] = {1.f, 1.f};
   auto load = [&](int g) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       row[i] = prow[min(g + 8 * i + lr, rows - 1)];
+      if constexpr (DT == TD_F16) bk[i] = back[min(g + 8 * i + lr, rows - 1)];
       yv[i] = *reinterpret_cast<const uint4*>(yb + row[i] * p.ldy);
     }
 #pragma unroll
@@ -258,6 +311,7 @@ __device__ __forceinline__ void lr_expand(const LoraParams& p, const uint16_t* s
     __builtin_amdgcn_wave_barrier();
     const uint4 v[2] = {yv[0], yv[1]};
     const int64_t r[2] = {row[0], row[1]};
+    const float b[2] = {bk[0], bk[1]};
     if (g + 16 < rows) load(g + 16);
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
@@ -266,7 +320,10 @@ __device__ __forceinline__ void lr_expand(const LoraParams& p, const uint16_t* s
       const v4f* d = reinterpret_cast<const v4f*>(turn + (8 * i + lr) * LR_TURN + 8 * (threadIdx.x & 7));
       const v4f d0 = d[0], d1 = d[1];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) { f[e] += d0[e]; f[4 + e] += d1[e]; }
+      for (int e = 0; e < 4; ++e) {        // two factors: their product alone may be past fp32
+        f[e] = fmaf(DT == TD_F16 ? d0[e] * b[i] : d0[e], scale, f[e]);
+        f[4 + e] = fmaf(DT == TD_F16 ? d1[e] * b[i] : d1[e], scale, f[4 + e]);
+      }
       if (cin && g + 8 * i + lr < rows) *reinterpret_cast<uint4*>(ob + r[i] * p.ldo) = pack8<DT>(f);
     }
   }
@@ -281,6 +338,7 @@ __global__ __launch_bounds__(256, RJ <= 8 ? 2 : 1) void lora_expand_kernel(const
   const int64_t n = (int64_t)blockIdx.y * 256 + 64 * wave;
   __shared__ int32_t prow[LR_WIDE];
   __shared__ __attribute__((aligned(16))) float turn[4][16 * LR_TURN];
+  __shared__ float back[DT == TD_F16 ? LR_WIDE : 1];
   if (threadIdx.x < t.rows) prow[threadIdx.x] = p.perm[t.perm0 + threadIdx.x];
   if (t.adapter < 0) {            // rows without an adapter: copy
     __syncthreads();
@@ -294,26 +352,37 @@ __global__ __launch_bounds__(256, RJ <= 8 ? 2 : 1) void lora_expand_kernel(const
   const uint16_t* sb = reinterpret_cast<const uint16_t*>(p.s) + (int64_t)t.perm0 * RS;
   int srs = RS;
   __shared__ __attribute__((aligned(16))) uint16_t ssum[LR_NARROW * (RS + 8)];
-  if (p.splits > 1) {             // add the parts of S, scale, round (narrow tiles only)
+  if (p.splits > 1) {             // add the parts of S, round (narrow tiles only); 2^lw neighbouring lanes take a row
     const float* sp = reinterpret_cast<const float*>(p.s) + (int64_t)t.perm0 * RS;
-    const int quads = ad.rank8() / 4;
-    for (int i = threadIdx.x; i < t.rows * quads; i += 256) {
-      const int r = i / quads, c = 4 * (i - r * quads);
+    const int quads = ad.rank8() / 4, lw = 32 - __builtin_clz(quads - 1), q = threadIdx.x & ((1 << lw) - 1), c = 4 * q;
+    for (int r = threadIdx.x >> lw; r < t.rows; r += 256 >> lw) {
       float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (q < quads) {
 #pragma unroll 8
-      for (int s = 0; s < p.splits; ++s) {
-        const float4 o = *reinterpret_cast<const float4*>(sp + (s * p.rows + r) * RS + c);
-        v.x += o.x; v.y += o.y; v.z += o.z; v.w += o.w;
+        for (int s = 0; s < p.splits; ++s) {
+          const float4 o = *reinterpret_cast<const float4*>(sp + (s * p.rows + r) * RS + c);
+          v.x += o.x; v.y += o.y; v.z += o.z; v.w += o.w;
+        }
+        v = lr_within(v, c, ad.rank);
       }
-      *reinterpret_cast<uint2*>(ssum + r * (RS + 8) + c) = lr_scaled<DT>(v, ad.scale, c, ad.rank);
+      int shift = 0;
+      if constexpr (DT == TD_F16) {
+        float m = lr_largest(v);
+        for (int o = (1 << lw) / 2; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+        shift = lr_shift<DT>(m);
+        if (q == 0) back[r] = lr_power(-shift);
+      }
+      if (q < quads) *reinterpret_cast<uint2*>(ssum + r * (RS + 8) + c) = lr_round<DT>(v, shift);
     }
     sb = ssum;
     srs = RS + 8;
+  } else if (DT == TD_F16 && threadIdx.x < t.rows) {
+    back[threadIdx.x] = p.back[t.perm0 + threadIdx.x];
   }
   __syncthreads();
   if (n >= p.N) return;
   const uint16_t* bp = p.bank + ad.b_off + lane * 8;
-#define LR_EXPAND(NK_) lr_expand<DT, NK_>(p, sb, srs, prow, t.rows, bp, ad.rank8(), n, l16, lq, turn[wave])
+#define LR_EXPAND(NK_) lr_expand<DT, NK_>(p, sb, srs, prow, back, t.rows, bp, ad.rank8(), ad.scale, n, l16, lq, turn[wave])
   if (ad.rank8() <= 32) LR_EXPAND(1);
   else if constexpr (KK > 1) {
     if (ad.rank8() <= 64) LR_EXPAND(2);
@@ -339,6 +408,7 @@ __global__ __launch_bounds__(512) void lora_few_kernel(const LoraParams p) {
   __shared__ __attribute__((aligned(16))) char smem[RED > W * 4096 ? RED : W * 4096];
   __shared__ __attribute__((aligned(16))) uint16_t ssum[LR_NARROW * (RS + 8)];
   __shared__ int32_t prow[LR_NARROW];
+  __shared__ float back[LR_NARROW], largest[2 * RJ][16];
   if ((int)threadIdx.x < t.rows) prow[threadIdx.x] = p.perm[t.perm0 + threadIdx.x];
   __syncthreads();
   if (t.adapter < 0) {            // rows without an adapter: copy
@@ -374,15 +444,34 @@ __global__ __launch_bounds__(512) void lora_few_kernel(const LoraParams p) {
 #pragma unroll
       for (int j = 0; j < RJ; ++j) red[wave][g * RJ + j][lane] = make_float4(acc[g][j][0], acc[g][j][1], acc[g][j][2], acc[g][j][3]);
     __syncthreads();
+    const int g = wave / RJ, j = wave % RJ, r = 16 * g + l16;
+    float4 v;
     if (wave < 2 * RJ) {
-      const int g = wave / RJ, j = wave % RJ, r = 16 * g + l16;
-      float4 v = red[0][wave][lane];
+      v = red[0][wave][lane];
 #pragma unroll
       for (int w = 1; w < W; ++w) {
         const float4 o = red[w][wave][lane];
         v.x += o.x; v.y += o.y; v.z += o.z; v.w += o.w;
       }
-      *reinterpret_cast<uint2*>(ssum + r * (RS + 8) + 16 * j + 4 * lq) = lr_scaled<DT>(v, ad.scale, 16 * j + 4 * lq, ad.rank);
+      v = lr_within(v, 16 * j + 4 * lq, ad.rank);
+      if constexpr (DT == TD_F16) {
+        float m = lr_largest(v);
+        m = fmaxf(m, __shfl_xor(m, 16, 64));
+        m = fmaxf(m, __shfl_xor(m, 32, 64));
+        if (lq == 0) largest[wave][l16] = m;
+      }
+    }
+    if constexpr (DT == TD_F16) __syncthreads();
+    if (wave < 2 * RJ) {
+      int shift = 0;
+      if constexpr (DT == TD_F16) {
+        float m = largest[g * RJ][l16];
+#pragma unroll
+        for (int k = 1; k < RJ; ++k) m = fmaxf(m, largest[g * RJ + k][l16]);
+        shift = lr_shift<DT>(m);
+        if (j == 0 && lq == 0) back[r] = lr_power(-shift);
+      }
+      *reinterpret_cast<uint2*>(ssum + r * (RS + 8) + 16 * j + 4 * lq) = lr_round<DT>(v, shift);
     }
     __syncthreads();
   }
@@ -390,7 +479,7 @@ __global__ __launch_bounds__(512) void lora_few_kernel(const LoraParams p) {
   if (wave >= 4 || n >= p.N) return;
   const uint16_t* bp = p.bank + ad.b_off + lane * 8;
   float* const turn = reinterpret_cast<float*>(smem) + wave * 16 * LR_TURN;
-#define LR_EXPAND(NK_) lr_expand<DT, NK_>(p, ssum, RS + 8, prow, t.rows, bp, ad.rank8(), n, l16, lq, turn)
+#define LR_EXPAND(NK_) lr_expand<DT, NK_>(p, ssum, RS + 8, prow, back, t.rows, bp, ad.rank8(), ad.scale, n, l16, lq, turn)
   if (ad.rank8() <= 32) LR_EXPAND(1);
   else if constexpr (KK > 1) LR_EXPAND(2);
 #undef LR_EXPAND
@@ -456,7 +545,7 @@ extern "C" int td_lora_workspace(const int64_t* counts, int64_t k, int64_t n, in
   TD_REQUIRE(counts && floats && k > 0 && n > 0 && max_rank > 0 && max_rank <= LR_MAX_RANK, TD_ERR_INVALID, "td_lora_workspace: k = %lld, rank %d",
              (long long)k, max_rank);
   const LoraShape s = lora_shape(counts, k, n, max_rank);
-  *floats = s.few ? 0 : (int64_t)s.splits * counts[3] * 16 * s.rj / (s.splits == 1 ? 2 : 1);
+  *floats = s.few ? 0 : s.splits == 1 ? counts[3] * (8 * s.rj + 1) : s.splits * counts[3] * 16 * s.rj;       // 16-bit S and a factor a row; parts of S
   return TD_OK;
 }
 
@@ -499,6 +588,7 @@ extern "C" int td_lora_add(const void* x, int64_t ldx, const void* y, int64_t ld
   p.tiles = reinterpret_cast<const LoraTile*>(table);
   p.perm = table + 4 * (counts[0] + counts[1]);
   p.s = ws; p.rows = counts[3]; p.K = k; p.N = n;
+  p.back = ws ? ws + counts[3] * 8 * sh.rj : nullptr;
   p.splits = sh.splits; p.chunks = sh.chunks;
   const int64_t tiles = counts[0] + (out == y ? 0 : counts[1]);
   if (tiles == 0) return TD_OK;

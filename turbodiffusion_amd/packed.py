@@ -331,8 +331,8 @@ def lora_add(y, x, bank, plan, out=None):
     """y [rows, n] + the adapters' updates of x [rows, k] (row stride: any multiple of 8 elements) -> [rows, n]: row r of a request
     with adapter i becomes y[r] + scale_i * (x[r] A_i^T) B_i^T, one without stays y[r].  ``y`` is the output of the projection that
     all requests share (``int8_linear``, ``Int8Linear``, a 16-bit GEMM).  ``out``: written instead of a new tensor; ``out=y`` adds
-    in place; any other overlap is refused.  x A^T is summed in fp32 and, scaled, rounded once to the adapters' type; the update
-    is added in fp32 and rounded with the result.  Any stream, capturable; bank and plan must outlive a captured graph."""
+    in place; any other overlap is refused.  x A^T is summed in fp32 and rounded once to the adapters' type (f16: each row times a power
+    of two, undone in fp32, so that its size does not matter); scale and sum are fp32, rounded with the result.  Any stream, capturable; bank and plan must outlive a captured graph."""
     dev = plan.device
     _check_tensors("lora_add", dev, y, x, out, bank.data)
     key = (_layout(y), _layout(x), _layout(out), bank.layout)
