@@ -31,7 +31,7 @@ from __future__ import annotations
 import torch
 import torch.nn.functional as F
 
-from .packed import AdapterBank, AdapterPlan, AttentionPlan, distance_buckets, lora_add, packed_attention, relative_bias
+from .packed import AdapterBank, AdapterPlan, AttentionPlan, _lengths, distance_buckets, lora_add, packed_attention, relative_bias
 
 
 def _fp16_clamp(x):
@@ -168,18 +168,25 @@ class Umt5Encoder:
         plan = AttentionPlan(lens, heads=H, head_dim=c, device=self.device)
         if plan.tokens == 0:
             return [torch.empty(0, self.dim, dtype=self.dtype, device=self.device) for _ in lens]
-        rows = None
+        rows = {}                       # plans by the rows' places in a bank: projections that the same adapters change share one
         if adapters is not None:
+            adapter_ids = _lengths(adapter_ids, "encode_packed adapter_ids")
             adapters.check(self, adapter_ids)
-            rows = AdapterPlan(lens, adapter_ids, device=self.device)
         if self._distance_bias is None:
             tables = [self.pos] if self.shared_pos else [lay["pos"] for lay in self.layers]
             self._distance_bias = [relative_bias(t, self.max_dist) for t in tables]
             torch.cuda.current_stream(self.device).synchronize()                                 # complete for every later stream
 
         def adapt(y, x, layer, target):     # in place
-            bank = None if rows is None else adapters.banks[layer].get(target)
-            return y if bank is None else lora_add(y, x, bank, rows, out=y)
+            bank, place = (None, None) if adapters is None else adapters.banks[layer].get(target, (None, None))
+            if bank is None:
+                return y
+            at = tuple(-1 if j < 0 else place[j] for j in adapter_ids)
+            if max(at) < 0:
+                return y
+            if at not in rows:
+                rows[at] = AdapterPlan(lens, at, device=self.device)
+            return lora_add(y, x, bank, rows[at], out=y)
 
         flat = torch.cat([p.to(self.device) for p in ids])
         if int(flat.min()) < 0 or int(flat.max()) >= self.emb.shape[0]:
@@ -187,12 +194,15 @@ class Umt5Encoder:
         x = F.embedding(flat, self.emb)                                                          # gather (plumbing)
         for i, lay in enumerate(self.layers):
             h = K.t5_norm(x, lay["n1"], self.eps)
-            qkv = adapt(K.gemm_bf16(h, lay["qkv"]), h, i, "qkv").view(-1, 3, H, c)
+            qkv = K.gemm_bf16(h, lay["qkv"])
+            for t, y in zip(("attn.q", "attn.k", "attn.v"), qkv.split(self.dim_attn, 1)):
+                adapt(y, h, i, t)
+            qkv = qkv.view(-1, 3, H, c)
             o = packed_attention(qkv[:, 0], qkv[:, 1], qkv[:, 2], plan, scale=1.0,               # no 1/sqrt(d) (umt5.py:183)
                                  bias=self._distance_bias[0 if self.shared_pos else i]).view(-1, H * c)
-            x = _fp16_clamp(adapt(K.gemm_bf16(o, lay["o"], res=x), o, i, "o"))
+            x = _fp16_clamp(adapt(K.gemm_bf16(o, lay["o"], res=x), o, i, "attn.o"))
             h = K.gemm_bf16(K.t5_norm(x, lay["n2"], self.eps), lay["gf"], epilogue="geglu")
-            x = _fp16_clamp(adapt(K.gemm_bf16(h, lay["fc2"], res=x), h, i, "fc2"))
+            x = _fp16_clamp(adapt(K.gemm_bf16(h, lay["fc2"], res=x), h, i, "ffn.fc2"))
         return list(K.t5_norm(x, self.final_norm, self.eps).split(lens))
 
     @torch.no_grad()
@@ -214,9 +224,10 @@ class Umt5Encoder:
 
 class Umt5Adapters:
     """Low-rank adapters of many requests for one ``Umt5Encoder``: ``adapters[j]`` = {"blocks.0.attn.q": (A [rank, in], B [out, rank]),
-    ...} over attn.q / attn.k / attn.v / attn.o / ffn.fc2 of any blocks, ``scales[j]`` (default 1) multiplies its updates.  The q, k
-    and v pairs of a block become one pair of the fused projection (ranks side by side, B block by block).  ffn.gate / ffn.fc1 have
-    none: their activation rides in the projection's epilogue, in front of which an update would have to land."""
+    ...} over attn.q / attn.k / attn.v / attn.o / ffn.fc2 of any blocks, each of any rank that ``AdapterBank`` takes; ``scales[j]``
+    (default 1) multiplies its updates.  Every projection of a block has a bank of the pairs that name it (q, k and v update their
+    columns of the fused projection); rows whose adapter does not are not touched there.  ffn.gate / ffn.fc1 have none: their
+    activation rides in the projection's epilogue, in front of which an update would have to land."""
 
     TARGETS = ("attn.q", "attn.k", "attn.v", "attn.o", "ffn.fc2")
 
@@ -235,27 +246,18 @@ class Umt5Adapters:
                 if a.dim() != 2 or b.dim() != 2 or a.shape[1] != inp or b.shape != (out, a.shape[0]):
                     raise ValueError(f"Umt5Adapters: adapter {j}, {name}: {tuple(a.shape)} / {tuple(b.shape)}, wanted [rank, {inp}] / [{out}, rank]")
 
-        def pair(j, i, targets, width):
-            a, b, row = [], [], 0
-            for t in targets:
-                ab = adapters[j].get(f"blocks.{i}.{t}")
-                out, inp = shape[t]
-                if ab is not None:
-                    a.append(ab[0].to(dev, dt))
-                    wide = torch.zeros(width, ab[0].shape[0], dtype=dt, device=dev)
-                    wide[row:row + out] = ab[1].to(dev, dt)
-                    b.append(wide)
-                row += out
-            if not a:      # this adapter leaves the projection alone: an update of zero
-                return torch.zeros(1, shape[targets[0]][1], dtype=dt, device=dev), torch.zeros(width, 1, dtype=dt, device=dev)
-            return torch.cat(a), torch.cat(b, 1)
-
-        self.banks = []
+        scales = [1.0] * self.n if scales is None else list(scales)
+        if len(scales) != self.n:
+            raise ValueError(f"Umt5Adapters: {self.n} adapters, {len(scales)} scales")
+        self.banks = []         # per block: target -> (bank, each adapter's place in it or -1)
         for i in range(len(encoder.layers)):
             banks = {}
-            for key, targets, width in (("qkv", ("attn.q", "attn.k", "attn.v"), 3 * da), ("o", ("attn.o",), dim), ("fc2", ("ffn.fc2",), dim)):
-                if any(f"blocks.{i}.{t}" in ad for ad in adapters for t in targets):
-                    banks[key] = AdapterBank([pair(j, i, targets, width) for j in range(self.n)], scales, device=dev)
+            for t in self.TARGETS:
+                name = f"blocks.{i}.{t}"
+                mine = [j for j in range(self.n) if name in adapters[j]]
+                if mine:
+                    pairs = [tuple(m.to(dev, dt) for m in adapters[j][name]) for j in mine]
+                    banks[t] = (AdapterBank(pairs, [scales[j] for j in mine], device=dev), [mine.index(j) if j in mine else -1 for j in range(self.n)])
             self.banks.append(banks)
 
     def check(self, encoder, adapter_ids):
