@@ -103,3 +103,19 @@ def test_infinities_are_the_formulas(rank, rows, k):
     ref, tol = formula(y, x, a, b, 1.0)
     o = ops.lora_add(y, x, ops.AdapterBank([(a, b)]), ops.AdapterPlan([rows], [0]))
     check(o[[0, 1] + list(range(3, rows))], ref[[0, 1] + list(range(3, rows))], tol[[0, 1] + list(range(3, rows))])
+
+
+@pytest.mark.parametrize("rows,k", SIZES)
+def test_columns_of_one_buffer(rows, k):
+    """x, y and out as column ranges of one buffer; in place beside x"""
+    y, x, a, b = make(rows, k, 16, torch.bfloat16, seed=9)
+    bank, plan = ops.AdapterBank([(a, b)]), ops.AdapterPlan([rows], [0])
+    want = ops.lora_add(y, x, bank, plan)
+    buf = torch.cat([y, x, torch.zeros_like(y)], 1)
+    y_, x_, out = buf.split([64, k, 64], 1)
+    assert ops.lora_add(y_, x_, bank, plan, out=out) is out
+    assert torch.equal(out, want) and torch.equal(y_, y) and torch.equal(x_, x)
+    assert torch.equal(ops.lora_add(y_, x_, bank, plan, out=y_), want) and torch.equal(x_, x)
+    for bad in (buf[:, 64:128], buf[:, 8:72]):
+        with pytest.raises(ValueError):
+            ops.lora_add(y_, x_, bank, plan, out=bad)

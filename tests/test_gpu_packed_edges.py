@@ -161,3 +161,19 @@ def test_order_of_the_largest_biases(D, path, past, here):
     ref, _ = formula(q, k, v, lens, lens_k, False, 1.0, bias, exact_scores=True)
     u = torch.finfo(torch.bfloat16).eps / 2
     check(ops.packed_attention(q, k, v, plan, scale=1.0, bias=bias), ref, torch.full_like(ref, (u + 2.0 ** -18) * v.double().abs().max()))       # u A
+
+
+@pytest.mark.parametrize("heads", [(4, 4), (4, 2)])
+def test_out_between_the_heads_of_a_fused_buffer(heads):
+    """q | k | v | room for o in one buffer: out interleaves with every input and touches none"""
+    H, Hkv = heads
+    lens = [70, 1, 130]
+    buf = torch.randn(201, 2 * H + 2 * Hkv, 128, device="cuda").to(torch.bfloat16)
+    q, k, v, out = buf.split([H, Hkv, Hkv, H], 1)
+    plan = ops.AttentionPlan(lens, heads=H, kv_heads=Hkv, head_dim=128, causal=True)
+    want, before = ops.packed_attention(q, k, v, plan), buf.clone()
+    assert ops.packed_attention(q, k, v, plan, out=out) is out
+    assert torch.equal(out, want) and torch.equal(buf[:, :-H], before[:, :-H])
+    for bad in (buf[:, 1:1 + H], buf[:, -H - 1:-1]):
+        with pytest.raises(ValueError):
+            ops.packed_attention(q, k, v, plan, out=bad)

@@ -1,0 +1,52 @@
+"""Host side of the packed operators: checks of arguments that need no GPU."""
+import random
+
+import pytest
+import torch
+
+from turbodiffusion_amd import packed
+
+
+def shared(a, b):
+    """from the elements' addresses"""
+    def where(t):
+        at = torch.zeros(t.shape, dtype=torch.int64)
+        for d, (n, st) in enumerate(zip(t.shape, t.stride())):
+            at += (torch.arange(n) * st * t.element_size()).view([-1 if i == d else 1 for i in range(t.dim())])
+        return {t.data_ptr() + x + i for x in at.flatten().tolist() for i in range(t.element_size())}
+    return bool(where(a) & where(b))
+
+
+def test_overlap_of_slices_of_one_buffer():
+    buf = torch.zeros(12, 10, 24, dtype=torch.bfloat16)
+    assert not packed._overlap(buf[:, :4], buf[:, 4:8])                   # heads of a fused projection
+    assert not packed._overlap(buf[:, :4], buf[:, 4:])
+    assert not packed._overlap(buf[..., :8], buf[..., 8:16])              # columns of every head
+    assert not packed._overlap(buf[1:11, 2:6, :16], buf[1:11, 2:6, 16:])
+    assert not packed._overlap(buf[0::2], buf[1::2])                      # every other row
+    assert not packed._overlap(buf.transpose(0, 1)[:3], buf.transpose(0, 1)[3:])
+    assert not packed._overlap(buf[:6], buf[6:])
+    assert not packed._overlap(buf[:0], buf)
+    flat = buf.view(12, 240)
+    assert not packed._overlap(flat[:, :64], flat[:, 64:128])
+    assert packed._overlap(flat[:, :64], flat[:, 63:128])
+    assert packed._overlap(buf, buf) and packed._overlap(buf[:, :4], buf[:, 3:8]) and packed._overlap(buf[:7], buf[6:])
+    assert packed._overlap(buf[..., :16], buf[..., 8:])
+    assert packed._overlap(buf[3:4, 2:3, :1].expand(5, 4, 8), buf)
+
+
+def test_overlap_is_never_missed():
+    rng, found = random.Random(0), [0, 0]
+    buf = torch.zeros(1000, dtype=torch.float16)
+    for _ in range(4000):
+        ts = []
+        for _ in range(2):
+            size = [rng.choice([1, 1, 2, 3, 4]) for _ in range(rng.choice([2, 3]))]
+            stride = [rng.choice([0, 1, 2, 4, 8, 12, 24, 30, 48, 96]) for _ in size]
+            ts.append(torch.as_strided(buf, size, stride, rng.randrange(100)))
+        if shared(*ts):
+            found[0] += 1
+            assert packed._overlap(*ts)
+        else:
+            found[1] += not packed._overlap(*ts)
+    assert min(found) > 500

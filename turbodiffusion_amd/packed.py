@@ -85,12 +85,22 @@ def _check_tensors(what, dev, *tensors):
 
 
 def _overlap(a, b):
-    """whether the memory ranges of two tensors intersect"""
-    def span(t):
-        n = sum((s - 1) * st for s, st in zip(t.shape, t.stride())) + 1 if t.numel() else 0
-        return t.data_ptr(), t.data_ptr() + n * t.element_size()
-    (a0, a1), (b0, b1) = span(a), span(b)
-    return a0 < b1 and b0 < a1
+    """whether two tensors may share memory.  Their ranges may intersect without it: column ranges of one buffer, heads of a fused
+    projection.  Seen modulo a stride of either, a tensor is one interval if the strides that are no multiples of it fit into one period;
+    two intervals apart there are apart everywhere."""
+    if a.numel() == 0 or b.numel() == 0:
+        return False
+    dims = [[(n, st * t.element_size()) for n, st in zip(t.shape, t.stride()) if n > 1] for t in (a, b)]
+    at = a.data_ptr(), b.data_ptr()
+    size = [sum((n - 1) * st for n, st in d) + t.element_size() for d, t in zip(dims, (a, b))]
+    if at[0] + size[0] <= at[1] or at[1] + size[1] <= at[0]:
+        return False
+    for period in {st for d in dims for _, st in d if st}:
+        wa, wb = (sum((n - 1) * st for n, st in d if st % period) + t.element_size() for d, t in zip(dims, (a, b)))
+        gap = (at[1] - at[0]) % period               # from the beginning of a's interval to that of b's, and on to a's next
+        if wa <= gap and wb <= period - gap:
+            return False
+    return True
 
 
 class AttentionPlan(_Plan):
@@ -339,7 +349,7 @@ def lora_add(y, x, bank, plan, out=None):
     ldy, ldx, ldo, floats, dt = plan._admitted.get(key) or plan._admit(key, _lora_layout(y, x, bank, plan, out))
     if out is None:
         out = y.new_empty((plan.rows, bank.n))
-    elif _overlap(out, x) or (_overlap(out, y) and (out.data_ptr() != y.data_ptr() or ldo != ldy)):
+    elif _overlap(out, x) or ((out.data_ptr() != y.data_ptr() or ldo != ldy) and _overlap(out, y)):
         raise ValueError("lora_add: out overlaps an input (out=y alone may)")
     if plan.rows == 0:
         return out
