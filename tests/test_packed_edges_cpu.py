@@ -43,10 +43,10 @@ def test_overlap_is_never_missed():
         for _ in range(2):
             size = [rng.choice([1, 1, 2, 3, 4]) for _ in range(rng.choice([2, 3]))]
             stride = [rng.choice([0, 1, 2, 4, 8, 12, 24, 30, 48, 96]) for _ in size]
-            ts.append(torch.as_strided(buf, size, stride, rng.randrange(100)))
+            ts.append(torch.as_strided(buf, size, stride, rng.randrange(24)))
         if shared(*ts):
             found[0] += 1
             assert packed._overlap(*ts)
         else:
             found[1] += not packed._overlap(*ts)
-    assert min(found) > 500
+    assert min(found) > 250
