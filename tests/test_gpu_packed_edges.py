@@ -177,3 +177,37 @@ def test_out_between_the_heads_of_a_fused_buffer(heads):
     for bad in (buf[:, 1:1 + H], buf[:, -H - 1:-1]):
         with pytest.raises(ValueError):
             ops.packed_attention(q, k, v, plan, out=bad)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("G", [1, 2, 5])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("layout", ["plain", "padded", "heads"])
+def test_some_tokens_behind_long_pasts(dtype, D, G, causal, layout):
+    """up to 32 rows each on the kernel whose waves take different keys: several tokens an item, another end for each under a causal
+    mask, no keys, fewer keys than queries, split ranges"""
+    Hkv = 2
+    H = G * Hkv
+    lens = [min(n, 32 // G) for n in (2, 7, 31, 1, 32, 5, 6, 0, 16)]
+    for lens_k in ([700, 5000, 131, 0, 32, 3, 200, 40, 257], [130, 129, 33, 1, 64, 300, 5, 0, 16]):
+        g = torch.Generator(device="cuda").manual_seed(G)
+
+        def r(t, h):
+            if layout == "heads":
+                return torch.randn(h, t, D, generator=g, device="cuda").to(dtype).transpose(0, 1)
+            wide = torch.randn(t, h + 1, D + 8, generator=g, device="cuda").to(dtype)
+            return wide[:, 1:, :D] if layout == "padded" else wide[:, 1:, :D].contiguous()
+
+        q, k, v = r(sum(lens), H), r(sum(lens_k), Hkv), r(sum(lens_k), Hkv)
+        plan = ops.AttentionPlan(lens, lens_k, heads=H, kv_heads=Hkv, head_dim=D, causal=causal)
+        assert plan._counts[0] == 0 and (plan._counts[2] > 0) == (max(lens_k) > 4000)
+        for R in (None, 0, 20):
+            bias = None if R is None else torch.randn(H, 2 * R + 1, device="cuda")
+            ref, tol = formula(q, k, v, lens, lens_k, causal, D ** -0.5, bias)
+            check(ops.packed_attention(q, k, v, plan, bias=bias), ref, tol)
+        big = torch.full((sum(lens) + 2, H + 1, D + 8), 7.0, dtype=dtype, device="cuda")
+        ops.packed_attention(q, k, v, plan, bias=bias, out=big[1:-1, 1:, :D])
+        check(big[1:-1, 1:, :D], ref, tol)
+        big[1:-1, 1:, :D] = 7.0
+        assert (big == 7.0).all()
