@@ -50,3 +50,11 @@ def test_overlap_is_never_missed():
         else:
             found[1] += not packed._overlap(*ts)
     assert min(found) > 250
+
+
+def test_a_scale_past_fp32_is_refused():
+    """finite as Python holds it, infinite as the kernels do: the update of zero would be NaN"""
+    a, b = torch.zeros(4, 16, dtype=torch.bfloat16), torch.zeros(24, 4, dtype=torch.bfloat16)
+    for scale in (1e39, -1e300, float("inf")):
+        with pytest.raises(ValueError, match="scales must be finite"):
+            packed.AdapterBank([(a, b)], [scale])

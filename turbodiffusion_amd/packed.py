@@ -247,8 +247,8 @@ class AdapterBank:
         scales = [1.0] * len(pairs) if scales is None else [float(s) for s in scales]
         if len(scales) != len(pairs):
             raise ValueError(f"AdapterBank: {len(pairs)} adapters, {len(scales)} scales")
-        if not all(math.isfinite(s) for s in scales):
-            raise ValueError(f"AdapterBank: scales must be finite, got {scales}")
+        if not torch.tensor(scales, dtype=torch.float32).isfinite().all():
+            raise ValueError(f"AdapterBank: scales must be finite in fp32, got {scales}")
         self.dtype = pairs[0][0].dtype
         if self.dtype not in (torch.bfloat16, torch.float16):
             raise TypeError(f"AdapterBank: bf16 or f16 adapters, got {self.dtype}")
