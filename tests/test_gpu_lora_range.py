@@ -119,3 +119,16 @@ def test_columns_of_one_buffer(rows, k):
     for bad in (buf[:, 64:128], buf[:, 8:72]):
         with pytest.raises(ValueError):
             ops.lora_add(y_, x_, bank, plan, out=bad)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("rows,k", [(3, 96), (40, 8224), (8200, 96), (8200, 104)])
+def test_an_infinite_weight(dtype, rows, k):
+    """A infinite in its last columns, where k ends inside a step of 64: infinity as in the formula, not NaN"""
+    y, x, a, b = make(rows, k, 12, dtype, seed=10)
+    x.copy_(x.abs() + 0.5)
+    b.copy_(b.abs() + 0.5)
+    a[3, k - 1] = float("inf")
+    a[3, k - 20] = float("inf")
+    o = ops.lora_add(y, x, ops.AdapterBank([(a, b)]), ops.AdapterPlan([rows], [0]))
+    assert (o == float("inf")).all()

@@ -143,6 +143,7 @@ __device__ __forceinline__ void lr_shrink(v4f (&acc)[2][RJ], const uint16_t* con
     __builtin_amdgcn_wave_barrier();
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
+      if (h && 2 * c + 1 > last) break;           // x is zero there and A another step's, which may be infinite
       const char* f = turn + l16 * 128 + (((4 * h + lq) ^ ((l16 >> 1) & 7)) << 4);
       const v4i x0 = *reinterpret_cast<const v4i*>(f), x1 = *reinterpret_cast<const v4i*>(f + 2048);
 #pragma unroll
