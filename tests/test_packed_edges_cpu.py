@@ -58,3 +58,17 @@ def test_a_scale_past_fp32_is_refused():
     for scale in (1e39, -1e300, float("inf")):
         with pytest.raises(ValueError, match="scales must be finite"):
             packed.AdapterBank([(a, b)], [scale])
+
+
+@pytest.mark.parametrize("kw", [{"heads": 2.5}, {"heads": 4, "kv_heads": 1.5}, {"heads": float("nan")}, {"heads": float("inf")}, {"heads": 1 << 31}])
+def test_numbers_of_heads_are_whole(kw):
+    with pytest.raises(ValueError, match="heads"):
+        packed.AttentionPlan([3], **kw)
+
+
+@pytest.mark.parametrize("n", [float("inf"), float("nan"), 2.5, True])
+def test_lengths_are_whole(n):
+    for make in (lambda: packed.AttentionPlan([3, n], heads=2), lambda: packed.AttentionPlan([3, 4], [4, n], heads=2),
+                 lambda: packed.AdapterPlan([n], [0]), lambda: packed.AdapterPlan([3], [n])):
+        with pytest.raises(ValueError, match="whole numbers"):
+            make()

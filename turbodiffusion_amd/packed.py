@@ -27,7 +27,7 @@ def _lengths(lens, what):
         lens = lens.tolist()
     lens = list(lens)
     for n in lens:
-        if isinstance(n, bool) or int(n) != n:
+        if isinstance(n, bool) or isinstance(n, float) and not math.isfinite(n) or int(n) != n:
             raise ValueError(f"{what}: whole numbers, got {n!r}")
         if not -1 << 63 <= n < 1 << 63:
             raise ValueError(f"{what}: {n} does not fit 64 bits")
@@ -113,8 +113,8 @@ class AttentionPlan(_Plan):
         self.lens_k = self.lens if lens_k is None else _lengths(lens_k, "AttentionPlan lens_k")
         if len(self.lens) != len(self.lens_k):
             raise ValueError(f"AttentionPlan: {len(self.lens)} query and {len(self.lens_k)} key sequences")
-        self.heads, self.kv_heads = int(heads), int(heads if kv_heads is None else kv_heads)
-        if self.heads < 1 or self.kv_heads < 1 or self.heads % self.kv_heads:
+        self.heads, self.kv_heads = _lengths([heads, heads if kv_heads is None else kv_heads], "AttentionPlan heads, kv_heads")
+        if not 1 <= self.heads < 1 << 31 or self.kv_heads < 1 or self.heads % self.kv_heads:
             raise ValueError(f"AttentionPlan: {heads} heads do not share {kv_heads} key heads evenly")
         if head_dim not in (64, 128):
             raise ValueError(f"AttentionPlan: head_dim = {head_dim} (64 or 128)")
