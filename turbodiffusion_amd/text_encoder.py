@@ -159,7 +159,10 @@ class Umt5Encoder:
         ``adapters``: ``Umt5Adapters``; prompt i is encoded with adapter ``adapter_ids[i]`` (-1: with the plain weights)."""
         K, H = self.K, self.num_heads
         c = self.dim_attn // H
-        ids = [torch.as_tensor(p, dtype=torch.long).reshape(-1) for p in prompts]
+        ids = [torch.as_tensor(p).reshape(-1) for p in prompts]
+        if any(p.is_floating_point() and not torch.equal(p, p.trunc()) for p in ids):
+            raise ValueError("encode_packed: token ids must be whole numbers")
+        ids = [p.long() for p in ids]
         lens = [p.numel() for p in ids]
         if (adapters is None) != (adapter_ids is None):
             raise ValueError("encode_packed: adapters and adapter_ids go together")
