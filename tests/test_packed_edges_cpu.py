@@ -1,9 +1,11 @@
 """Host side of the packed operators: checks of arguments that need no GPU."""
+import ctypes
 import random
 
 import pytest
 import torch
 
+from turbodiffusion_amd import _lib as L
 from turbodiffusion_amd import packed
 
 
@@ -72,3 +74,11 @@ def test_lengths_are_whole(n):
                  lambda: packed.AdapterPlan([n], [0]), lambda: packed.AdapterPlan([3], [n])):
         with pytest.raises(ValueError, match="whole numbers"):
             make()
+
+
+def test_rows_of_out_may_not_overlap_at_the_c_entry():
+    """refused before anything is launched (the addresses are not memory)"""
+    counts = (ctypes.c_int64 * 6)(1, 0, 3, 3, 1, 32)
+    for ldo in (0, 56):
+        with pytest.raises(L.TurboDiffusionAMDError, match="overlap"):
+            L.call("td_lora_add", 4096, 64, 8192, 64, 16384, ldo, L.TD_BF16, 64, 64, 4096, 4096, 1, 8, 4096, counts, 4096, None)

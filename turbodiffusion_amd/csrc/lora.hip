@@ -579,6 +579,7 @@ extern "C" int td_lora_add(const void* x, int64_t ldx, const void* y, int64_t ld
   TD_REQUIRE(counts[4] <= num_adapters, TD_ERR_INVALID, "td_lora_add: the plan names adapter %lld of %d", (long long)counts[4] - 1, num_adapters);
   TD_REQUIRE(counts[0] >= 0 && counts[1] >= 0 && counts[0] + counts[1] < (1 << 28), TD_ERR_INVALID, "td_lora_add: counts");
   TD_REQUIRE(counts[5] == LR_WIDE || counts[5] == LR_NARROW, TD_ERR_INVALID, "td_lora_add: counts");
+  TD_REQUIRE(counts[2] <= 1 || ldo >= n, TD_ERR_INVALID, "td_lora_add: the rows of out overlap");
   TD_REQUIRE(out != y || ldo == ldy || counts[2] <= 1, TD_ERR_INVALID, "td_lora_add: out = y with another row stride");
   const LoraShape sh = lora_shape(counts, k, n, max_rank);
   TD_REQUIRE(counts[3] == 0 || sh.few || ws, TD_ERR_INVALID, "td_lora_add: null workspace");
