@@ -511,7 +511,7 @@ int td_sla_linear_kv_final_packed(const float* ws_kv, const float* ws_ks, int nc
  * nothing to attend to is 0.  q, k, v, o: 16-bit (TD_F16 | TD_BF16), head_dim 64 or 128 contiguous; strides[8] = token and
  * head strides of q, k, v, o in elements (multiples of 8; pointers 16-byte aligned).  bias: f32 [heads, 2 bias_range + 1] or NULL; G (2 bias_range + 193) <= 8192.
  * td_attn_packed_plan (host only): the lengths of the sequences -> work table (records of 8 int32; call with table = NULL for
- * counts = {tile items, few-row items, joins, partial rows, query tokens, key tokens}; records = the first three added up).  The
+ * counts = {tile items, few-row items, joins, partial rows, query tokens, key tokens}, one of the first two 0; records = the first three added up).  The
  * table goes to the device unchanged and is valid for every call with these lengths, heads and causality.  td_attn_packed trusts
  * it: q / k / v / o must hold the planned tokens.  ws: f32 [kv_heads * partial rows * (head_dim + 2)] (NULL when that is 0). */
 int td_attn_packed_plan(const int64_t* lens_q, const int64_t* lens_k, int64_t nseq, int heads, int kv_heads, int causal, int32_t* table,

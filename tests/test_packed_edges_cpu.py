@@ -82,3 +82,10 @@ def test_rows_of_out_may_not_overlap_at_the_c_entry():
     for ldo in (0, 56):
         with pytest.raises(L.TurboDiffusionAMDError, match="overlap"):
             L.call("td_lora_add", 4096, 64, 8192, 64, 16384, ldo, L.TD_BF16, 64, 64, 4096, 4096, 1, 8, 4096, counts, 4096, None)
+
+
+def test_a_table_for_both_kernels_is_refused():
+    """a batch is one kernel's; refused before anything is launched"""
+    counts, strides = (ctypes.c_int64 * 6)(1, 1, 0, 0, 2, 2), (ctypes.c_int64 * 8)(*[128, 64] * 4)
+    with pytest.raises(L.TurboDiffusionAMDError, match="counts"):
+        L.call("td_attn_packed", 4096, 8192, 16384, 32768, strides, L.TD_BF16, 2, 2, 64, 1.0, 0, None, 0, 4096, counts, None, None)

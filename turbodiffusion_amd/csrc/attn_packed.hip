@@ -37,7 +37,7 @@ typedef __attribute__((address_space(3))) ap_v4s* ap_trptr_t;
 #define AP_MANY_KEYS 384   // ... this many (128 tokens over 150 keys each 39.9 against 26.1 us, 400: 68.7 against 60.0, 777: 116 against 127)
 #define AP_PAD 96          // the bias table repeats its ends: distances within a key tile of the range need no clamp
 #define AP_TAU 8.0f        // a row's reference moves when a score exceeds it by 8 (a weight of 2^8),
-#define AP_LOOK 4096.0f    // looked for when the 16 (32) weights of a lane in a tile add up to more than this
+#define AP_LOOK 4096.0f    // looked for when a lane's weights of a tile add up to more than this (16; few kernel, D = 64: 32)
 #define AP_STEP 4194304.0f // from here on a reference's own rounding (2^-24 of it) is a matter of weights: 2^22, where that is 2^0.25
 
 // One workgroup's work per key head: `rows` rows from head `head0` of query token `token`, which stands at position `pos` of its
@@ -200,9 +200,9 @@ __device__ __forceinline__ ApScore ap_score(const ApParams& p, const ApItem& it,
 }
 
 // Running state of a wave's rows: weights are exp2(score - ref).  ref is a row's maximum when it was last looked at, not its
-// running maximum: the maximum of a tile is taken only when a lane's weights of it add up to more than 2^12, which one weight of
-// more than 2^8 must have caused (of 60 vector instructions a block 24 less: 32 760 causal tokens 3.06 -> 2.85 ms).  Weights up to 2^12
-// fit f16, bf16 and the fp32 sums.
+// running maximum: the maximum of a tile is taken only when a lane's weights of it add up to more than 2^12 (of 60 vector instructions a
+// block 24 less: 32 760 causal tokens 3.06 -> 2.85 ms).  Of 16 weights one must then be above 2^8, and the row moves; of 32 all may lie
+// between 2^7 and 2^8, and the row is looked at again in the next such tile.  Weights up to 2^12 fit f16, bf16 and the fp32 sums.
 //
 // score = mul * s + base is fused into the exponent, so it is never rounded by itself, while ref is.  Where a score is large (a far tile
 // under a bias of -1e9, products of 1e9) that rounding is many powers of two: a weight against ref could be anything.  Rows whose ref
@@ -698,8 +698,8 @@ __global__ __launch_bounds__(256) void attn_packed_join_kernel(const ApParams p,
 }
 
 // ---- the plan: which workgroup does what (host) --------------------------------------------------------------------
-// Table of 8-word records: tile items, few items, joins (in this order).  counts = {tile items, few items, joins, partial rows,
-// query tokens, key tokens}.
+// Table of 8-word records: items (all for one of the two kernels), then joins.  counts = {tile items, few items, joins, partial rows,
+// query tokens, key tokens}; one of the first two is 0.
 
 // Keys a few workgroup takes.  One has a CU to itself and needs 2.5 us beside its keys; all 256 read 39 keys a us each (D = 128), one
 // alone 150.  W keys in parts of L take W / (39 * 256) + 2.5 W / (256 L) and, while the last ones run without the others, L / 150:
@@ -779,14 +779,16 @@ extern "C" int td_attn_packed_plan(const int64_t* lens_q, const int64_t* lens_k,
         q0 += ql; k0 += kl;
       }
       if (pass == 0) {
-        // 256 CUs, two tile workgroups each.  A key range is split when it is longer than the share of one of these slots; a part is
-        // at least 512 keys, below which writing and joining partials costs more than it saves.
+        // A tile range is cut when it is longer than one of 512 even shares of all keys; a part is at least 512 keys, below which writing
+        // and joining partials costs more than it saves.  The chip holds more workgroups (256 CUs, three or for D = 64 four each), but
+        // shares for 768 (1024) of them are slower, as more partials are written and joined: causal, 10 heads of 128 over 2,
+        // 4000 tokens 65 us against 70 (72), 8000 175 against 190 (185); 40 over 8, 4000 tokens 164 against 180 (188).
         chunk = few ? ap_few_chunk(ranges, total, kv_heads) : std::max<int64_t>(512, td_cdiv(total * kv_heads, 512));
       }
     }
     // longest first: the short ones fill the tail
     std::stable_sort(work.begin(), work.end(), [](const Work& a, const Work& b) { return a.keys > b.keys; });
-    counts[few] = (int64_t)work.size(); counts[!few] = 0; counts[2] = (int64_t)joins.size();
+    counts[few ? 1 : 0] = (int64_t)work.size(); counts[few ? 0 : 1] = 0; counts[2] = (int64_t)joins.size();
     counts[3] = ws_rows; counts[4] = tq; counts[5] = tk;
     const int64_t n = counts[0] + counts[1] + counts[2];
     if (table) {
@@ -829,7 +831,7 @@ extern "C" int td_attn_packed(const void* q, const void* k, const void* v, void*
   TD_REQUIRE(counts[4] <= 1 || strides[6] >= head_dim, TD_ERR_INVALID, "td_attn_packed: the tokens of o overlap");
   TD_REQUIRE(scale > 0.f && scale <= 1e38f, TD_ERR_INVALID, "td_attn_packed: scale must be positive, at most 1e38");
   const int64_t nt = counts[0], nf = counts[1], nj = counts[2], wr = counts[3];
-  TD_REQUIRE(nt >= 0 && nf >= 0 && nj >= 0 && wr >= 0 && (nj == 0 || ws), TD_ERR_INVALID, "td_attn_packed: counts / workspace");
+  TD_REQUIRE(nt >= 0 && nf >= 0 && (nt == 0 || nf == 0) && nj >= 0 && wr >= 0 && (nj == 0 || ws), TD_ERR_INVALID, "td_attn_packed: counts / workspace");
   TD_REQUIRE(counts[5] == 0 || (k && v), TD_ERR_INVALID, "td_attn_packed: null keys or values");
   TD_REQUIRE(nt < (1ll << 31) && nf < (1ll << 31) && nj < (1ll << 31) && kv_heads <= 65535, TD_ERR_UNSUPPORTED,
              "td_attn_packed: too many workgroups");
@@ -852,21 +854,19 @@ extern "C" int td_attn_packed(const void* q, const void* k, const void* v, void*
   p.gmagic = G > 1 ? (uint32_t)(((1ull << 32) + G - 1) / G) : 0;
   p.c = scale * 1.4426950408889634f;
   hipStream_t st = (hipStream_t)stream;
-  for (int few = 0; few < 2; ++few) {
-    const int64_t n = few ? nf : nt;
-    p.items = reinterpret_cast<const ApItem*>(table) + (few ? nt : 0);
-    p.n_items = (int)n;
-    if (n == 0) continue;
+  const int64_t n = nt + nf;
+  p.items = reinterpret_cast<const ApItem*>(table);
+  p.n_items = (int)n;
+  if (n == 0) return TD_OK;
 #define AP_GO2(DT_, D_, F_) { if (bias) ap_launch<DT_, D_, F_, true>(p, n, bias_bytes, st); else ap_launch<DT_, D_, F_, false>(p, n, 0, st); }
-#define AP_GO1(DT_, D_) { if (few) AP_GO2(DT_, D_, true) else AP_GO2(DT_, D_, false) }
-    if (dtype == TD_BF16) { if (head_dim == 64) AP_GO1(TD_BF16, 64) else AP_GO1(TD_BF16, 128) }
-    else { if (head_dim == 64) AP_GO1(TD_F16, 64) else AP_GO1(TD_F16, 128) }
+#define AP_GO1(DT_, D_) { if (nf > 0) AP_GO2(DT_, D_, true) else AP_GO2(DT_, D_, false) }
+  if (dtype == TD_BF16) { if (head_dim == 64) AP_GO1(TD_BF16, 64) else AP_GO1(TD_BF16, 128) }
+  else { if (head_dim == 64) AP_GO1(TD_F16, 64) else AP_GO1(TD_F16, 128) }
 #undef AP_GO1
 #undef AP_GO2
-    TD_CHECK_LAUNCH();
-  }
+  TD_CHECK_LAUNCH();
   if (nj > 0) {
-    const ApJoin* joins = reinterpret_cast<const ApJoin*>(table) + nt + nf;
+    const ApJoin* joins = reinterpret_cast<const ApJoin*>(table) + n;
     const dim3 grid((unsigned)nj, (unsigned)kv_heads, (nt > 0 ? AP_ROWS : AP_FEW) / 4);
     if (dtype == TD_BF16) { if (head_dim == 64) attn_packed_join_kernel<TD_BF16, 64><<<grid, 256, 0, st>>>(p, joins); else attn_packed_join_kernel<TD_BF16, 128><<<grid, 256, 0, st>>>(p, joins); }
     else { if (head_dim == 64) attn_packed_join_kernel<TD_F16, 64><<<grid, 256, 0, st>>>(p, joins); else attn_packed_join_kernel<TD_F16, 128><<<grid, 256, 0, st>>>(p, joins); }
