@@ -132,3 +132,32 @@ def test_an_infinite_weight(dtype, rows, k):
     a[3, k - 20] = float("inf")
     o = ops.lora_add(y, x, ops.AdapterBank([(a, b)]), ops.AdapterPlan([rows], [0]))
     assert (o == float("inf")).all()
+
+
+@pytest.mark.parametrize("rank", [24, 200])
+@pytest.mark.parametrize("rows,k", SIZES)
+def test_f16_on_another_stream_and_in_two_graphs(rank, rows, k):
+    """the rows' powers of two are each call's own"""
+    y, x, a, b = make(rows, k, rank, torch.float16, seed=11)
+    bank, plan = ops.AdapterBank([(a, b)], [3.0]), ops.AdapterPlan([rows], [0])
+    base = ops.lora_add(y, x, bank, plan)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        small = ops.lora_add(y, x * 2.0 ** -9, bank, plan)
+    other = ops.lora_add(y, x, bank, plan)
+    torch.cuda.synchronize()
+    assert torch.equal(other, base) and torch.equal(small, ops.lora_add(y, x * 2.0 ** -9, bank, plan))
+    xs, graphs, outs = [x.clone(), x * 2.0 ** 6], [], []
+    for x_ in xs:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            outs.append(ops.lora_add(y, x_, bank, plan))
+    for i in range(3):
+        for x_ in xs:
+            x_.mul_(0.5)
+        want = [ops.lora_add(y, x_, bank, plan) for x_ in xs]
+        for g in graphs:
+            g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(o, w) for o, w in zip(outs, want))
