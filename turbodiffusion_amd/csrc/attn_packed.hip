@@ -300,11 +300,11 @@ __device__ __forceinline__ void ap_tile(const ApScore& score, const char* sk, co
 }
 
 // ---- 128 rows, 32 per wave; key tiles of 32 shared by the waves, two LDS stages, one barrier a tile ----
-// What bounds it.  Long ranges: the matrix pipe at the clock that the power limit leaves (causal, 32 760 tokens, 12 heads of 128: 2.85
-// ms, 1.16 PFLOP/s, 0.84 of a large library product on the same card; with the softmax arithmetic taken out 2.72 ms).  Short
+// What bounds it.  Long ranges: the matrix pipe at the clock that the power limit leaves (causal, 32 760 tokens, 12 heads of 128: 2.79
+// to 2.86 ms, 1.15 to 1.18 PFLOP/s, 0.84 of a large library product on the same card; with the softmax arithmetic taken out 2.72 ms).  Short
 // ranges: the latency of a workgroup's first loads and the vector instructions around the loop.  Hence tiles of 32 keys - three
 // (D = 64: four) workgroups a CU instead of two: 226 keys under 50 960 rows of 12 heads 91 us (94 against 100 when tried), prompts
-// of 1 to 512 tokens, 64 heads of 64, 34.8 (35.3 against 36.7), the long range 1 % slower - and pointers that step instead of
+// of 1 to 512 tokens, 64 heads of 64, 35.2 (35.3 against 36.7 when tried), the long range 1 % slower - and pointers that step instead of
 // addresses computed row by row (1250 -> 950 vector instructions a wave at 226 keys, 107 -> 100 us).
 template <int DT, int D, bool BIAS>
 __global__ __launch_bounds__(256, D == 128 ? 3 : 4) void attn_packed_tile_kernel(const ApParams p) {
@@ -490,7 +490,7 @@ __device__ __forceinline__ void ap_read_v(const uint32_t (&a)[4], v4i (&vf)[8]) 
 }
 
 // ---- up to 32 rows; the waves take different keys, each with a K and a V stage of its own, and join at the end ----
-// What bounds it: memory, K and V once: 16 sequences of up to 32 760 keys, 40 heads of 128 over 8 key heads, 702 MB in 134 us, 5.2
+// What bounds it: memory, K and V once: 16 sequences of up to 32 760 keys, 40 heads of 128 over 8 key heads, 702 MB in 135 us, 5.2
 // TB/s (a large copy moves 4.9).  One workgroup a CU with up to 128 KB in flight; 32 rows of the MFMA for G = 5 valid ones cost nothing
 // beside that.  A wave fetches its next K tile once this one is in registers and its next V tile likewise, so that 16 KB hold what
 // two stages did and eight waves fit where four did: a range of 777 keys of 12 heads 8.7 against 11.4 us.

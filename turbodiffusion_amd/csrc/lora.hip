@@ -16,8 +16,8 @@
 //
 // What bounds it: memory; y and out dominate, then x, at 2 rank flops per byte.  MFMA fragments want 64 bytes from each of 16 rows;
 // memory wants whole 128-byte lines, so x, y and out pass through LDS on their way (50 960 rows, 1536 -> 8960, ranks 128 and 64:
-// expand 506 -> 419 us, 4.4 TB/s, shrink 85 -> 65 us; 32 760 rows, 5120 -> 5120, rank 32: 162 -> 122 us, 5.5 TB/s, and 103 -> 98, where
-// shrink also waits for the previous pass's writes).  A large copy moves 4.9 TB/s.  With B_i read again for every 64 rows expand
+// expand 506 -> 419 us, 4.4 TB/s, shrink 85 -> 65 us, 423 and 70 with f16's powers of two, both 452 -> 455 in a graph; 32 760 rows,
+// 5120 -> 5120, rank 32: 162 -> 122 us, 5.5 TB/s, and 103 -> 98, where shrink also waits for the previous pass's writes).  A large copy moves 4.9 TB/s.  With B_i read again for every 64 rows expand
 // took 639 us; non-temporal loads and stores cost 2 to 15 %.
 #include "td_common.h"
 #include <algorithm>
@@ -397,8 +397,8 @@ __global__ __launch_bounds__(256, RJ <= 8 ? 2 : 1) void lora_expand_kernel(const
 
 // Both steps in one launch, for a few rows: every workgroup of 256 columns forms the tile's S itself, its 8 waves splitting K, and
 // the first four expand.  A_i is read once per workgroup (from L2), which pays while there are few of them.  One row, K = N =
-// 4096, rank 16: 8.8 us a call instead of 12.2 (a second launch costs the host 3 us); replayed from a graph, where launches are
-// cheap, 6.4 instead of 5.9.
+// 4096, rank 16: 8.0 us a call instead of 11.8 (a second launch costs the host 3 us); replayed from a graph, where launches are
+// cheap, 6.9 instead of 6.2.
 template <int DT, int RJ>
 __global__ __launch_bounds__(512) void lora_few_kernel(const LoraParams p) {
   constexpr int RS = 16 * RJ, KK = (RJ + 1) / 2, W = 8;
