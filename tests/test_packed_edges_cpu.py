@@ -89,3 +89,17 @@ def test_a_table_for_both_kernels_is_refused():
     counts, strides = (ctypes.c_int64 * 6)(1, 1, 0, 0, 2, 2), (ctypes.c_int64 * 8)(*[128, 64] * 4)
     with pytest.raises(L.TurboDiffusionAMDError, match="counts"):
         L.call("td_attn_packed", 4096, 8192, 16384, 32768, strides, L.TD_BF16, 2, 2, 64, 1.0, 0, None, 0, 4096, counts, None, None)
+
+
+@pytest.mark.parametrize("n,buckets,max_dist", [(5, 64, 10), (8, 32, 8), (16, 64, 16), (40, 32, 128), (300, 32, 128)])
+def test_buckets_that_widen_nowhere(n, buckets, max_dist):
+    """as many single distances as max_dist or more: the encoder's table for prompts shorter than that is one bucket a distance"""
+    from turbodiffusion_amd.text_encoder import relative_buckets
+    got, half = relative_buckets(n, buckets, max_dist, "cpu"), buckets // 2
+    rel = torch.arange(n)[None, :] - torch.arange(n)[:, None]
+    near = rel.abs() < half // 2
+    assert torch.equal(got[near], (rel.abs() + half * (rel > 0))[near])
+    if max_dist <= half // 2:
+        assert near.all()
+        with pytest.raises(ValueError, match="widen"):
+            packed.relative_bias(torch.zeros(buckets, 2), max_dist)          # its table ends at max_dist, where buckets would differ

@@ -210,8 +210,6 @@ def distance_buckets(rel, num_buckets, max_dist, bidirectional=True):
     keys share bucket 0 and earlier ones have all buckets."""
     nb = num_buckets // 2 if bidirectional else num_buckets
     exact = nb // 2
-    if exact < 1 or max_dist <= exact:
-        raise ValueError(f"{num_buckets} buckets up to distance {max_dist} leave none to widen")
     if bidirectional:
         out = (rel > 0).long() * nb
         rel = rel.abs()
@@ -229,6 +227,9 @@ def relative_bias(table, max_dist=128, bidirectional=True):
     per layer."""
     if table.dim() != 2:
         raise ValueError(f"relative_bias: table is {tuple(table.shape)}, wanted [buckets, heads]")
+    exact = table.shape[0] // (4 if bidirectional else 2)
+    if exact < 1 or max_dist <= exact:
+        raise ValueError(f"relative_bias: {table.shape[0]} buckets up to distance {max_dist} leave none to widen")
     rel = torch.arange(-max_dist, max_dist + 1, device=table.device)
     return table.detach().float()[distance_buckets(rel, table.shape[0], max_dist, bidirectional)].t().contiguous()
 
